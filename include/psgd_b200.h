@@ -414,6 +414,77 @@ int psgd_permute(const PsgdPermuteItem* items, const uint32_t* work, int nwork, 
 int psgd_apply_noalloc(void* param, int param_bf16, const float* pg, long long numel, float lr_params,
                        float max_avg_amp, float max_elem_amp, cudaStream_t stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Operators of the model that is trained (no counterpart in the reference). Element types: PSGD_F32 / BF16 / F16;
+ * arithmetic, statistics and sums are fp32. */
+#define PSGD_F32 0
+#define PSGD_BF16 1
+#define PSGD_F16 2
+
+/* Dropout with a counter-based mask: out = [residual +] (kept ? x * scale : 0) over n elements. Element i is kept when
+ * 16-bit field i % 8 (low halves first) of the Philox4x32-10 output for counter (i / 8, offset), each as two 32-bit words,
+ * and key seed is at least threshold (= round(65536 p), at most 65536). rng: two values (seed, offset) in device memory
+ * instead of the two fields, or NULL. out may be x or residual. */
+typedef struct PsgdDropout {
+  const void* x; const void* residual; void* out;
+  long long n;
+  int dtype; unsigned threshold; float scale;
+  unsigned long long seed, offset;
+  const long long* rng;
+} PsgdDropout;
+int psgd_dropout(const PsgdDropout* d, cudaStream_t stream);
+
+/* The joint between two blocks, per row of d elements (d <= PSGD_JOINT_MAX_D):
+ *   u = post ? norm(y; post_weight, post_bias) : y;  out = x + scale * gate * dropout(u);  normed = norm(out; weight, bias)
+ * kind PSGD_NORM_RMS (no mean, biases ignored) or PSGD_NORM_LAYER. weight / bias / post_weight / post_bias: d values of
+ * param_dtype, or NULL (ones / zeros). gate: `gates` rows of d values, each serving rows / gates consecutive rows, or
+ * NULL. stats: four fp32 values a row (mean and 1 / deviation of post, then of the second norm), 16-byte aligned.
+ * Dropout as in PsgdDropout (threshold 0: none), element index row * d + column, keep_scale on the kept values.
+ * x and y (and d_out, d_normed) have row strides ld_* in elements; every other matrix is contiguous.
+ * Backward: x holds the forward pass's out; d_out / d_normed may be NULL (zero); writes dx, dy, dweight and, where the
+ * forward pass has them, dbias (layer), dpost_weight, dpost_bias (post, layer), dgate. Sums over rows have a fixed order.
+ * The workspace of psgd_joint_workspace(j) bytes is 16-byte aligned. rows = 0 launches nothing. */
+#define PSGD_NORM_RMS 0
+#define PSGD_NORM_LAYER 1
+#define PSGD_JOINT_MAX_D 8192
+typedef struct PsgdJoint {
+  const void* x; const void* y; void* out; void* normed; float* stats;
+  const void* weight; const void* bias; const void* post_weight; const void* post_bias; const void* gate;
+  const void* d_out; const void* d_normed; void* dx; void* dy;
+  void* dweight; void* dbias; void* dpost_weight; void* dpost_bias; void* dgate;
+  long long ld_x, ld_y, ld_d_out, ld_d_normed, rows, gates;
+  int d, dtype, param_dtype, kind, post;
+  float scale, eps;
+  unsigned threshold; float keep_scale;
+  unsigned long long seed, offset;
+  const long long* rng;
+} PsgdJoint;
+int psgd_joint_forward(const PsgdJoint* j, cudaStream_t stream);
+long long psgd_joint_workspace(const PsgdJoint* j);
+int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cudaStream_t stream);
+
+/* Softmax cross entropy of a linear head: logits h w^T (h: n rows of d, w: v rows of d, row strides ld_h, ld_w), target
+ * n values; rows whose target is ignore_index count nothing (no value of theirs enters any result; an out-of-range
+ * target sets PSGD_ERR_BAD_TARGET and counts nothing either). With lse = log sum exp of a row's logits l:
+ *   loss = (1 - label_smoothing) (lse - l_target) + label_smoothing (lse - mean l) + z_loss lse^2
+ * reduction PSGD_REDUCE_NONE (loss: n values, 0 where ignored), _MEAN over the counted rows (0 when there is none) or
+ * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type, for the upstream
+ * gradient grad (n values for _NONE, one otherwise; NULL: ones). Tokens are taken in pieces of at most piece_bytes of
+ * kept exponentials (and at least 128 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned. */
+#define PSGD_REDUCE_NONE 0
+#define PSGD_REDUCE_MEAN 1
+#define PSGD_REDUCE_SUM 2
+#define PSGD_ERR_BAD_TARGET 32
+typedef struct PsgdLce {
+  const void* h; const void* w; const long long* target; const float* grad;
+  float* loss; void* dh; void* dw; void* workspace;
+  long long ld_h, ld_w, ignore_index, workspace_bytes, piece_bytes;
+  int n, d, v, dtype, reduction, grads;
+  float label_smoothing, z_loss;
+} PsgdLce;
+long long psgd_lce_workspace(const PsgdLce* a);
+int psgd_lce(const PsgdLce* a, int* dev_err, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -10,6 +10,7 @@ LIB_PATH = os.environ.get("PSGD_B200_LIB") or os.path.join(_HERE, "_lib", "libps
 
 c_vp, c_ll, c_int, c_float = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_float
 c_fp = ctypes.POINTER(ctypes.c_float)
+c_uint, c_ull = ctypes.c_uint, ctypes.c_ulonglong
 
 ERRORS = {-1: "invalid argument (shape, stride, alignment or mode)", -2: "CUDA launch failed",
           -3: "TMA descriptor encoding failed", -4: "caller table or workspace too small",
@@ -110,6 +111,36 @@ class PermuteItem(ctypes.Structure):
                 ("out_lo", c_vp), ("ld_out", c_ll), ("out_f32", c_vp), ("row_sq", c_vp), ("part", c_vp)]
 
 
+class Dropout(ctypes.Structure):
+    """Mirror of PsgdDropout."""
+    _fields_ = [("x", c_vp), ("residual", c_vp), ("out", c_vp), ("n", c_ll), ("dtype", c_int), ("threshold", c_uint),
+                ("scale", c_float), ("seed", c_ull), ("offset", c_ull), ("rng", c_vp)]
+
+
+class Joint(ctypes.Structure):
+    """Mirror of PsgdJoint."""
+    _fields_ = [("x", c_vp), ("y", c_vp), ("out", c_vp), ("normed", c_vp), ("stats", c_vp), ("weight", c_vp),
+                ("bias", c_vp), ("post_weight", c_vp), ("post_bias", c_vp), ("gate", c_vp), ("d_out", c_vp),
+                ("d_normed", c_vp), ("dx", c_vp), ("dy", c_vp), ("dweight", c_vp), ("dbias", c_vp),
+                ("dpost_weight", c_vp), ("dpost_bias", c_vp), ("dgate", c_vp), ("ld_x", c_ll), ("ld_y", c_ll),
+                ("ld_d_out", c_ll), ("ld_d_normed", c_ll), ("rows", c_ll), ("gates", c_ll), ("d", c_int),
+                ("dtype", c_int), ("param_dtype", c_int), ("kind", c_int), ("post", c_int), ("scale", c_float),
+                ("eps", c_float), ("threshold", c_uint), ("keep_scale", c_float), ("seed", c_ull), ("offset", c_ull),
+                ("rng", c_vp)]
+
+
+class Lce(ctypes.Structure):
+    """Mirror of PsgdLce."""
+    _fields_ = [("h", c_vp), ("w", c_vp), ("target", c_vp), ("grad", c_vp), ("loss", c_vp), ("dh", c_vp), ("dw", c_vp),
+                ("workspace", c_vp), ("ld_h", c_ll), ("ld_w", c_ll), ("ignore_index", c_ll), ("workspace_bytes", c_ll),
+                ("piece_bytes", c_ll), ("n", c_int), ("d", c_int), ("v", c_int), ("dtype", c_int),
+                ("reduction", c_int), ("grads", c_int), ("label_smoothing", c_float), ("z_loss", c_float)]
+
+
+PSGD_F32, PSGD_BF16, PSGD_F16 = 0, 1, 2
+PSGD_NORM_RMS, PSGD_NORM_LAYER = 0, 1
+PSGD_REDUCE_NONE, PSGD_REDUCE_MEAN, PSGD_REDUCE_SUM = 0, 1, 2
+JOINT_MAX_D = 8192
 PSGD_PREP_NORMAL, PSGD_PREP_TRANS, PSGD_PREP_DIRECT = 0, 1, 2
 PREP_ROWS = 8
 ROT_ROWS = 8
@@ -150,12 +181,19 @@ SIGNATURES = [
     ("psgd_set_wait_limit_ns", ctypes.c_ulonglong, [ctypes.c_ulonglong]),
     ("psgd_wait_probe", c_int, [c_vp, ctypes.c_ulonglong, c_vp]),
     ("psgd_permute", c_int, [c_vp, c_vp, c_int, c_vp, c_vp]),
+    ("psgd_dropout", c_int, [ctypes.POINTER(Dropout), c_vp]),
+    ("psgd_joint_forward", c_int, [ctypes.POINTER(Joint), c_vp]),
+    ("psgd_joint_workspace", c_ll, [ctypes.POINTER(Joint)]),
+    ("psgd_joint_backward", c_int, [ctypes.POINTER(Joint), c_vp, c_ll, c_vp]),
+    ("psgd_lce_workspace", c_ll, [ctypes.POINTER(Lce)]),
+    ("psgd_lce", c_int, [ctypes.POINTER(Lce), c_vp, c_vp]),
 ]
 
 # device error word bits (include/psgd_b200.h PSGD_ERR_*)
 ERR_BITS = {1: "a wait for a TMA stage gave up", 2: "a wait for a free stage gave up",
             4: "a wait on an accumulator handoff gave up", 8: "a descriptor failed a device-side check",
-            16: "a factor's L or the Procrustes step came out NaN or infinite"}
+            16: "a factor's L or the Procrustes step came out NaN or infinite",
+            32: "a target of the cross entropy is neither a class nor the ignored value"}
 
 
 def describe_err(v):
@@ -163,7 +201,7 @@ def describe_err(v):
 
 # the structs in the order psgd_struct_sizes reports them
 STRUCTS = [GemmSpec, PrepItem, NlbPrepItem, FactorItem, SkewItem, RotItem, TraceItem, ApplyItem, BalanceFactor,
-           BalanceParam, SymItem, NlbFinishItem, PermuteItem]
+           BalanceParam, SymItem, NlbFinishItem, PermuteItem, Dropout, Joint, Lce]
 
 
 def _check_layout(L):

@@ -19,6 +19,7 @@ enum : int {
   ERR_TIMEOUT_ACC = 4,      // epilogue / MMA waited too long on an accumulator handoff
   ERR_BAD_DESC = 8,         // a descriptor failed a device-side sanity check
   ERR_NONFINITE = 16,       // a factor's L, step size or norm bound came out NaN or infinite
+  ERR_BAD_TARGET = 32,      // a target of the cross entropy is neither a class nor the ignored value
 };
 
 // A wait gives up after this many nanoseconds of %globaltimer; legitimate waits are microseconds.

@@ -1,0 +1,116 @@
+// Elements of the model-side operators (fp32, bf16 or fp16 in memory, fp32 in registers) and the 16-bit fields of the
+// counter-based generator that dropout compares.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "philox.cuh"
+#include "psgd_b200.h"
+
+namespace psgd {
+
+template <typename T> __host__ __device__ constexpr bool is_half() { return false; }
+template <> __host__ __device__ constexpr bool is_half<__half>() { return true; }
+
+PSGD_DEVI float to_f32(float v) { return v; }
+PSGD_DEVI float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+PSGD_DEVI float to_f32(__half v) { return __half2float(v); }
+template <typename T> PSGD_DEVI T from_f32(float v);
+template <> PSGD_DEVI float from_f32<float>(float v) { return v; }
+template <> PSGD_DEVI __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> PSGD_DEVI __half from_f32<__half>(float v) { return __float2half_rn(v); }
+
+PSGD_DEVI float2 unpack2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+PSGD_DEVI float2 unpack2(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+PSGD_DEVI uint32_t pack2(float a, float b, __nv_bfloat16) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+PSGD_DEVI uint32_t pack2(float a, float b, __half) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// V consecutive elements (V = 8: 16-byte aligned vectors; V = 1: any address).
+template <typename T, int V>
+PSGD_DEVI void load_vec(const T* __restrict__ p, float* v) {
+  if constexpr (V == 1) {
+    v[0] = to_f32(*p);
+  } else if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+  } else {
+    const uint4 a = *reinterpret_cast<const uint4*>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2(w[i], T());
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T, int V>
+PSGD_DEVI void store_vec(T* p, const float* v) {
+  if constexpr (V == 1) {
+    *p = from_f32<T>(v[0]);
+  } else if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  } else {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()), pack2(v[4], v[5], T()),
+                                              pack2(v[6], v[7], T()));
+  }
+}
+
+// One element of a parameter vector whose type is known at run time (PSGD_F32 / PSGD_BF16 / PSGD_F16).
+PSGD_DEVI float load_any(const void* p, int dtype, long long i) {
+  if (dtype == PSGD_F32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == PSGD_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return __half2float(reinterpret_cast<const __half*>(p)[i]);
+}
+PSGD_DEVI void store_any(void* p, int dtype, long long i, float v) {
+  if (dtype == PSGD_F32) reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == PSGD_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
+}
+
+// Which elements dropout keeps: element i of a tensor (in its row-major order) belongs to block i / 8 of the generator's
+// sequence `offset` under key `seed`, and is kept when 16-bit field i % 8 of that block's four words (low half first) is
+// at least the threshold T = round(65536 p). Sixteen bits an element halve the generator's work against one word an
+// element; the kept values are scaled by 1 / (1 - T / 65536), the inverse of the probability that is really used.
+struct Keep {
+  uint32_t o0, o1, threshold;
+  PhiloxKeys keys;
+  PSGD_DEVI Keep(unsigned long long seed, unsigned long long offset, const long long* rng, uint32_t t) : threshold(t) {
+    if (rng) {
+      seed = (unsigned long long)rng[0];
+      offset = (unsigned long long)rng[1];
+    }
+    keys = philox_keys((uint32_t)seed, (uint32_t)(seed >> 32));
+    o0 = (uint32_t)offset;
+    o1 = (uint32_t)(offset >> 32);
+  }
+  PSGD_DEVI uint4 block(unsigned long long b) const {
+    return philox4x32_10(make_uint4((uint32_t)b, (uint32_t)(b >> 32), o0, o1), keys);
+  }
+  // bit f: field f of the block is kept
+  PSGD_DEVI uint32_t mask8(unsigned long long b) const {
+    const uint4 r = block(b);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m |= ((w[i] & 0xFFFFu) >= threshold ? 1u : 0u) << (2 * i);
+      m |= ((w[i] >> 16) >= threshold ? 1u : 0u) << (2 * i + 1);
+    }
+    return m;
+  }
+  PSGD_DEVI bool one(unsigned long long i) const { return (mask8(i >> 3) >> (i & 7)) & 1u; }
+};
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace psgd

@@ -56,7 +56,10 @@ class _ErrorWords:
                                "(a bounded wait gave up); the results of the calls since are not valid")
 
     def pending(self, dev):
-        """Raises when an earlier call's copy of the word has landed and is nonzero (no waiting)."""
+        """Raises when an earlier call's copy of the word has landed and is nonzero (no waiting; not while the stream is
+        captured, when events cannot be asked)."""
+        if torch.cuda.is_current_stream_capturing():
+            return
         k = dev.index if dev.index is not None else torch.cuda.current_device()
         ev = self.event.get(k)
         if ev is not None and ev.query():
