@@ -437,7 +437,7 @@ int psgd_dropout(const PsgdDropout* d, cudaStream_t stream);
 /* The joint between two blocks, per row of d elements (d <= PSGD_JOINT_MAX_D):
  *   u = post ? norm(y; post_weight, post_bias) : y;  out = x + scale * gate * dropout(u);  normed = norm(out; weight, bias)
  * kind PSGD_NORM_RMS (no mean, biases ignored) or PSGD_NORM_LAYER. weight / bias / post_weight / post_bias: d values of
- * param_dtype, or NULL (ones / zeros). gate: `gates` rows of d values, each serving rows / gates consecutive rows, or
+ * param_dtype (PSGD_F32 or dtype), or NULL (ones / zeros). gate: `gates` rows of d values, each serving rows / gates consecutive rows, or
  * NULL. stats: four fp32 values a row (mean and 1 / deviation of post, then of the second norm), 16-byte aligned.
  * Dropout as in PsgdDropout (threshold 0: none), element index row * d + column, keep_scale on the kept values.
  * x and y (and d_out, d_normed) have row strides ld_* in elements; every other matrix is contiguous.
@@ -470,7 +470,8 @@ int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cu
  * reduction PSGD_REDUCE_NONE (loss: n values, 0 where ignored), _MEAN over the counted rows (0 when there is none) or
  * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type, for the upstream
  * gradient grad (n values for _NONE, one otherwise; NULL: ones). Tokens are taken in pieces of at most piece_bytes of
- * kept exponentials (and at least 128 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned. */
+ * kept exponentials (and at least 128 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
+ * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong. */
 #define PSGD_REDUCE_NONE 0
 #define PSGD_REDUCE_MEAN 1
 #define PSGD_REDUCE_SUM 2

@@ -301,6 +301,11 @@ PSGD_DEVI void named_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
+// Programmatic dependent launch: lets the next launch of the stream start its blocks, and waits for the one before (all
+// of it, and with it everything earlier). Without the launch attribute both do nothing.
+PSGD_DEVI void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+PSGD_DEVI void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 PSGD_DEVI float warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);

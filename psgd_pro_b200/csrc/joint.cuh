@@ -1,0 +1,846 @@
+// The joint between two blocks of a network, one pass over its rows (d elements each):
+//   u = post(y) (a norm, or y itself), k = dropout(u), out = x + scale * gate * k, normed = pre(out)
+// and its backward pass. rms norm: a / sqrt(mean a^2 + eps) * weight; layer norm: (a - mean) / sqrt(var + eps) * weight
+// + bias. statistics: (mean, 1 / deviation) of post, then of pre, per row.
+//
+// Both passes are bound by memory traffic (a row in and out once) as long as the arithmetic stays out of its way: about
+// 100 instructions per thread for 8 elements are what the SMs can issue in the time that the copies take. So
+// arithmetic goes two elements to an instruction (f32x2), everything a call does not have is compiled out, and what is
+// constant along a column is kept out of the rows' loop. The rows to come are copied to shared memory asynchronously,
+// each thread its own 16-byte pieces (which therefore need no barrier).
+//
+// A row belongs to a group of `tpr` threads (whole warps) and a thread to 8 * NV elements of it: with VEC (16-byte
+// aligned rows) vectors of 8 neighbours, tpr vectors apart; otherwise single elements, tpr apart. A block holds
+// blockDim.y groups, each with rows of its own, whose threads meet at a named barrier of the group.
+#pragma once
+#include "elem.cuh"
+
+namespace psgd {
+
+constexpr int JOINT_MAX_D = PSGD_JOINT_MAX_D;
+constexpr int JOINT_MAX_GROUPS = 8;  // of a block
+constexpr int JOINT_MAX_THREADS = 512;
+// Kernels by the elements that a thread has of a row and the threads of a block: 8 (rows of up to 256 elements, a warp
+// each), 16 (up to 4096, 256 threads), 16 (beyond, 512 threads, whose registers no longer hold a layer norm's sums).
+enum JointWidth { W8 = 0, W16 = 1, W16_512 = 2 };
+PSGD_HD constexpr int width_nv(int w) { return w == W8 ? 1 : 2; }
+PSGD_HD constexpr int width_threads(int w) { return w == W16_512 ? 512 : 256; }
+
+// How rows are dealt out to blocks: consecutive ones, `per_block` each. With a gate a block holds whole gate groups
+// (chunks = 0: a group of threads takes a gate group at a time and writes its gradient itself) or a chunk of one gate
+// group (`chunks` to a gate group). A group of threads takes every blockDim.y-th row (gate group) of its block.
+struct JointPlan {
+  int blocks, per_block, chunks, per_gate;
+  int tpr, groups, vec, nv, wide, stages, smem;
+  int slot[5];  // of dweight, dbias, dpost_weight, dpost_bias, dgate in `part` [slot][block][d up to 8], or -1
+  int slots;
+};
+
+int joint_forward_f32(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream);
+int joint_forward_bf16(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream);
+int joint_forward_f16(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream);
+int joint_backward_f32(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
+int joint_backward_bf16(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
+int joint_backward_f16(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
+
+// Dynamic shared memory beyond the 48 KB that dynamic and static shared memory have without asking. A refusal is cleared:
+// it would be taken for the next launch's.
+template <typename K>
+int joint_allow_smem(K kernel, int smem) {
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    cudaGetLastError();
+    return PSGD_ELAUNCH;
+  }
+  return PSGD_OK;
+}
+
+// ---- two fp32 values in one register pair -----------------------------------------------------------------------------
+struct F2 {
+  unsigned long long v;
+};
+PSGD_DEVI F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
+}
+PSGD_DEVI F2 f2(float a) { return f2(a, a); }
+PSGD_DEVI float2 un2(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+PSGD_DEVI F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+PSGD_DEVI F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+PSGD_DEVI F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+PSGD_DEVI float sum2(F2 a) {
+  const float2 f = un2(a);
+  return f.x + f.y;
+}
+
+// Eight elements as four pairs.
+template <typename T>
+PSGD_DEVI void unpack8(uint4 a, F2* v) {
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2(w[i], T());
+    v[i] = f2(f.x, f.y);
+  }
+}
+template <typename T>
+PSGD_DEVI void load8(const T* p, F2* v) {
+  if constexpr (sizeof(T) == 4) {
+    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+    v[0] = f2(a.x, a.y), v[1] = f2(a.z, a.w), v[2] = f2(b.x, b.y), v[3] = f2(b.z, b.w);
+  } else {
+    unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
+  }
+}
+template <typename T>
+PSGD_DEVI void store8(T* p, const F2* v) {
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 a = un2(v[i]);
+    f[2 * i] = a.x, f[2 * i + 1] = a.y;
+  }
+  store_vec<T, 8>(p, f);
+}
+
+// The elements of a row that are this thread's: vector i is at e(i) (VEC), or its elements at e(i), e(i) + tpr, ...
+template <bool VEC>
+struct Place {
+  int d, tpr, t;
+  PSGD_DEVI Place(int d_) : d(d_), tpr(blockDim.x), t(threadIdx.x) {}
+  PSGD_DEVI int e(int i) const { return VEC ? (i * tpr + t) * 8 : i * 8 * tpr + t; }
+  PSGD_DEVI bool any(int i) const { return e(i) < d; }
+  PSGD_DEVI int at(int i, int k) const { return VEC ? e(i) + k : e(i) + k * tpr; }
+  PSGD_DEVI bool has(int i, int k) const { return VEC ? any(i) : at(i, k) < d; }
+  template <typename T>
+  PSGD_DEVI void load(const T* row, int i, F2* v) const {
+    if constexpr (VEC) {
+      if (any(i)) {
+        load8<T>(row + e(i), v);
+        return;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
+    } else {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = has(i, k) ? to_f32(row[at(i, k)]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = f2(f[2 * k], f[2 * k + 1]);
+    }
+  }
+  template <typename T>
+  PSGD_DEVI void store(T* row, int i, const F2* v) const {
+    if constexpr (VEC) {
+      if (any(i)) store8<T>(row + e(i), v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = un2(v[k]);
+        if (has(i, 2 * k)) row[at(i, 2 * k)] = from_f32<T>(f.x);
+        if (has(i, 2 * k + 1)) row[at(i, 2 * k + 1)] = from_f32<T>(f.y);
+      }
+    }
+  }
+  // A parameter vector of fp32 or of T, `otherwise` where there is none.
+  template <typename T>
+  PSGD_DEVI void param(const void* p, int dtype, float otherwise, int i, F2* v) const {
+    if (!p) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = f2(otherwise);
+    } else if (dtype == PSGD_F32) {
+      load(reinterpret_cast<const float*>(p), i, v);
+    } else {
+      load(reinterpret_cast<const T*>(p), i, v);
+    }
+  }
+  // Bit k: element k is kept by dropout.
+  PSGD_DEVI uint32_t kept(const Keep& keep, long long row, int i) const {
+    const unsigned long long at0 = (unsigned long long)row * d;
+    if constexpr (VEC) {
+      return keep.mask8((at0 + e(i)) >> 3);
+    } else {
+      uint32_t m = 0;
+#pragma unroll 1
+      for (int k = 0; k < 8; ++k)
+        if (has(i, k)) m |= (uint32_t)keep.one(at0 + at(i, k)) << k;
+      return m;
+    }
+  }
+};
+PSGD_DEVI F2 select2(F2 a, uint32_t mask, int k) {  // elements k, k + 1 of 8, zero where dropped
+  const float2 f = un2(a);
+  return f2((mask >> k) & 1u ? f.x : 0.f, (mask >> (k + 1)) & 1u ? f.y : 0.f);
+}
+
+// Sum of v[0..N) over the threads of a group of at most WARPS warps. `red` holds two buffers taken in turn: a thread writes
+// one again only after the barrier of the other's sum, which every thread reaches after its reads of the first. The
+// places of warps that are not there stay zero.
+template <int N, int WARPS>
+struct GroupSum {
+  static constexpr int FLOATS = 2 * JOINT_MAX_GROUPS * WARPS * N;
+  float* at;
+  int tpr, turn;
+  PSGD_DEVI GroupSum(float* red) : at(red + threadIdx.y * (WARPS * N)), tpr(blockDim.x), turn(0) {
+    if (tpr == 32) return;
+    for (int i = threadIdx.y * blockDim.x + threadIdx.x; i < FLOATS; i += blockDim.x * blockDim.y) red[i] = 0.f;
+    __syncthreads();
+  }
+  PSGD_DEVI void operator()(float* v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[k] += __shfl_xor_sync(0xffffffffu, v[k], o);
+    if (tpr == 32) return;
+    float* to = at + turn;
+    turn ^= JOINT_MAX_GROUPS * WARPS * N;
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+      for (int k = 0; k < N; ++k) to[k * WARPS + (threadIdx.x >> 5)] = v[k];
+    named_sync(1 + threadIdx.y, tpr);
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      v[k] = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; w += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(to + k * WARPS + w);
+        v[k] += (b.x + b.y) + (b.z + b.w);
+      }
+    }
+  }
+};
+
+// ---- the rows to come -------------------------------------------------------------------------------------------------
+// A ring of `stages` rows' pieces, ARR arrays each, in shared memory: this thread's 16-byte pieces, a block's threads
+// side by side (no bank conflicts). fetch() starts a row's copies (null arrays are skipped, and stay zero where they
+// were cleared), wait() waits for the oldest row, read() unpacks a piece of it.
+template <typename T, int NV, int ARR>
+struct Ring16 {
+  static constexpr int H = sizeof(T) / 2;  // 16-byte pieces to 8 elements
+  uint32_t base, apart, stage, all, put, get;  // bytes: first piece, from piece to piece, of a stage, of the ring; turns
+  int stages;
+  PSGD_DEVI Ring16(void* smem, int s) : put(0), get(0), stages(s) {
+    apart = blockDim.x * blockDim.y * 16;
+    stage = apart * (ARR * NV * H);
+    all = stage * s;
+    base = smem_u32(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+  }
+  PSGD_DEVI void fetch(const Place<true>& at, const T* const* rows, bool there) {
+    if (there)
+#pragma unroll
+      for (int a = 0; a < ARR; ++a)
+        if (rows[a])
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+            if (at.any(i))
+#pragma unroll
+              for (int h = 0; h < H; ++h)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
+                             ::"r"(base + put + apart * ((a * NV + i) * H + h)),
+                             "l"(reinterpret_cast<const uint4*>(rows[a] + at.e(i)) + h)
+                             : "memory");
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put += stage;
+    if (put == all) put = 0;
+  }
+  PSGD_DEVI void wait() {  // one group was committed for each of the stages - 1 rows after the oldest
+    if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+  }
+  PSGD_DEVI void read(const Place<true>& at, int a, int i, F2* v) const {
+    if (at.any(i)) {
+#pragma unroll
+      for (int h = 0; h < H; ++h) {
+        uint4 x;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                     : "r"(base + get + apart * ((a * NV + i) * H + h))
+                     : "memory");
+        if constexpr (H == 2) {
+          v[2 * h] = f2(__uint_as_float(x.x), __uint_as_float(x.y));
+          v[2 * h + 1] = f2(__uint_as_float(x.z), __uint_as_float(x.w));
+        } else {
+          unpack8<T>(x, v);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
+    }
+  }
+  PSGD_DEVI void next() {
+    get += stage;
+    if (get == all) get = 0;
+  }
+};
+
+// ---- forward ----------------------------------------------------------------------------------------------------------
+constexpr int F_POST = 1, F_GATE = 2, F_LAYER = 4, F_DROP = 8, F_DIRECT = 16, F_RUNTIME = 32;
+
+// What is constant along a column is formed once: f = scale gate post_weight (and with it the post norm's bias), with the
+// gate where it has one row; other gates multiply row by row.
+template <typename T, bool VEC, int W, int F>
+__global__ void __launch_bounds__(width_threads(W), W == W8 ? 3 : 1) joint_forward_kernel(const PsgdJoint j, const JointPlan p) {
+  constexpr int NV = width_nv(W), P = NV * 4;
+  const bool post = F & F_RUNTIME ? j.post != 0 : bool(F & F_POST);
+  const bool layer = F & F_RUNTIME ? j.kind == PSGD_NORM_LAYER : bool(F & F_LAYER);
+  const bool drop = F & F_RUNTIME ? j.threshold != 0 : bool(F & F_DROP);
+  extern __shared__ uint4 smem[];
+  using Sum = GroupSum<1, width_threads(W) / 32>;
+  __shared__ __align__(16) float red[Sum::FLOATS];
+  const int d = j.d;
+  const Place<VEC> at(d);
+  Sum sum(red);
+  const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
+  const float inv_d = 1.f / (float)d;
+  const int step = gridDim.x * blockDim.y, rows_all = (int)j.rows, ld_x = (int)j.ld_x, ld_y = (int)j.ld_y;
+  const bool one_gate = j.gate && p.per_gate == rows_all, row_gate = j.gate && !one_gate;
+  Ring16<T, NV, 2> ring(smem, p.stages);
+
+  auto sources = [&](int row, const T** rows) {
+    rows[0] = reinterpret_cast<const T*>(j.x) + (long long)row * ld_x;
+    rows[1] = reinterpret_cast<const T*>(j.y) + (long long)row * ld_y;
+  };
+  int row = blockIdx.x * blockDim.y + threadIdx.y, ahead = row;
+  if constexpr (VEC) {
+    for (int s = 0; s + 1 < p.stages; ++s, ahead += step) {
+      const T* rows[2];
+      sources(ahead, rows);
+      ring.fetch(at, rows, ahead < rows_all);
+    }
+  }
+  F2 w[P], b[P], f[P], fb[P];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const F2 c = f2(j.scale * (drop ? j.keep_scale : 1.f));
+    at.template param<T>(j.weight, j.param_dtype, 1.f, i, w + i * 4);
+    if (layer) at.template param<T>(j.bias, j.param_dtype, 0.f, i, b + i * 4);
+    at.template param<T>(post ? j.post_weight : nullptr, j.param_dtype, 1.f, i, f + i * 4);
+    if (post && layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, fb + i * 4);
+    F2 g[4] = {c, c, c, c};
+    if (one_gate) {
+      at.load(reinterpret_cast<const T*>(j.gate), i, g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = mul2(g[k], c);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f[i * 4 + k] = mul2(f[i * 4 + k], g[k]);
+      if (post && layer) fb[i * 4 + k] = mul2(fb[i * 4 + k], g[k]);
+    }
+  }
+  // (mean, 1 / deviation) of a row (zero beyond d); the variance is a second pass over the registers: no cancellation
+  auto statistics = [&](const F2* a, float& mean, float& r) {
+    mean = 0.f;
+    F2 q = f2(0.f);
+    if (layer) {
+#pragma unroll
+      for (int i = 0; i < P; ++i) q = add2(q, a[i]);
+      float s = sum2(q);
+      sum(&s);
+      mean = s * inv_d;
+      q = f2(0.f);
+      const F2 m = f2(-mean);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (at.any(i))
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            F2 c = add2(a[i * 4 + k], m);
+            if (!VEC) {
+              const float2 x = un2(c);
+              c = f2(at.has(i, 2 * k) ? x.x : 0.f, at.has(i, 2 * k + 1) ? x.y : 0.f);
+            }
+            q = fma2(c, c, q);
+          }
+    } else {
+#pragma unroll
+      for (int i = 0; i < P; ++i) q = fma2(a[i], a[i], q);
+    }
+    float s = sum2(q);
+    sum(&s);
+    r = rsqrtf(s * inv_d + j.eps);
+  };
+
+  for (; row < rows_all; row += step) {
+    F2 u[P], x[P];
+    if constexpr (VEC) {
+      const T* rows[2];
+      sources(ahead, rows);
+      ring.fetch(at, rows, ahead < rows_all);
+      ahead += step;
+      ring.wait();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        ring.read(at, 0, i, x + i * 4);
+        ring.read(at, 1, i, u + i * 4);
+      }
+      ring.next();
+    } else {
+      const T* rows[2];
+      sources(row, rows);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        at.load(rows[0], i, x + i * 4);
+        at.load(rows[1], i, u + i * 4);
+      }
+    }
+    T* po = reinterpret_cast<T*>(j.out) + (long long)row * d;
+    T* pn = reinterpret_cast<T*>(j.normed) + (long long)row * d;
+    float mean_y = 0.f, r_y = 1.f, mean_o, r_o;
+    if (post) statistics(u, mean_y, r_y);
+    const F2 ry = f2(r_y), my = f2(-mean_y * r_y);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      if (!at.any(i)) continue;
+      F2* ui = u + i * 4;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (post) ui[k] = layer ? fma2(ui[k], ry, my) : mul2(ui[k], ry);
+        ui[k] = post && layer ? fma2(ui[k], f[i * 4 + k], fb[i * 4 + k]) : mul2(ui[k], f[i * 4 + k]);
+      }
+      if (row_gate) {
+        const int g = p.per_gate == 1 ? row : (int)((unsigned)row / (unsigned)p.per_gate);
+        F2 v[4];
+        at.load(reinterpret_cast<const T*>(j.gate) + (long long)g * d, i, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ui[k] = mul2(ui[k], v[k]);
+      }
+      if (drop) {
+        const uint32_t m = at.kept(keep, row, i);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) ui[k] = select2(ui[k], m, 2 * k);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i * 4 + k] = add2(x[i * 4 + k], ui[k]);
+      at.store(po, i, x + i * 4);
+    }
+    statistics(x, mean_o, r_o);
+    const F2 ro = f2(r_o), mo = f2(-mean_o * r_o);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        o[k] = layer ? fma2(x[i * 4 + k], ro, mo) : mul2(x[i * 4 + k], ro);
+        o[k] = layer ? fma2(o[k], w[i * 4 + k], b[i * 4 + k]) : mul2(o[k], w[i * 4 + k]);
+      }
+      at.store(pn, i, o);
+    }
+    if (threadIdx.x == 0) reinterpret_cast<float4*>(j.stats)[row] = make_float4(mean_y, r_y, mean_o, r_o);
+  }
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------
+// hat = (out - mean) r, dhat = d_normed w:  dx = d_out + r (dhat - hat mean(dhat hat) [- mean(dhat)]).
+// Let m be dx where dropout kept the element (0 elsewhere), c its scale times the residual scale, yh the post norm's
+// (y - mean) r (or y). Then, with f = c gate post_weight constant along a column (of a gate group):
+//   dy = f m, through the post norm as above;  A = sum m yh and B = sum m over rows give
+//   dpost_weight = c gate A, dpost_bias = c gate B, dgate = c (post_weight A + post_bias B): one multiply-add a row for
+//   three gradients. dweight = sum d_normed hat, dbias = sum d_normed.
+// The sums over rows are kept in registers and written once a block, as rows of `part`, which joint_reduce_kernel adds in
+// a fixed order.
+struct JointRows {  // a group's rows: every groups-th one, or (direct) every groups-th gate group's
+  int row, g, end, per_gate, groups;
+  bool direct;
+  PSGD_DEVI bool there() const { return direct ? g < end : row < end; }
+  PSGD_DEVI bool last_of_gate() const { return row + 1 == (g + 1) * per_gate; }
+  PSGD_DEVI void next() {
+    if (!direct) {
+      row += groups;
+    } else if (last_of_gate()) {
+      g += groups;
+      row = g * per_gate;
+    } else {
+      ++row;
+    }
+  }
+};
+
+// Blocks that an SM has to hold: three of 256 threads where what a thread keeps fits in 84 registers.
+PSGD_HD constexpr int joint_min_blocks(int w, int f) {
+  return w == W16_512 ? 1 : w == W16 ? 1 : (f & F_RUNTIME) ? 2 : (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER)) ? 2 : 3;
+}
+
+template <typename T, bool VEC, int W, int F>
+__global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
+    joint_backward_kernel(const PsgdJoint j, const JointPlan p, float* part) {
+  constexpr int NV = width_nv(W), P = NV * 4;
+  constexpr bool RT = F & F_RUNTIME;
+  const bool post = RT ? j.post != 0 : bool(F & F_POST);
+  const bool gate = RT ? j.gate != nullptr : bool(F & F_GATE);
+  const bool layer = RT ? j.kind == PSGD_NORM_LAYER : bool(F & F_LAYER);
+  const bool drop = RT ? j.threshold != 0 : bool(F & F_DROP);
+  const bool direct = RT ? gate && p.chunks == 0 : bool(F & F_DIRECT);
+  const bool use_y = post || gate;
+  extern __shared__ uint4 smem[];
+  constexpr int NS = RT || (F & F_LAYER) ? 2 : 1;
+  using Sum = GroupSum<NS, width_threads(W) / 32>;
+  __shared__ __align__(16) float red[Sum::FLOATS];
+  const int d = j.d, dp = (d + 7) & ~7;
+  const Place<VEC> at(d);
+  Sum sum(red);
+  const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
+  const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
+  Ring16<T, NV, 4> ring(smem, p.stages);
+
+  JointRows it;
+  it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
+  int gate_row = 0;  // of a block that holds (part of) one gate group
+  if (direct) {
+    const int held = p.per_block / p.per_gate, g0 = blockIdx.x * held;
+    it.g = g0 + threadIdx.y;
+    it.end = min(g0 + held, (int)j.gates);
+    it.row = it.g * p.per_gate;
+  } else if (p.chunks) {
+    gate_row = blockIdx.x / p.chunks;
+    const int r0 = gate_row * p.per_gate + (blockIdx.x - gate_row * p.chunks) * p.per_block;
+    it.row = r0 + threadIdx.y;
+    it.end = min(r0 + p.per_block, (gate_row + 1) * p.per_gate);
+    it.g = 0;
+  } else {
+    it.row = blockIdx.x * p.per_block + threadIdx.y;
+    it.end = (int)min((blockIdx.x + 1LL) * p.per_block, j.rows);
+    it.g = 0;
+  }
+
+  // f, per column, of a gate group
+  auto column_factor = [&](int g, int i, F2* f) {
+    if (post) at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, f);
+    else
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = f2(1.f);
+    if (gate) {
+      F2 v[4];
+      at.load(reinterpret_cast<const T*>(j.gate) + (long long)g * d, i, v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = mul2(f[k], v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = mul2(f[k], f2(c));
+  };
+  const int ld_dn = (int)j.ld_d_normed, ld_do = (int)j.ld_d_out, ld_x = (int)j.ld_x, ld_y = (int)j.ld_y;
+  auto sources = [&](long long row, const T** rows) {
+    rows[0] = j.d_normed ? reinterpret_cast<const T*>(j.d_normed) + row * ld_dn : nullptr;
+    rows[1] = j.d_out ? reinterpret_cast<const T*>(j.d_out) + row * ld_do : nullptr;
+    rows[2] = reinterpret_cast<const T*>(j.x) + row * ld_x;
+    rows[3] = use_y ? reinterpret_cast<const T*>(j.y) + row * ld_y : nullptr;
+  };
+
+  F2 dw[P], db[P], A[P], B[P], dpw[P], dpb[P], w[P], f[P];
+#pragma unroll
+  for (int k = 0; k < P; ++k) dw[k] = db[k] = A[k] = B[k] = dpw[k] = dpb[k] = f2(0.f);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    at.template param<T>(j.weight, j.param_dtype, 1.f, i, w + i * 4);
+    if (!direct) column_factor(gate_row, i, f + i * 4);
+  }
+
+  JointRows ahead = it;
+  if constexpr (VEC) {
+    for (int s = 0; s + 1 < p.stages; ++s) {
+      const T* rows[4];
+      const bool there = ahead.there();
+      sources(ahead.row, rows);
+      ring.fetch(at, rows, there);
+      if (there) ahead.next();
+    }
+  }
+  bool fresh = true;  // the gate group's factor is to be formed
+  for (; it.there(); it.next()) {
+    const int row = it.row;
+    const float4 st = reinterpret_cast<const float4*>(j.stats)[row];
+    F2 dn[P], hat[P], dx[P], y[P];
+    if constexpr (VEC) {
+      const T* rows[4];
+      const bool there = ahead.there();
+      sources(ahead.row, rows);
+      ring.fetch(at, rows, there);
+      if (there) ahead.next();
+      ring.wait();
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (j.d_normed) ring.read(at, 0, i, dn + i * 4);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dn[i * 4 + k] = f2(0.f);
+        ring.read(at, 2, i, hat + i * 4);
+      }
+    } else {
+      const T* rows[4];
+      sources(row, rows);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        at.load(rows[2], i, hat + i * 4);
+        if (rows[0]) at.load(rows[0], i, dn + i * 4);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dn[i * 4 + k] = f2(0.f);
+        if (rows[1]) at.load(rows[1], i, dx + i * 4);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dx[i * 4 + k] = f2(0.f);
+        if (use_y) at.load(rows[3], i, y + i * 4);
+      }
+    }
+    F2 s0 = f2(0.f), s1 = f2(0.f);
+    {
+      const F2 r = f2(st.w), m = f2(-st.z * st.w);
+#pragma unroll
+      for (int k = 0; k < P; ++k) {
+        hat[k] = layer ? fma2(hat[k], r, m) : mul2(hat[k], r);
+        dw[k] = fma2(dn[k], hat[k], dw[k]);
+        if (layer) db[k] = add2(db[k], dn[k]);
+        dn[k] = mul2(dn[k], w[k]);
+        s0 = fma2(dn[k], hat[k], s0);
+        if (layer) s1 = add2(s1, dn[k]);
+      }
+    }
+    float s[2] = {sum2(s0), sum2(s1)};
+    sum(s);
+    if constexpr (VEC) {  // (read after the sum: what waits in shared memory needs no registers)
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (j.d_out) ring.read(at, 1, i, dx + i * 4);
+        else
+#pragma unroll
+          for (int k = 0; k < 4; ++k) dx[i * 4 + k] = f2(0.f);
+        if (use_y) ring.read(at, 3, i, y + i * 4);
+      }
+      ring.next();
+    }
+    if (direct && fresh) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) column_factor(it.g, i, f + i * 4);
+    }
+    const F2 r = f2(st.w), c1 = f2(-s[0] * inv_d), c2 = f2(layer ? -s[1] * inv_d : 0.f);
+    const F2 ry = f2(st.y), my = f2(-st.x * st.y);
+    s0 = s1 = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      uint32_t kept = 0xFFu;
+      if (drop && at.any(i)) kept = at.kept(keep, row, i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = i * 4 + k;
+        F2 t = fma2(hat[n], c1, dn[n]);
+        if (layer) t = add2(t, c2);
+        dx[n] = fma2(r, t, dx[n]);
+      }
+      at.store(reinterpret_cast<T*>(j.dx) + (long long)row * d, i, dx + i * 4);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = i * 4 + k;
+        F2 m = drop ? select2(dx[n], kept, 2 * k) : dx[n];
+        if (!VEC) {  // beyond d, where a layer norm's dx is not zero
+          const float2 v = un2(m);
+          m = f2(at.has(i, 2 * k) ? v.x : 0.f, at.has(i, 2 * k + 1) ? v.y : 0.f);
+        } else if (!at.any(i)) {
+          m = f2(0.f);
+        }
+        if (use_y) {
+          if (post) y[n] = layer ? fma2(y[n], ry, my) : mul2(y[n], ry);
+          A[n] = fma2(m, y[n], A[n]);
+        }
+        if (post && layer) B[n] = add2(B[n], m);
+        dx[n] = mul2(m, f[n]);
+        if (post) {
+          s0 = fma2(dx[n], y[n], s0);
+          if (layer) s1 = add2(s1, dx[n]);
+        }
+      }
+      if (!post) at.store(reinterpret_cast<T*>(j.dy) + (long long)row * d, i, dx + i * 4);
+    }
+    if (post) {
+      s[0] = sum2(s0), s[1] = sum2(s1);
+      sum(s);
+      const F2 c3 = f2(-s[0] * inv_d), c4 = f2(layer ? -s[1] * inv_d : 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int n = i * 4 + k;
+          F2 t = fma2(y[n], c3, dx[n]);
+          if (layer) t = add2(t, c4);
+          dx[n] = mul2(ry, t);
+        }
+        at.store(reinterpret_cast<T*>(j.dy) + (long long)row * d, i, dx + i * 4);
+      }
+    }
+    if (direct) {
+      fresh = it.last_of_gate();
+      if (fresh) {  // the gate group ends here, and with it its gradient
+        const T* pg = reinterpret_cast<const T*>(j.gate) + (long long)it.g * d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (!at.any(i)) continue;
+          F2 g[4], pw[4], pb[4], v[4];
+          at.load(pg, i, g);
+          if (post) {
+            at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, pw);
+            if (layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, pb);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int n = i * 4 + k;
+            const F2 a = mul2(A[n], f2(c)), b = mul2(B[n], f2(c));
+            v[k] = post ? mul2(a, pw[k]) : a;
+            if (post && layer) v[k] = fma2(b, pb[k], v[k]);
+            if (post) dpw[n] = fma2(a, g[k], dpw[n]);
+            if (post && layer) dpb[n] = fma2(b, g[k], dpb[n]);
+            A[n] = B[n] = f2(0.f);
+          }
+          at.store(reinterpret_cast<T*>(j.dgate) + (long long)it.g * d, i, v);
+        }
+      }
+    }
+  }
+
+  // What this group has of the block's rows of `part`: dweight, dbias, then from A and B.
+  if (!direct) {
+    const T* pg = gate ? reinterpret_cast<const T*>(j.gate) + (long long)gate_row * d : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 g[4], pw[4], pb[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = f2(1.f);
+      if (gate) at.load(pg, i, g);
+      if (gate && post) {
+        at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, pw);
+        if (layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, pb);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = i * 4 + k;
+        const F2 a = mul2(A[n], f2(c)), b = mul2(B[n], f2(c));
+        dpw[n] = gate ? mul2(a, g[k]) : a;
+        if (layer) dpb[n] = gate ? mul2(b, g[k]) : b;
+        A[n] = post && gate ? mul2(a, pw[k]) : a;
+        if (post && gate && layer) A[n] = fma2(b, pb[k], A[n]);
+      }
+    }
+  }
+  // The groups' shares are added in their order, through shared memory (the ring is done with).
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  float* share = reinterpret_cast<float*>(smem);
+  auto write = [&](int a, const F2* v) {
+    if (p.slot[a] < 0) return;
+    if (blockDim.y > 1) {
+      __syncthreads();
+      if (threadIdx.y > 0)
+#pragma unroll
+        for (int i = 0; i < NV; ++i) at.store(share + (threadIdx.y - 1) * dp, i, v + i * 4);
+      __syncthreads();
+      if (threadIdx.y > 0) return;
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 t[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[k] = v[i * 4 + k];
+      for (int g = 1; g < (int)blockDim.y; ++g) {
+        F2 o[4];
+        at.load(share + (g - 1) * dp, i, o);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = add2(t[k], o[k]);
+      }
+      at.store(part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp, i, t);
+    }
+  };
+  write(0, dw);
+  if (layer) write(1, db);
+  if (post) write(2, dpw);
+  if (post && layer) write(3, dpb);
+  if (gate && !direct) write(4, A);
+}
+
+// ---- launches of one element type -------------------------------------------------------------------------------------
+template <typename T, bool VEC, int W, int F>
+int joint_forward_launch(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
+  auto k = joint_forward_kernel<T, VEC, W, F>;
+  if (int rc = joint_allow_smem(k, p.smem)) return rc;
+  k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p);
+  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+}
+template <typename T, bool VEC, int W, int F>
+int joint_backward_launch(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
+  auto k = joint_backward_kernel<T, VEC, W, F>;
+  if (int rc = joint_allow_smem(k, p.smem)) return rc;
+  k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p, part);
+  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+}
+
+inline int joint_flags(const PsgdJoint& j, const JointPlan& p) {
+  return (j.post ? F_POST : 0) | (j.gate ? F_GATE : 0) | (j.kind == PSGD_NORM_LAYER ? F_LAYER : 0) |
+         (j.threshold ? F_DROP : 0) | (j.gate && !p.chunks ? F_DIRECT : 0);
+}
+
+// The kernel compiled for the flags f (F and up that can occur; the forward kernels take the gate at run time).
+template <typename T, int W, int F = 0>
+int joint_forward_pick(int f, const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
+  if constexpr (F >= F_DIRECT) {
+    return PSGD_EINVAL;
+  } else {
+    if constexpr (!(F & F_GATE))
+      if (f == F) return joint_forward_launch<T, true, W, F>(j, p, stream);
+    return joint_forward_pick<T, W, F + 1>(f, j, p, stream);
+  }
+}
+template <typename T, int W, int F = 0>
+int joint_backward_pick(int f, const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
+  if constexpr (F >= F_RUNTIME) {
+    return PSGD_EINVAL;
+  } else {
+    if constexpr (!(F & F_DIRECT) || (F & F_GATE))
+      if (f == F) return joint_backward_launch<T, true, W, F>(j, p, part, stream);
+    return joint_backward_pick<T, W, F + 1>(f, j, p, part, stream);
+  }
+}
+
+template <typename T>
+int joint_forward_of(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
+  const int f = joint_flags(j, p) & ~(F_GATE | F_DIRECT);
+  switch (p.wide) {
+    case W8: return p.vec ? joint_forward_pick<T, W8>(f, j, p, stream) : joint_forward_launch<T, false, W8, F_RUNTIME>(j, p, stream);
+    case W16:
+      return p.vec ? joint_forward_pick<T, W16>(f, j, p, stream) : joint_forward_launch<T, false, W16, F_RUNTIME>(j, p, stream);
+    default:
+      return p.vec ? joint_forward_launch<T, true, W16_512, F_RUNTIME>(j, p, stream)
+                   : joint_forward_launch<T, false, W16_512, F_RUNTIME>(j, p, stream);
+  }
+}
+
+template <typename T>
+int joint_backward_of(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
+  const int f = joint_flags(j, p);
+  switch (p.wide) {
+    case W8:
+      return p.vec ? joint_backward_pick<T, W8>(f, j, p, part, stream)
+                   : joint_backward_launch<T, false, W8, F_RUNTIME>(j, p, part, stream);
+    case W16:
+      return p.vec ? joint_backward_pick<T, W16>(f, j, p, part, stream)
+                   : joint_backward_launch<T, false, W16, F_RUNTIME>(j, p, part, stream);
+    default:
+      return p.vec ? joint_backward_launch<T, true, W16_512, F_RUNTIME>(j, p, part, stream)
+                   : joint_backward_launch<T, false, W16_512, F_RUNTIME>(j, p, part, stream);
+  }
+}
+
+}  // namespace psgd

@@ -18,11 +18,12 @@
 namespace psgd {
 namespace {
 
-constexpr int LM = 128, LN = 256, LK = 64, L_STAGES = 4, L_THREADS = 192;
-constexpr int L_A_BYTES = LM * LK * 2, L_B_BYTES = LN * LK * 2, L_STAGE_BYTES = L_A_BYTES + L_B_BYTES;
-constexpr int L_SMEM = 1024 + L_STAGES * L_STAGE_BYTES + 256;
+constexpr int LM = 256, LK = 64;    // rows of a tile (two CTAs of 128), depth of a copied block
+constexpr int L_THREADS = 384;      // a warpgroup for copies and products, two on the accumulators
+// Registers a thread: 168 at launch (384 threads); 3 * 168 = 56 + 2 * 224.
+constexpr int L_REGS_LOW = 56, L_REGS_HIGH = 224;
 constexpr int L_LIMBS = 3;          // of an fp32 operand
-constexpr int L_GROUP_M = 8;        // row tiles that walk the column tiles together (L2 reuse of both operands)
+constexpr int L_GROUP_M = 4;        // row tiles that walk the column tiles together (L2 reuse of both operands)
 // Kept exponentials are fp16 of 2^15 exp(l - m), exp(l - m) in [0, 1]: 11 significant bits down to 2^-29 of the row's
 // maximum in these 256 columns, so that the one rounding to 16 bits that matters is that of g.
 constexpr float L_KEEP_SCALE = 32768.f;
@@ -35,68 +36,97 @@ struct LceState {  // device scalars of one call
   float row_unit;  // per-row upstream gradients are divided by this
 };
 
+// The error word may be pinned host memory, where atomics are not to be relied on: bits are added by a plain store (when
+// two kinds of error meet, one of them is reported).
+PSGD_DEVI void report(int* err, int bits) {
+  volatile int* w = err;
+  *w = *w | bits;
+  __threadfence_system();
+}
+
 // ---- plan ------------------------------------------------------------------------------------------------------------
-// One block: thread k owns the targets [k * per, (k + 1) * per); a scan of the threads' counts numbers the counted rows in
-// their order.
+// One block numbers the counted rows in their order. 65536 targets at a time: every warp counts its groups of 32, the
+// counts are scanned, and each row's number is its group's start plus its place in the group.
+constexpr int PLAN_GROUPS = 64;  // groups of 32 targets that a warp has at a time
 __global__ void __launch_bounds__(1024) lce_plan_kernel(const long long* __restrict__ target, int n, int v,
                                                         long long ignore, int reduction, int half,
                                                         const float* __restrict__ grad, int* __restrict__ rank,
                                                         int* __restrict__ row_of, int* __restrict__ row_target,
                                                         float* __restrict__ loss, LceState* state, int* err) {
-  __shared__ int counts[32];
+  __shared__ int count[PLAN_GROUPS * 32];
+  __shared__ int warp_total[32];
   __shared__ float tops[32];
-  const int t = threadIdx.x, lane = t & 31, warp = t >> 5, per = (n + 1023) / 1024;
-  const int a = min(n, t * per), b = min(n, a + per);
-  int mine = 0;
+  const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+  const bool none = reduction == PSGD_REDUCE_NONE;
   float top = 0.f;
   bool bad = false;
-  for (int i = a; i < b; ++i) {
-    const long long x = target[i];
-    if (x == ignore) continue;
-    if (x < 0 || x >= v) {
-      bad = true;
-      continue;
+  int total = 0;
+  pdl_trigger();
+  pdl_wait();
+  for (int base = 0; base < n; base += 1024 * PLAN_GROUPS) {
+    const int groups = min(PLAN_GROUPS, (n - base + 1023) / 1024);
+#pragma unroll 8
+    for (int g = 0; g < groups; ++g) {
+      const int i = base + g * 1024 + t;
+      const long long x = i < n ? target[i] : ignore;
+      const bool counted = x != ignore && x >= 0 && x < v;
+      bad |= x != ignore && !counted;
+      if (none && grad && counted) top = fmaxf(top, fabsf(grad[i]));
+      const uint32_t m = __ballot_sync(0xffffffffu, counted);
+      if (lane == 0) count[g * 32 + warp] = __popc(m);
     }
-    ++mine;
-    if (reduction == PSGD_REDUCE_NONE && grad) top = fmaxf(top, fabsf(grad[i]));
-  }
-  int before = mine;  // inclusive scan
+    for (int g = groups * 32 + t; g < PLAN_GROUPS * 32; g += 1024) count[g] = 0;
+    __syncthreads();
+    // exclusive scan of the 2048 counts, two to a thread
+    const int c0 = count[2 * t], c1 = count[2 * t + 1];
+    int sum = c0 + c1;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += up;
-  }
-  top = warp_max(top);
-  if (lane == 31) counts[warp] = before;
-  if (lane == 0) tops[warp] = top;
-  if (bad) atomicOr(err, ERR_BAD_TARGET);
-  __syncthreads();
-  int base = 0, total = 0;
-  for (int w = 0; w < 32; ++w) {
-    if (w < warp) base += counts[w];
-    total += counts[w];
-    top = fmaxf(top, tops[w]);
-  }
-  int r = base + before - mine;
-  for (int i = a; i < b; ++i) {
-    const long long x = target[i];
-    const bool counted = x != ignore && x >= 0 && x < v;
-    if (rank) rank[i] = counted ? r : -1;
-    if (counted) {
-      row_of[r] = i;
-      row_target[r] = (int)x;
-      ++r;
-    } else if (reduction == PSGD_REDUCE_NONE) {
-      loss[i] = 0.f;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
     }
+    if (lane == 31) warp_total[warp] = sum;
+    __syncthreads();
+    int before = total, all = 0;
+    for (int w = 0; w < 32; ++w) {
+      if (w < warp) before += warp_total[w];
+      all += warp_total[w];
+    }
+    before += sum - c0 - c1;
+    count[2 * t] = before;
+    count[2 * t + 1] = before + c0;
+    total += all;
+    __syncthreads();
+#pragma unroll 8
+    for (int g = 0; g < groups; ++g) {
+      const int i = base + g * 1024 + t;
+      const long long x = i < n ? target[i] : ignore;
+      const bool counted = x != ignore && x >= 0 && x < v;
+      const uint32_t m = __ballot_sync(0xffffffffu, counted);
+      const int r = count[g * 32 + warp] + __popc(m & ((1u << lane) - 1u));
+      if (i >= n) continue;
+      rank[i] = counted ? r : -1;
+      if (counted) {
+        row_of[r] = i;
+        row_target[r] = (int)x;
+      } else if (none) {
+        loss[i] = 0.f;
+      }
+    }
+    __syncthreads();
   }
+  if (bad) report(err, ERR_BAD_TARGET);
+  top = warp_max(top);
+  if (lane == 0) tops[warp] = top;
+  __syncthreads();
   if (t == 0) {
+    for (int w = 1; w < 32; ++w) top = fmaxf(top, tops[w]);
     state->counted = total;
     // fp16 gradients: per-row upstream values are taken relative to the largest, so that g stays in range
-    const float unit = half && reduction == PSGD_REDUCE_NONE && grad && top > 0.f ? top : 1.f;
+    const float unit = half && none && grad && top > 0.f ? top : 1.f;
     state->row_unit = unit;
     float alpha = half ? unit / L_HALF_SCALE : 1.f;
-    if (reduction != PSGD_REDUCE_NONE && grad) alpha *= *grad;
+    if (!none && grad) alpha *= *grad;
     if (reduction == PSGD_REDUCE_MEAN) alpha /= (float)max(total, 1);
     state->alpha = alpha;
   }
@@ -111,46 +141,59 @@ PSGD_DEVI void limbs3(float x, float* l) {
   l[2] = r - l[1];
 }
 
-// Row i of src (n rows of d) to row rank[i] (i without a rank) of the operand: itself, or its bf16 limbs `plane`
-// elements apart. Rows without a rank zero their row of dh instead. The 64 threads groups beyond n zero the operand's
-// rows from the count to the next multiple of 64, which a reduction over rows reads.
+// Tensor-core operands from matrices: row i of src to row rank[i] (i without ranks), itself or its bf16 limbs `plane`
+// elements apart. Rows whose rank is -1 zero their row of dh instead. Blocks beyond the rows zero the operand's rows from
+// the count to the next multiple of 64, which a reduction over rows reads.
+template <typename T>
+struct LceStage {
+  const T* src;
+  long long ld, ld_out, plane;
+  const int* rank;
+  uint16_t* out;
+  T* dh;
+  int n, blocks;  // (8 rows a block)
+};
 template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) lce_stage_kernel(const T* __restrict__ src, long long ld, int n, int d,
-                                                        const int* __restrict__ rank, const LceState* state,
-                                                        uint16_t* __restrict__ out, long long ld_out, long long plane,
-                                                        T* __restrict__ dh) {
+__global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, const LceStage<T> w, int d,
+                                                        const LceState* state) {
   constexpr int V = VEC ? 8 : 1;
-  const int lane = threadIdx.x & 31;
-  const long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (i >= (long long)n + (rank ? 64 : 0)) return;
+  pdl_trigger();
+  pdl_wait();
+  const bool first = (int)blockIdx.x < h.blocks;
+  const LceStage<T>& a = first ? h : w;
+  const int lane = threadIdx.x & 31, i = (blockIdx.x - (first ? 0 : h.blocks)) * 8 + (threadIdx.x >> 5);
   long long r = i;
-  if (i >= n) {
-    r = state->counted + (i - n);
+  if (i >= a.n) {
+    if (!a.rank || i >= a.n + 64) return;
+    r = state->counted + (i - a.n);
     if (r >= ((state->counted + 63) & ~63)) return;
-  } else if (rank) {
-    r = rank[i];
+  } else if (a.rank) {
+    r = a.rank[i];
   }
   if (r < 0) {
-    if (dh)
+    if (a.dh)
       for (int e = lane * V; e < d; e += 32 * V) {
         const float zero[8] = {};
-        store_vec<T, V>(dh + i * d + e, zero);
+        store_vec<T, V>(a.dh + (long long)i * d + e, zero);
       }
     return;
   }
+  const bool there = i < a.n;
+  const T* src = a.src + (there ? i * a.ld : 0);
+  uint16_t* out = a.out + r * a.ld_out;
   for (int e = lane * V; e < d; e += 32 * V) {
     if constexpr (sizeof(T) == 2) {
-      T* to = reinterpret_cast<T*>(out) + r * ld_out + e;
+      T* to = reinterpret_cast<T*>(out) + e;
       if constexpr (VEC) {
-        *reinterpret_cast<uint4*>(to) = i < n ? *reinterpret_cast<const uint4*>(src + i * ld + e) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(to) = there ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0, 0, 0, 0);
       } else {
-        *to = i < n ? src[i * ld + e] : from_f32<T>(0.f);
+        *to = there ? src[e] : from_f32<T>(0.f);
       }
     } else {
       float x[V], l[3][V];
 #pragma unroll
       for (int k = 0; k < V; ++k) x[k] = 0.f;
-      if (i < n) load_vec<T, V>(src + i * ld + e, x);
+      if (there) load_vec<T, V>(src + e, x);
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         float p[3];
@@ -159,18 +202,17 @@ __global__ void __launch_bounds__(256) lce_stage_kernel(const T* __restrict__ sr
       }
 #pragma unroll
       for (int q = 0; q < 3; ++q)
-        store_vec<__nv_bfloat16, V>(reinterpret_cast<__nv_bfloat16*>(out) + q * plane + r * ld_out + e, l[q]);
+        store_vec<__nv_bfloat16, V>(reinterpret_cast<__nv_bfloat16*>(out) + q * a.plane + e, l[q]);
     }
   }
 }
 
 // ---- the products ----------------------------------------------------------------------------------------------------
-// D (M x N) = A B^T over K, in `nseg` passes over K that take the limbs segs[i] = (limb of A) | (limb of B) << 4 in turn.
-// An operand is K-major (rows of M or N, K contiguous) or MN-major (rows of K, M or N contiguous: *_mn).
+// D (M x N) = A B^T over K. An operand is K-major (rows of M or N, K contiguous) or MN-major (rows of K, M or N contiguous:
+// *_mn). fp32 operands are three bf16 limbs: the products of limbs (i, j) with i + j <= 2 (2^-24 of the whole is left out).
 struct LceProblem {
   CUtensorMap ta[L_LIMBS], tb[L_LIMBS];
-  int a_mn, b_mn, nseg;
-  uint8_t segs[8];
+  int a_mn, b_mn;
   int M, N, K;    // bounds; the counted rows replace M (dyn 1) or K (dyn 2)
   int dyn, row0;  // first counted row of this piece
   int splits;     // K blocks are dealt to this many units of a tile, whose sums go to `part`
@@ -183,17 +225,19 @@ struct LceProblem {
   float* acc_out;    // sums so far, fp32, instead of out
 };
 struct LceShape {
-  int M, K, tiles_m, tiles_n, kblocks, units;
+  int M, K, tiles_m, tiles_n, kblocks, units, unit_kblocks;
 };
+template <int BN>
 PSGD_DEVI LceShape lce_shape(const LceProblem& p, const LceState* state) {
   LceShape s;
   const int there = max(0, state->counted - p.row0);
   s.M = p.dyn == 1 ? min(p.M, there) : p.M;
   s.K = p.dyn == 2 ? min(p.K, there) : p.K;
   s.tiles_m = (s.M + LM - 1) / LM;
-  s.tiles_n = (p.N + LN - 1) / LN;
+  s.tiles_n = (p.N + BN - 1) / BN;
   s.kblocks = (s.K + LK - 1) / LK;
   s.units = s.tiles_m * s.tiles_n * p.splits;
+  s.unit_kblocks = s.kblocks / p.splits;
   return s;
 }
 struct LceUnit {
@@ -213,22 +257,73 @@ PSGD_DEVI LceUnit lce_unit(const LceProblem& p, const LceShape& s, int u) {
   return x;
 }
 
+// The units of a cluster: its share of the first problem's, dealt in turn, then of the second's, of which the clusters
+// that had one unit less of the first take as many more first as make up for it (the first problem's units are the
+// longer ones: without this the longest and the shortest share would be one of them apart).
+struct LceDeal {
+  int c, n, h, rem, extra, base, u0, u1;
+  PSGD_DEVI LceDeal(const LceShape& s0, const LceShape& s1, bool two) {
+    c = blockIdx.x >> 1;
+    n = gridDim.x >> 1;
+    u0 = s0.units;
+    u1 = two ? s1.units : 0;
+    rem = u0 % n;
+    h = u0 / n + (c < rem);
+    extra = two && rem && s1.unit_kblocks ? s0.unit_kblocks / s1.unit_kblocks : 0;
+    base = (n - rem) * extra;
+  }
+  // Unit k of this cluster: (problem, index), or false.
+  PSGD_DEVI bool get(int k, int& problem, int& index) const {
+    problem = k >= h;
+    if (!problem) {
+      index = c + k * n;
+      return true;
+    }
+    k -= h;
+    const bool is_short = c >= rem;
+    if (is_short && k < extra) {
+      index = (c - rem) + k * (n - rem);
+    } else {
+      index = base + (is_short ? c - rem : c + (n - rem)) + (k - (is_short ? extra : 0)) * n;
+    }
+    return index < u1;
+  }
+};
+
 struct LceLogits {  // what the logits' epilogue keeps
-  float2* stats;  // [row][column tile]: (maximum, sum of exp)
-  float* linear;  // [row][column tile]: sum of the logits (label smoothing), or NULL
+  float2* stats;  // [row][half a tile's columns]: (maximum, sum of exp)
+  float* linear;  // [row][half a tile's columns]: sum of the logits (label smoothing), or NULL
   float* target_logit;
   const int* row_target;
   void* kept;  // exp(l - m), [row][ld_kept], or NULL
   long long ld_kept;
+  int tiles;
 };
 
 struct __align__(64) LceArgs {
   LceProblem p[2];
-  int nproblems;
+  int nproblems, chunk;  // chunk: K blocks that a sum runs over before it is added in fp32
   LceLogits logits;
   const LceState* state;
+  const float* loss_rows;  // summed into loss by the first block, or NULL
+  float* loss;
+  int mean;
   int* err;
   unsigned long long wait_ns;
+};
+
+// Shared memory of a stage: KS blocks of 64 of K, each LIMBS tiles of A (this CTA's 128 rows) and of B (its half of BN).
+template <int LIMBS, int BN>
+struct LceCfg {
+  static constexpr int KS = LIMBS == 1 ? 2 : 1;
+  static constexpr int STAGES = 3;
+  static constexpr int A = 128 * LK * 2, B = (BN / 2) * LK * 2;
+  static constexpr int BLOCK = LIMBS * (A + B), STAGE = KS * BLOCK;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 512;
+  static constexpr int COLS = BN / 2;                  // accumulator columns of an epilogue thread
+  static constexpr int ACC = (LIMBS == 1 ? 1 : 2) * BN;  // TMEM columns of an accumulator (fp32: the small products apart)
+  static constexpr int TMEM = 2 * ACC < 512 ? 256 : 512;
+  static_assert(2 * ACC <= 512 && SMEM <= 232448, "TMEM and shared memory of an SM");
 };
 
 PSGD_DEVI uint64_t lce_desc(uint32_t saddr, bool mn) {
@@ -238,279 +333,401 @@ PSGD_DEVI uint64_t lce_desc(uint32_t saddr, bool mn) {
   if (mn) d = (d & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(8192 >> 4) << 16);
   return d;
 }
-template <typename T>
+template <typename OP, int BN>
 PSGD_DEVI uint32_t lce_idesc(bool a_mn, bool b_mn) {
-  const uint32_t fmt = sizeof(T) == 2 && !is_half<T>() ? 1u : 0u;
+  const uint32_t fmt = is_half<OP>() ? 0u : 1u;
   return (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-         ((uint32_t)(LN >> 3) << 17) | ((uint32_t)(LM >> 4) << 24);
+         ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(LM >> 4) << 24);
 }
 
 constexpr float LOG2E = 1.4426950408889634f;
-PSGD_DEVI float exp_fast(float x) {  // exp of x <= 0 (or NaN); x log2 e is rounded to fp32: relative error 6e-8 |x| + 2 ulp
+PSGD_DEVI float exp2_fast(float x) {
   float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * LOG2E));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-
-// The logits' epilogue for one row of a tile (thread = row).
-template <typename KT>
-PSGD_DEVI void logits_row(const LceProblem& p, const LceShape& sh, const LceLogits& g, const LceUnit& u, uint32_t tacc,
-                          int row_in_tile) {
-  constexpr bool WIDE = sizeof(KT) == 4;
-  const long long row = (long long)u.tm * LM + row_in_tile;
-  const bool live = row < sh.M;
-  const int n0 = u.tn * LN, width = min(LN, p.N - n0);
-  float top = -INFINITY, linear = 0.f;
-  const int at = live ? g.row_target[p.row0 + row] - n0 : -1;
-  for (int c = 0; c < LN; c += 32) {
-    if (c >= width) break;
-    float v[32];
-    tmem_ld32(tacc + (uint32_t)c, v);
-    if (c + 32 <= width) {
+// 32 bytes at once (a whole sector of a row that other lanes do not share).
+PSGD_DEVI void store32(void* p, const uint32_t* w) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+template <typename T>
+PSGD_DEVI void store_row32(T* p, const float* v) {  // 32 bytes of T
+  uint32_t w[8];
 #pragma unroll
-      for (int k = 0; k < 32; ++k) top = fmaxf(top, v[k]);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (c + k < width) top = fmaxf(top, v[k]);
-    }
-    if (g.linear)
-#pragma unroll
-      for (int k = 0; k < 32; ++k) linear += c + k < width ? v[k] : 0.f;
-    const bool here = at >= c && at < c + 32;
-    if (__any_sync(0xffffffffu, here)) {
-      float x = 0.f;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) x = at == c + k ? v[k] : x;
-      if (here) g.target_logit[row] = x;
-    }
+  for (int k = 0; k < 8; ++k) {
+    if constexpr (sizeof(T) == 4) w[k] = __float_as_uint(v[k]);
+    else w[k] = pack2(v[2 * k], v[2 * k + 1], T());
   }
-  const float ref = top == -INFINITY ? 0.f : top;
+  store32(p, w);
+}
+
+// The logits' epilogue: this thread's COLS columns of one row.
+template <typename KT, int COLS>
+PSGD_DEVI void logits_row(const LceProblem& p, const LceShape& sh, const LceLogits& g, long long row, int n0, float* v) {
+  constexpr bool WIDE = sizeof(KT) == 4;
+  const bool live = row < sh.M;
+  const int width = min(COLS, p.N - n0);  // (n0 is below N: see the caller)
+  const int at = live ? g.row_target[p.row0 + row] - n0 : -1;
+  const bool here = at >= 0 && at < width;
+  if (__any_sync(0xffffffffu, here)) {
+    float x = 0.f;
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) x = at == k ? v[k] : x;
+    if (here) g.target_logit[row] = x;
+  }
+  float linear = 0.f;
+  if (g.linear)
+#pragma unroll
+    for (int k = 0; k < COLS; ++k) linear += k < width ? v[k] : 0.f;
+  if (width < COLS)
+#pragma unroll
+    for (int k = 0; k < COLS; ++k)
+      if (k >= width) v[k] = -INFINITY;
+  float top = v[0];
+#pragma unroll
+  for (int k = 1; k < COLS; ++k) top = fmaxf(top, v[k]);
+  const float ref = top == -INFINITY || top != top ? 0.f : top;
   float sum = 0.f;
-  KT* kept = g.kept ? reinterpret_cast<KT*>(g.kept) + row * g.ld_kept + n0 : nullptr;
-  for (int c = 0; c < LN; c += 32) {
-    if (c >= width) break;
-    float v[32];
-    tmem_ld32(tacc + (uint32_t)c, v);
 #pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      v[k] = WIDE ? expf(v[k] - ref) : exp_fast(v[k] - ref);
-      if (c + k >= width) v[k] = 0.f;
-      sum += v[k];
-      if (!WIDE) v[k] *= L_KEEP_SCALE;
-    }
-    if (kept && live)
+  for (int k = 0; k < COLS; ++k) {
+    // 16 bits: 2^15 exp(l - m), the factor added to the exponent, whose rounding is 2^-21 at most
+    v[k] = WIDE ? expf(v[k] - ref) : exp2_fast(fmaf(v[k] - ref, LOG2E, 15.f));
+    sum += v[k];
+  }
+  if (!WIDE) sum *= 1.f / L_KEEP_SCALE;
+  if (g.kept && live) {
+    KT* to = reinterpret_cast<KT*>(g.kept) + row * g.ld_kept + n0;
+    constexpr int S = 32 / sizeof(KT);
 #pragma unroll
-      for (int k = 0; k < 32; k += 8) store_vec<KT, 8>(kept + c + k, v + k);
+    for (int k = 0; k < COLS; k += S)
+      if (k < width) store_row32<KT>(to + k, v + k);  // (ld_kept is a multiple of 64: zeros up to there)
   }
   if (live) {
-    g.stats[row * sh.tiles_n + u.tn] = make_float2(top, sum);
-    if (g.linear) g.linear[row * sh.tiles_n + u.tn] = linear;
+    const long long to = row * g.tiles + n0 / COLS;
+    g.stats[to] = make_float2(top, sum);
+    if (g.linear) g.linear[to] = linear;
   }
 }
 
-// The gradients' epilogue for one row of a tile.
-template <typename T>
-PSGD_DEVI void grad_row(const LceProblem& p, const LceShape& sh, const LceUnit& u, uint32_t tacc, int row_in_tile,
-                        float alpha) {
-  const long long row = (long long)u.tm * LM + row_in_tile;
-  const bool live = row < sh.M, zero = u.k0 >= u.k1;
-  const int n0 = u.tn * LN, width = min(LN, p.N - n0);
-  const long long to = live ? (p.row_of ? p.row_of[p.row0 + row] : row) : 0;
-  const bool vec = p.ld_out % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
-  const bool vec4 = p.N % 4 == 0;
-  for (int c = 0; c < LN; c += 32) {
-    if (c >= width) break;
-    float v[32];
-    tmem_ld32(tacc + (uint32_t)c, v);
-    if (!live) continue;
-    if (zero)
+// The gradients' epilogue: this thread's COLS columns of one row.
+template <typename T, int COLS>
+PSGD_DEVI void grad_row(const LceProblem& p, const LceShape& sh, int split, long long row, int n0, float* v, float alpha) {
+  if (row >= sh.M) return;
+  const int width = min(COLS, p.N - n0);
+  const long long flat = row * p.N + n0;
+  const float* from = p.acc ? p.acc + flat : nullptr;
+  if (from) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k) v[k] = 0.f;
-    const int w = min(32, width - c);
-    const long long flat = row * p.N + n0 + c;
-    if (p.acc) {
+    for (int k = 0; k < COLS; ++k)
+      if (k < width) v[k] += from[k];
+  }
+  float* wide = p.part ? p.part + (long long)split * p.M * p.N + flat : p.acc_out ? p.acc_out + flat : nullptr;
+  if (wide) {
+    if (width == COLS && p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(wide) & 31) == 0) {
 #pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (k < w) v[k] += p.acc[flat + k];
-    }
-    float* wide = p.part ? p.part + (long long)u.split * p.M * p.N + flat : p.acc_out ? p.acc_out + flat : nullptr;
-    if (wide) {
-      if (vec4 && w == 32) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 4) *reinterpret_cast<float4*>(wide + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 32; ++k)
-          if (k < w) wide[k] = v[k];
-      }
-      continue;
-    }
-#pragma unroll
-    for (int k = 0; k < 32; ++k) v[k] *= alpha;
-    T* out = reinterpret_cast<T*>(p.out) + to * p.ld_out + n0 + c;
-    if (vec && w == 32) {
-#pragma unroll
-      for (int k = 0; k < 32; k += 8) store_vec<T, 8>(out + k, v + k);
+      for (int k = 0; k < COLS; k += 8) store_row32<float>(wide + k, v + k);
     } else {
 #pragma unroll
-      for (int k = 0; k < 32; ++k)
-        if (k < w) out[k] = from_f32<T>(v[k]);
+      for (int k = 0; k < COLS; ++k)
+        if (k < width) wide[k] = v[k];
     }
+    return;
+  }
+  constexpr int S = 32 / sizeof(T);
+  T* out = reinterpret_cast<T*>(p.out) + (p.row_of ? p.row_of[p.row0 + row] : row) * p.ld_out + n0;
+#pragma unroll
+  for (int k = 0; k < COLS; ++k) v[k] *= alpha;
+  if (width == COLS && p.ld_out % S == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0) {
+#pragma unroll
+    for (int k = 0; k < COLS; k += S) store_row32<T>(out + k, v + k);
+  } else {
+#pragma unroll
+    for (int k = 0; k < COLS; ++k)
+      if (k < width) out[k] = from_f32<T>(v[k]);
   }
 }
 
-// OP: operand type of the tensor cores; OUT: logits (float: kept exponentials in fp32, __half: in fp16) or gradients of
-// type OUT. Warp 0 copies tiles, warp 1 issues the products, warps 2..5 take the accumulators (two, in turn).
-template <typename OP, typename OUT, bool LOGITS>
-__global__ void __launch_bounds__(L_THREADS, 1) lce_product_kernel(const __grid_constant__ LceArgs args) {
+template <int COLS>
+PSGD_DEVI void add_columns(uint32_t at, float* v) {
+#pragma unroll
+  for (int b = 0; b < COLS; b += 32) {
+    float t[32];
+    tmem_ld32(at + b, t);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) v[b + e] += t[e];
+  }
+}
+
+// A cluster of two CTAs on neighbouring SMs computes 256 x BN tiles: each CTA stages its 128 rows of A and its half of
+// B, the leader (rank 0) issues M = 256 products that read both CTAs' shared memory, and each CTA's TMEM receives its 128
+// rows. Against one-CTA tiles of 128 x 256 this takes a third less through L2 and shared memory for a product.
+//   warp 0      copies; warp 1 (leader) products; warps 4..11: TMEM lanes 32 (w % 4)..., half of the columns each.
+// Handshakes (waits bounded): full[s] at the leader counts both CTAs' copies of stage s, go[s] tells the peer that the
+// leader has armed it, empty[s] frees it (the products' commit, in both CTAs), tfull / tempty hand the two accumulators
+// over. An accumulator takes `chunk` blocks of K; the epilogue adds the chunks in registers and hands the accumulator
+// back at once: the tensor cores' sums truncate (a bias of about 1.1e-9 a product, measured), so sums that are to be
+// right to fp32 stay short there, and the last step of a tile, from registers, never holds the tensor cores up.
+template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
+    lce_product_kernel(const __grid_constant__ LceArgs args) {
+  using C = LceCfg<LIMBS, BN>;
+  constexpr int S = C::STAGES, COLS = C::COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L_STAGES * L_STAGE_BYTES);
-  uint64_t* empty = full + L_STAGES;
-  uint64_t* tfull = empty + L_STAGES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * C::STAGE);
+  uint64_t* empty = full + S;
+  uint64_t* go = empty + S;
+  uint64_t* tfull = go + S;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const LceShape s0 = lce_shape(args.p[0], args.state);
-  const LceShape s1 = args.nproblems > 1 ? lce_shape(args.p[1], args.state) : LceShape{};
-  const int units = s0.units + (args.nproblems > 1 ? s1.units : 0);
+  const uint32_t rank = cluster_rank();  // 0: leader
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < L_STAGES; ++s) {
+    for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      mbar_init(&go[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
-      mbar_init(&tempty[a], 4);
+      mbar_init(&tempty[a], 16);
     }
     mbar_init(drain, 1);
     *abort = 0;
     fence_barrier_init();
   }
+  pdl_trigger();
+  __syncthreads();
+  cluster_sync();  // both CTAs' barriers exist before any remote arrive or copy signal
   if (warp == 1) {
     __syncwarp();
-    tmem_alloc(tmem_slot, 2 * LN);
-    tmem_relinquish();
+    tmem_alloc_pair(tmem_slot, C::TMEM);
+    tmem_relinquish_pair();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();  // what the launch before wrote is read from here on
+  const bool two = args.nproblems > 1;
+  const LceShape s0 = lce_shape<BN>(args.p[0], args.state);
+  const LceShape s1 = two ? lce_shape<BN>(args.p[1], args.state) : LceShape{};
+  const LceDeal deal(s0, s1, two);
+  const int chunk = args.chunk / C::KS;  // rounds of the stage ring to an accumulator
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L_REGS_LOW));
+    if (warp == 0 && lane == 0) {
+      // ---------------- copies (both CTAs) ----------------
       int s = 0;
-      uint32_t ph = 0, rounds = 0;
-      for (int x = blockIdx.x; x < units && !*abort; x += gridDim.x) {
-        const LceProblem& p = args.p[x >= s0.units];
-        const LceShape& sh = x >= s0.units ? s1 : s0;
-        const LceUnit u = lce_unit(p, sh, x >= s0.units ? x - s0.units : x);
-        for (int seg = 0; seg < p.nseg && !*abort; ++seg) {
-          const CUtensorMap* ta = &p.ta[p.segs[seg] & 15];
-          const CUtensorMap* tb = &p.tb[p.segs[seg] >> 4];
-          for (int k = u.k0; k < u.k1; ++k) {
-            if (!mbar_wait_for(&empty[s], ph ^ 1, abort, args.wait_ns)) break;
-            mbar_arrive_expect_tx(&full[s], L_STAGE_BYTES);
+      uint32_t ph = 0, rounds = 0;  // rounds that the leader armed, landed before it leaves on abort
+      int which, index;
+      for (int k = 0; deal.get(k, which, index) && !*abort; ++k) {
+        const LceProblem& p = args.p[which];
+        const LceUnit u = lce_unit(p, which ? s1 : s0, index);
+        const int row = u.tm * LM + (int)rank * 128, col = u.tn * BN + (int)rank * (BN / 2);
+        for (int kb = u.k0; kb < u.k1; kb += C::KS) {
+          const int subs = min(C::KS, u.k1 - kb);
+          if (!mbar_wait_for(&empty[s], ph ^ 1, abort, args.wait_ns)) break;
+          if (rank == 0) {
+            mbar_arrive_expect_tx(&full[s], 2u * C::BLOCK * (uint32_t)subs);
             ++rounds;
-            uint8_t* sa = smem + s * L_STAGE_BYTES;
-            uint8_t* sb = sa + L_A_BYTES;
-            if (p.a_mn) {
-              for (int i = 0; i < LM / 64; ++i) tma_load_2d(sa + i * 8192, ta, &full[s], u.tm * LM + i * 64, k * LK);
-            } else {
-              tma_load_2d(sa, ta, &full[s], k * LK, u.tm * LM);
-            }
-            if (p.b_mn) {
-              for (int i = 0; i < LN / 64; ++i) tma_load_2d(sb + i * 8192, tb, &full[s], u.tn * LN + i * 64, k * LK);
-            } else {
-              tma_load_2d(sb, tb, &full[s], k * LK, u.tn * LN);
-            }
-            if (++s == L_STAGES) s = 0, ph ^= 1;
+            mbar_arrive_cluster_relaxed(mapa_shared(&go[s], 1));
+          } else if (!mbar_wait_for(&go[s], ph, abort, args.wait_ns)) {
+            break;
           }
+          const uint32_t fb = mapa_shared(&full[s], 0);
+          for (int j = 0; j < subs; ++j) {
+            const int x = (kb + j) * LK;
+#pragma unroll
+            for (int l = 0; l < LIMBS; ++l) {
+              uint8_t* sa = smem + s * C::STAGE + j * C::BLOCK + l * C::A;
+              uint8_t* sb = smem + s * C::STAGE + j * C::BLOCK + LIMBS * C::A + l * C::B;
+              if (p.a_mn) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) tma_load_2d_pair(sa + i * 8192, &p.ta[l], fb, row + i * 64, x);
+              } else {
+                tma_load_2d_pair(sa, &p.ta[l], fb, x, row);
+              }
+              if (p.b_mn) {
+#pragma unroll
+                for (int i = 0; i < BN / 128; ++i) tma_load_2d_pair(sb + i * 8192, &p.tb[l], fb, col + i * 64, x);
+              } else {
+                tma_load_2d_pair(sb, &p.tb[l], fb, x, col);
+              }
+            }
+          }
+          if (++s == S) s = 0, ph ^= 1;
         }
       }
-      if (*abort) {  // copies in flight land before shared memory is released: the last round of each stage that had one
-        for (int i = 0; i < L_STAGES; ++i) {
-          const uint32_t n = rounds / L_STAGES + ((uint32_t)i < rounds % L_STAGES);
+      if (*abort && rank == 0) {
+        for (int i = 0; i < S; ++i) {
+          const uint32_t n = rounds / S + ((uint32_t)i < rounds % S);
           volatile int never = 0;
           if (n) mbar_wait(&full[i], (n - 1) & 1, &never);
         }
       }
-    }
-  } else if (warp == 1) {
-    if (lane == 0) {
+    } else if (warp == 1 && lane == 0 && rank == 0) {
+      // ---------------- products (leader) ----------------
       int s = 0;
       uint32_t ph = 0, i = 0;
-      bool issued = false;
-      for (int x = blockIdx.x; x < units; x += gridDim.x, ++i) {
-        const LceProblem& p = args.p[x >= s0.units];
-        const LceShape& sh = x >= s0.units ? s1 : s0;
-        const LceUnit u = lce_unit(p, sh, x >= s0.units ? x - s0.units : x);
-        const uint32_t acc = i & 1, aph = (i >> 1) & 1;
-        if (!mbar_wait_for(&tempty[acc], aph ^ 1, abort, args.wait_ns)) break;
-        tc_fence_after();
-        const uint32_t idesc = lce_idesc<OP>(p.a_mn, p.b_mn);
+      bool issued = false, ok = true;
+      int which, index;
+      for (int k = 0; ok && deal.get(k, which, index); ++k) {
+        const LceProblem& p = args.p[which];
+        const LceUnit u = lce_unit(p, which ? s1 : s0, index);
+        const uint32_t idesc = lce_idesc<OP, BN>(p.a_mn, p.b_mn);
         const uint32_t a_step = p.a_mn ? 2048 : 32, b_step = p.b_mn ? 2048 : 32;  // 16 of K, in bytes
-        uint32_t first = 0;
-        bool ok = true;
-        for (int seg = 0; seg < p.nseg && ok; ++seg)
-          for (int k = u.k0; k < u.k1; ++k) {
+        const uint64_t a0 = lce_desc(smem_u32(smem), p.a_mn), b0 = lce_desc(smem_u32(smem), p.b_mn);
+        int kb = u.k0;
+        do {  // one accumulator
+          const uint32_t acc = i & 1, aph = (i >> 1) & 1;
+          ++i;
+          if (!mbar_wait_for(&tempty[acc], aph ^ 1, abort, args.wait_ns)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t dt = tmem_base + acc * C::ACC;
+          uint32_t more = 0;
+          for (int r = 0; r < chunk && kb < u.k1; ++r, kb += C::KS) {
             if (!mbar_wait_for(&full[s], ph, abort, args.wait_ns)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t sa = smem_u32(smem + s * L_STAGE_BYTES), sb = sa + L_A_BYTES;
+            const int subs = min(C::KS, u.k1 - kb);
 #pragma unroll
-            for (int kk = 0; kk < LK / 16; ++kk) {
-              umma_bf16(tmem_base + acc * LN, lce_desc(sa + kk * a_step, p.a_mn), lce_desc(sb + kk * b_step, p.b_mn), idesc,
-                        first);
-              first = 1;
+            for (int j = 0; j < C::KS; ++j) {
+              if (j >= subs) break;
+              const uint32_t at = s * C::STAGE + j * C::BLOCK;
+#pragma unroll
+              for (int kk = 0; kk < LK / 16; ++kk) {
+                const uint64_t ad = a0 + ((at + kk * a_step) >> 4), bd = b0 + ((at + LIMBS * C::A + kk * b_step) >> 4);
+                umma_bf16_pair(dt, ad, bd, idesc, more);
+                if constexpr (LIMBS == 3) {
+                  constexpr uint32_t LA = C::A >> 4, LB = C::B >> 4;
+                  umma_bf16_pair(dt + BN, ad, bd + 2 * LB, idesc, more);
+                  umma_bf16_pair(dt + BN, ad + 2 * LA, bd, idesc, 1);
+                  umma_bf16_pair(dt + BN, ad + LA, bd + LB, idesc, 1);
+                  umma_bf16_pair(dt + BN, ad, bd + LB, idesc, 1);
+                  umma_bf16_pair(dt + BN, ad + LA, bd, idesc, 1);
+                }
+                more = 1;
+              }
             }
             issued = true;
-            umma_commit(&empty[s]);
-            if (++s == L_STAGES) s = 0, ph ^= 1;
+            umma_commit_pair(&empty[s], 3);
+            if (++s == S) s = 0, ph ^= 1;
           }
-        if (!ok) break;
-        umma_commit(&tfull[acc]);
+          if (!ok) break;
+          umma_commit_pair(&tfull[acc], 3);
+        } while (kb < u.k1);
       }
-      if (*abort && issued) {
-        umma_commit(drain);
+      if (*abort && issued) {  // every issued product (it reads both CTAs' shared memory) finishes first
+        umma_commit_pair(drain, 1);
         volatile int never = 0;
         mbar_wait(drain, 0, &never);
       }
     }
   } else {
-    const int q = warp & 3;
-    uint32_t i = 0;
+    // ---------------- accumulators (warps 4..11 of both CTAs) ----------------
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(L_REGS_HIGH));
+    const int q = warp & 3, half = (warp - 4) >> 2;
+    if (args.loss_rows && blockIdx.x == 0) {  // the loss itself: fixed order, by the first block's 256 threads
+      const int t = threadIdx.x - 128, n = args.state->counted;
+      float* red = reinterpret_cast<float*>(smem + S * C::STAGE + 256);
+      float sum = 0.f;
+      for (int r = t; r < n; r += 256) sum += args.loss_rows[r];
+      sum = warp_sum(sum);
+      if (lane == 0) red[warp - 4] = sum;
+      named_sync(1, 256);
+      if (t == 0) {
+        for (int w = 1; w < 8; ++w) sum += red[w];
+        *args.loss = args.mean ? sum / (float)max(n, 1) : sum;
+      }
+    }
+    const uint32_t lead0 = mapa_shared(&tempty[0], 0), lead1 = mapa_shared(&tempty[1], 0);
     const float alpha = args.state->alpha;
-    for (int x = blockIdx.x; x < units; x += gridDim.x, ++i) {
-      const LceProblem& p = args.p[x >= s0.units];
-      const LceShape& sh = x >= s0.units ? s1 : s0;
-      const LceUnit u = lce_unit(p, sh, x >= s0.units ? x - s0.units : x);
-      const uint32_t acc = i & 1, aph = (i >> 1) & 1;
-      const bool ok = __all_sync(0xffffffffu, mbar_wait_for(&tfull[acc], aph, abort, args.wait_ns));
-      if (!ok) break;
-      tc_fence_after();
-      const uint32_t tacc = tmem_base + ((uint32_t)(q * 32) << 16) + acc * LN;
-      if constexpr (LOGITS) logits_row<OUT>(p, sh, args.logits, u, tacc, q * 32 + lane);
-      else grad_row<OUT>(p, sh, u, tacc, q * 32 + lane, alpha);
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&tempty[acc]);
+    uint32_t i = 0;
+    bool ok = true;
+    int which, index;
+    for (int k = 0; ok && deal.get(k, which, index); ++k) {
+      const LceProblem& p = args.p[which];
+      const LceShape& sh = which ? s1 : s0;
+      const LceUnit u = lce_unit(p, sh, index);
+      const int rounds = (u.k1 - u.k0 + C::KS - 1) / C::KS, chunks = max(1, (rounds + chunk - 1) / chunk);
+      const long long row = (long long)u.tm * LM + rank * 128 + q * 32 + lane;
+      const int n0 = u.tn * BN + half * COLS;
+      // The next accumulator of this unit, at this warp's lanes and columns.
+      auto take = [&]() -> uint32_t {
+        const uint32_t acc = i & 1, aph = (i >> 1) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait_for(&tfull[acc], aph, abort, args.wait_ns));
+        tc_fence_after();
+        return tmem_base + ((uint32_t)(q * 32) << 16) + acc * C::ACC + half * COLS;
+      };
+      auto give_back = [&]() {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(i & 1 ? lead1 : lead0);
+        ++i;
+      };
+      if constexpr (!LOGITS && LIMBS == 1) {  // one sum over all of K: no more than 32 columns in registers
+        const uint32_t at = take();
+        if (!ok) break;
+#pragma unroll 1
+        for (int c = 0; c < COLS; c += 32) {
+          float f[32];
+          tmem_ld32(at + c, f);
+          if (n0 + c >= p.N) break;
+          if (u.k0 >= u.k1)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) f[e] = 0.f;
+          grad_row<OUT, 32>(p, sh, u.split, row, n0 + c, f, alpha);
+        }
+        give_back();
+      } else {
+        float f[COLS];
+        uint32_t at = take();
+        if (!ok) break;
+#pragma unroll
+        for (int b = 0; b < COLS; b += 32) tmem_ld32(at + b, f + b);
+#pragma unroll 1
+        for (int c = 1; c < chunks; ++c) {
+          if constexpr (LIMBS == 3) add_columns<COLS>(at + BN, f);
+          give_back();
+          at = take();
+          if (!ok) break;
+          add_columns<COLS>(at, f);
+        }
+        if (!ok) break;
+        if constexpr (LIMBS == 3) add_columns<COLS>(at + BN, f);
+        give_back();
+        if (u.k0 >= u.k1)
+#pragma unroll
+          for (int e = 0; e < COLS; ++e) f[e] = 0.f;
+        if (n0 < p.N) {
+          if constexpr (LOGITS) logits_row<OUT, COLS>(p, sh, args.logits, row, n0, f);
+          else grad_row<OUT, COLS>(p, sh, u.split, row, n0, f, alpha);
+        }
+      }
     }
   }
+
   tc_fence_before();
   __syncthreads();
+  cluster_sync();  // neither CTA releases shared memory or TMEM while the other may still use them
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
-    tmem_dealloc(tmem_base, 2 * LN);
+    tmem_dealloc_pair(tmem_base, C::TMEM);
   }
-  if (threadIdx.x == 0 && *abort) atomicOr(args.err, ERR_TIMEOUT_FULL);
+  if (threadIdx.x == 0 && *abort) report(args.err, ERR_TIMEOUT_FULL);
 }
 
 // ---- rows ------------------------------------------------------------------------------------------------------------
@@ -546,12 +763,15 @@ struct LceRows {
   long long ld_kept, plane;
   int v, tiles, row0, rows, none;
   float smoothing, z;
+  int stat;  // columns to a statistic
 };
 
 // One block a row (and 1 / gridDim.y of its columns). KT / GT: types of the kept exponentials and of g.
 template <typename KT, typename GT>
 __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const LceState* state) {
   __shared__ float red[8];
+  pdl_trigger();
+  pdl_wait();
   const int row = blockIdx.x, there = min(a.rows, max(0, state->counted - a.row0));
   KT* kept = reinterpret_cast<KT*>(a.kept) + (a.kept ? row * a.ld_kept : 0);
   const int vecs = (a.v + 7) / 8, per = (vecs + gridDim.y - 1) / gridDim.y;
@@ -590,6 +810,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
     else a.loss_rows[a.row0 + row] = loss;
   }
   if (!a.kept) return;
+  const int shift = a.stat == 64 ? 6 : 7;
   constexpr float unit = is_half<GT>() ? L_HALF_SCALE : 1.f;
   const float c = (a.grad ? a.grad[a.row_of[a.row0 + row]] / state->row_unit : 1.f) * unit;
   const float pull = 1.f + 2.f * a.z * lse, uniform = a.smoothing / (float)a.v;
@@ -597,7 +818,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   // the target's element from its fp32 logit: p - 1 without cancellation
   const float at_target = c * (expm1f(lt - lse) + (pull - 1.f) * expf(lt - lse) + a.smoothing - uniform);
   for (int i = v0 + threadIdx.x; i < v1; i += 256) {
-    const float f = expf(st[i * 8 / LN].x - lse) * scale * pull;
+    const float f = expf(st[(i * 8) >> shift].x - lse) * scale * pull;
     float g[8];
     load_vec<KT, 8>(kept + i * 8, g);
 #pragma unroll
@@ -626,6 +847,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
 __global__ void __launch_bounds__(1024) lce_loss_kernel(const float* __restrict__ rows, const LceState* state, int mean,
                                                         float* loss) {
   __shared__ float red[32];
+  pdl_wait();
   const int n = state->counted;
   float s = 0.f;
   for (int i = threadIdx.x; i < n; i += 1024) s += rows[i];
@@ -633,19 +855,28 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float* __restrict_
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
-// Joins the splits of dh: out[row_of[r]] = alpha * sum over splits, in their order.
-template <typename T>
+// Joins the splits of dh: out[row_of[r]] = alpha * sum over splits, in their order. V: values at a time (N a multiple).
+template <typename T, int V>
 __global__ void __launch_bounds__(256) lce_join_kernel(const float* __restrict__ part, int splits, int M, int N, int row0,
                                                        const int* __restrict__ row_of, T* __restrict__ out,
                                                        const LceState* state) {
-  const int there = min(M, max(0, state->counted - row0));
-  const long long n = (long long)there * N, plane = (long long)M * N;
+  pdl_wait();
+  const int there = min(M, max(0, state->counted - row0)), per_row = N / V;
+  const long long n = (long long)there * per_row, plane = (long long)M * N;
   const float alpha = state->alpha;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    float s = 0.f;
-    for (int k = 0; k < splits; ++k) s += part[k * plane + i];
-    const long long r = i / N;
-    out[(long long)row_of[row0 + r] * N + (i - r * N)] = from_f32<T>(s * alpha);
+    float s[V] = {};
+#pragma unroll 4
+    for (int k = 0; k < splits; ++k) {
+      float x[V];
+      load_vec<float, V>(part + k * plane + i * V, x);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] *= alpha;
+    const int r = (int)(i / per_row);
+    store_vec<T, V>(out + (long long)row_of[row0 + r] * N + (i - (long long)r * per_row) * V, s);
   }
 }
 
@@ -680,7 +911,7 @@ int encode(CUtensorMap* m, const void* p, bool half, long long rows, long long c
 
 // Where everything lies in the workspace; the same from a size query and from the call.
 struct Layout {
-  int limbs, tiles, piece, pieces, splits;
+  int limbs, tiles, piece, pieces, splits, bn, bn_grads, stat;
   bool stage_w;
   long long ld_h, ld_w, ld_kept, h_plane, w_plane, g_plane;
   size_t state, rank, row_of, row_target, loss_rows, target_logit, stats, linear, h, w, kept, g, part, acc, bytes;
@@ -691,7 +922,14 @@ Layout layout(const PsgdLce& a) {
   const bool wide = a.dtype == PSGD_F32;
   auto up = [](long long x, long long m) { return (x + m - 1) / m * m; };
   l.limbs = wide ? L_LIMBS : 1;
-  l.tiles = (a.v + LN - 1) / LN;
+  // Narrow tiles (128 columns) where wide ones would not go twice around the clusters; fp32 always (three limbs a stage).
+  const int clusters = psgd_num_sms() / 2;
+  const long long wide_tiles = (((long long)a.n + LM - 1) / LM) * ((a.v + 255) / 256);
+  l.bn = wide || wide_tiles < 2 * clusters ? 128 : 256;
+  const long long wide_grads = (((long long)a.n + LM - 1) / LM + (a.v + LM - 1) / LM) * ((a.d + 255) / 256);
+  l.bn_grads = wide || wide_grads < 2 * clusters ? 128 : 256;
+  l.stat = l.bn / 2;
+  l.tiles = (a.v + l.stat - 1) / l.stat;
   l.ld_h = up(a.d, 8);
   l.ld_w = up(a.d, 8);
   l.ld_kept = up(a.v, 64);
@@ -703,12 +941,16 @@ Layout layout(const PsgdLce& a) {
   if (piece > up(a.n, LM)) piece = up(a.n, LM);
   l.piece = (int)piece;
   l.pieces = (int)((a.n + piece - 1) / piece);
-  // dh has few tiles and a long reduction over the vocabulary: split it until its units are no longer than an SM's share
-  // of the whole launch (dh and dw need the same number of products)
-  const long long tiles = (piece / LM) * ((a.d + LN - 1) / LN), kblocks = (a.v + LK - 1) / LK;
-  long long splits = (2 * psgd_num_sms() + tiles - 1) / tiles;
-  if (splits > kblocks / 8) splits = kblocks / 8;
+  // dh has few tiles and a long reduction over the vocabulary. It and dw need the same number of products, so a unit
+  // of at most a quarter of a cluster's share of both keeps the shares even.
+  const long long tiles_h = ((piece + LM - 1) / LM) * ((a.d + l.bn_grads - 1) / l.bn_grads);
+  const long long tiles_w = (((long long)a.v + LM - 1) / LM) * ((a.d + l.bn_grads - 1) / l.bn_grads);
+  const long long kb_h = (a.v + LK - 1) / LK, kb_w = (piece + LK - 1) / LK;
+  const long long quarter = (tiles_h * kb_h + tiles_w * kb_w) / (4 * clusters) + 1;
+  long long splits = (kb_h + quarter - 1) / quarter;
+  if (splits > (kb_h + 7) / 8) splits = (kb_h + 7) / 8;
   if (splits > 16) splits = 16;
+  if (tiles_h >= 4 * clusters) splits = 1;  // (the units are even enough, and partial sums are not free)
   l.splits = splits < 1 ? 1 : (int)splits;
   size_t at = 0;
   auto take = [&](size_t bytes) {
@@ -744,30 +986,42 @@ bool valid(const PsgdLce& a) {
          a.reduction >= 0 && a.reduction <= 2 && a.piece_bytes >= 0 && a.n <= (1 << 30) && a.v <= (1 << 30);
 }
 
-template <typename K>
-int launch(K kernel, const LceArgs& args, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L_SMEM) != cudaSuccess) {
-    cudaGetLastError();  // else it would be taken for the next launch's
-    return PSGD_ELAUNCH;
-  }
-  kernel<<<psgd_num_sms(), L_THREADS, L_SMEM, stream>>>(args);
-  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+// A launch that may start while the one before it ends (it waits for it in the kernel: pdl_wait).
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = smem, c.stream = stream;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at, c.numAttrs = 1;
+  if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess) return PSGD_OK;
+  cudaGetLastError();  // else it would be taken for a later launch's
+  return PSGD_ELAUNCH;
 }
 
-template <typename T>
-int stage(const T* src, long long ld, int n, int d, const int* rank, const LceState* state, uint16_t* out, long long ld_out,
-          long long plane, T* dh, cudaStream_t stream) {
-  const bool vec = d % 8 == 0 && aligned16(src) && ld * sizeof(T) % 16 == 0 && aligned16(dh);
-  const int grid = (int)(((long long)n + (rank ? 64 : 0) + 7) / 8);
-  if (vec) lce_stage_kernel<T, true><<<grid, 256, 0, stream>>>(src, ld, n, d, rank, state, out, ld_out, plane, dh);
-  else lce_stage_kernel<T, false><<<grid, 256, 0, stream>>>(src, ld, n, d, rank, state, out, ld_out, plane, dh);
-  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
+int product(const LceArgs& args, cudaStream_t stream) {
+  using C = LceCfg<LIMBS, BN>;
+  auto k = lce_product_kernel<OP, OUT, LIMBS, BN, LOGITS>;
+  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+    cudaGetLastError();
+    return PSGD_ELAUNCH;
+  }
+  return launch(k, dim3(psgd_num_sms() / 2 * 2), dim3(L_THREADS), C::SMEM, stream, args);
+}
+template <typename OP, typename OUT, int LIMBS, bool LOGITS>
+int product_bn(int bn, const LceArgs& args, cudaStream_t stream) {
+  if constexpr (LIMBS == 1)
+    if (bn == 256) return product<OP, OUT, 1, 256, LOGITS>(args, stream);
+  return product<OP, OUT, LIMBS, 128, LOGITS>(args, stream);
 }
 
 // T: type of h, w and the gradients; OP: operand type of the tensor cores; KT: type of the kept exponentials.
 template <typename T, typename OP, typename KT>
 int run(const PsgdLce& a, int* err, cudaStream_t stream) {
   constexpr bool half = is_half<OP>();
+  constexpr int LIMBS = sizeof(T) == 4 ? L_LIMBS : 1;
   const Layout l = layout(a);
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
   LceState* state = reinterpret_cast<LceState*>(ws + l.state);
@@ -778,42 +1032,41 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
   uint16_t* h = reinterpret_cast<uint16_t*>(ws + l.h);
   const uint16_t* w = l.stage_w ? reinterpret_cast<uint16_t*>(ws + l.w) : reinterpret_cast<const uint16_t*>(a.w);
   const long long ld_w = l.stage_w ? l.ld_w : a.ld_w;
-  const bool none = a.reduction == PSGD_REDUCE_NONE;
+  const bool none = a.reduction == PSGD_REDUCE_NONE, mean = a.reduction == PSGD_REDUCE_MEAN;
 
   lce_plan_kernel<<<1, 1024, 0, stream>>>(a.target, a.n, a.v, a.ignore_index, a.reduction, half, a.grad, rank, row_of,
                                           row_target, a.loss, state, err);
   if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
-  if (int rc = stage<T>(reinterpret_cast<const T*>(a.h), a.ld_h, a.n, a.d, rank, state, h, l.ld_h, l.h_plane,
-                        reinterpret_cast<T*>(a.grads ? a.dh : nullptr), stream))
+  const LceStage<T> sh = {reinterpret_cast<const T*>(a.h), a.ld_h, l.ld_h, l.h_plane, rank, h,
+                          reinterpret_cast<T*>(a.grads ? a.dh : nullptr), a.n, (int)((a.n + 64LL + 7) / 8)};
+  const LceStage<T> sw = {reinterpret_cast<const T*>(a.w), a.ld_w, l.ld_w, l.w_plane, nullptr, const_cast<uint16_t*>(w),
+                          nullptr, a.v, l.stage_w ? (a.v + 7) / 8 : 0};
+  const bool vec = a.d % 8 == 0 && aligned16(a.h) && a.ld_h * sizeof(T) % 16 == 0 && aligned16(sh.dh) &&
+                   (!l.stage_w || (aligned16(a.w) && a.ld_w * sizeof(T) % 16 == 0));
+  if (int rc = launch(vec ? lce_stage_kernel<T, true> : lce_stage_kernel<T, false>, dim3(sh.blocks + sw.blocks), dim3(256),
+                      0, stream, sh, sw, a.d, (const LceState*)state))
     return rc;
-  if (l.stage_w)
-    if (int rc = stage<T>(reinterpret_cast<const T*>(a.w), a.ld_w, a.v, a.d, nullptr, state, const_cast<uint16_t*>(w), l.ld_w,
-                          l.w_plane, nullptr, stream))
-      return rc;
 
   LceArgs args = {};
   args.state = state;
   args.err = err;
   args.wait_ns = WAIT_LIMIT_NS;
-  // fp32: the products of two limbs down to 2^-16 of the whole, smallest first (2^-24 is left out)
-  const uint8_t six[6] = {0x20, 0x02, 0x11, 0x10, 0x01, 0x00};
-  auto limbs = [&](LceProblem& p) {
-    p.nseg = l.limbs == 1 ? 1 : 6;
-    for (int i = 0; i < 6; ++i) p.segs[i] = l.limbs == 1 ? 0 : six[i];
-    p.splits = 1;
-  };
   for (int piece = 0; piece < l.pieces; ++piece) {
     const int row0 = piece * l.piece, rows = a.n - row0 < l.piece ? a.n - row0 : l.piece;
     const int rows64 = (rows + 63) / 64 * 64;
     LceProblem& p = args.p[0];
     p = LceProblem{};
-    limbs(p);
+    p.splits = 1;
     for (int i = 0; i < l.limbs; ++i) {
-      if (int rc = encode(&p.ta[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows, a.d, l.ld_h, LM)) return rc;
-      if (int rc = encode(&p.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, LN)) return rc;
+      if (int rc = encode(&p.ta[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows, a.d, l.ld_h, 128)) return rc;
+      if (int rc = encode(&p.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, l.bn / 2)) return rc;
     }
     p.M = rows, p.N = a.v, p.K = a.d, p.dyn = 1, p.row0 = row0;
     args.nproblems = 1;
+    // The loss is fp32 whatever the operands are: sums of at most 1024 products (512 for fp32 operands) stay in the tensor
+    // cores, which keeps their truncation at 1e-6 of a logit.
+    args.chunk = LIMBS == 1 ? 16 : 8;
+    args.loss_rows = nullptr;
     LceLogits& g = args.logits;
     g.stats = reinterpret_cast<float2*>(ws + l.stats);
     g.linear = a.label_smoothing != 0.f ? reinterpret_cast<float*>(ws + l.linear) : nullptr;
@@ -821,26 +1074,25 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     g.row_target = row_target;
     g.kept = a.grads ? ws + l.kept : nullptr;
     g.ld_kept = l.ld_kept;
-    if (int rc = launch(lce_product_kernel<OP, KT, true>, args, stream)) return rc;
+    g.tiles = l.tiles;
+    if (int rc = product_bn<OP, KT, LIMBS, true>(l.bn, args, stream)) return rc;
 
     LceRows r = {};
     r.stats = g.stats, r.linear = g.linear, r.target_logit = g.target_logit, r.row_target = row_target, r.row_of = row_of;
     r.grad = none ? a.grad : nullptr;
     r.loss_rows = loss_rows, r.loss = a.loss, r.kept = g.kept, r.limbs = reinterpret_cast<uint16_t*>(ws + l.g);
     r.ld_kept = l.ld_kept, r.plane = l.g_plane, r.v = a.v, r.tiles = l.tiles, r.row0 = row0, r.rows = rows, r.none = none;
-    r.smoothing = a.label_smoothing, r.z = a.z_loss;
+    r.smoothing = a.label_smoothing, r.z = a.z_loss, r.stat = l.stat;
     int cols = a.grads ? (2 * psgd_num_sms() + rows64 - 1) / rows64 : 1;
     if (cols > (a.v + 2047) / 2048) cols = (a.v + 2047) / 2048;
-    lce_rows_kernel<KT, OP><<<dim3(rows64, cols), 256, 0, stream>>>(r, state);
-    if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
+    if (int rc = launch(lce_rows_kernel<KT, OP>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state)) return rc;
     if (!a.grads) continue;
 
     const uint16_t* gm = reinterpret_cast<const uint16_t*>(ws + l.g);
     LceProblem& ph = args.p[0];  // dh = g w: g K-major, w (rows of K = vocabulary) MN-major
     ph = LceProblem{};
-    limbs(ph);
     for (int i = 0; i < l.limbs; ++i) {
-      if (int rc = encode(&ph.ta[i], gm + i * l.g_plane, half, rows, a.v, l.ld_kept, LM)) return rc;
+      if (int rc = encode(&ph.ta[i], gm + i * l.g_plane, half, rows, a.v, l.ld_kept, 128)) return rc;
       if (int rc = encode(&ph.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, 64)) return rc;
     }
     ph.b_mn = 1, ph.M = rows, ph.N = a.d, ph.K = a.v, ph.dyn = 1, ph.row0 = row0, ph.splits = l.splits;
@@ -848,12 +1100,11 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     ph.part = l.splits > 1 ? reinterpret_cast<float*>(ws + l.part) : nullptr;
     LceProblem& pw = args.p[1];  // dw = g^T h: both with rows of K = tokens
     pw = LceProblem{};
-    limbs(pw);
     for (int i = 0; i < l.limbs; ++i) {
       if (int rc = encode(&pw.ta[i], gm + i * l.g_plane, half, rows64, a.v, l.ld_kept, 64)) return rc;
       if (int rc = encode(&pw.tb[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows64, a.d, l.ld_h, 64)) return rc;
     }
-    pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0;
+    pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = 1;
     pw.out = a.dw, pw.ld_out = a.d;
     if (l.pieces > 1) {
       float* acc = sizeof(T) == 4 ? reinterpret_cast<float*>(a.dw) : reinterpret_cast<float*>(ws + l.acc);
@@ -861,18 +1112,21 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
       pw.acc_out = piece + 1 < l.pieces ? acc : nullptr;
     }
     args.nproblems = 2;
-    if (int rc = launch(lce_product_kernel<OP, T, false>, args, stream)) return rc;
+    args.chunk = LIMBS == 1 ? 1 << 20 : 8;  // (a 16-bit gradient's own rounding is a hundred times the truncation)
+    if (!none && piece + 1 == l.pieces) args.loss_rows = loss_rows, args.loss = a.loss, args.mean = mean;
+    if (int rc = product_bn<OP, T, LIMBS, false>(l.bn_grads, args, stream)) return rc;
     if (l.splits > 1) {
-      const long long n = (long long)rows * a.d, want = (n + 255) / 256, most = 8LL * psgd_num_sms();
-      lce_join_kernel<T><<<(int)(want < most ? want : most), 256, 0, stream>>>(ph.part, l.splits, rows, a.d, row0, row_of,
-                                                                              reinterpret_cast<T*>(a.dh), state);
-      if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
+      const bool four = a.d % 8 == 0 && aligned16(a.dh);
+      const long long n = (long long)rows * a.d / (four ? 8 : 1), want = (n + 255) / 256, most = 8LL * psgd_num_sms();
+      if (int rc = launch(four ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
+                          dim3(256), 0, stream, (const float*)ph.part, l.splits, rows, a.d, row0, (const int*)row_of,
+                          reinterpret_cast<T*>(a.dh), (const LceState*)state))
+        return rc;
     }
   }
-  if (!none) {
-    lce_loss_kernel<<<1, 1024, 0, stream>>>(loss_rows, state, a.reduction == PSGD_REDUCE_MEAN, a.loss);
-    if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
-  }
+  if (!none && !a.grads)
+    return launch(lce_loss_kernel, dim3(1), dim3(1024), 0, stream, (const float*)loss_rows, (const LceState*)state, (int)mean,
+                  a.loss);
   return PSGD_OK;
 }
 

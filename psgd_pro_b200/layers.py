@@ -11,17 +11,16 @@ Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 an
 enqueued on the current stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
 The functions take part in autograd; the *_forward / *_grad forms are the same launches for callers that hold the
 gradients themselves (KronWhiten.step_math takes them as they come). Argument errors raise RuntimeError at the call.
-A target that is no class is found on the device: it counts as ignored, and the next linear_cross_entropy (or
-check_errors()) raises, as for the operators of psgd_pro_b200.ops."""
+A target that is no class is found on the device: it counts as ignored, and later linear_cross_entropy calls (and
+check_errors(), which waits) raise until reset_errors(), as for the operators of psgd_pro_b200.ops."""
 import ctypes
 from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
 
-from . import _capi, ops
+from . import _capi
 from ._capi import check
-from .ops import check_errors, reset_errors
 
 __all__ = ["dropout", "dropout_grad", "residual_norm", "residual_norm_forward", "residual_norm_grad",
            "linear_cross_entropy", "linear_cross_entropy_grad", "ResidualNormGrads", "check_errors", "reset_errors"]
@@ -44,7 +43,7 @@ def _elements(t, name):
 
 
 def _like(t, ref, name, shape=None):
-    if t.dtype != ref.dtype or t.device != ref.device:
+    if t.dtype != ref.dtype or not t.is_cuda or t.get_device() != ref.get_device():
         _fail(f"{name} must have the type and device of the first argument")
     if shape is not None and t.shape != shape:
         _fail(f"{name} must have the shape {tuple(shape)}")
@@ -54,37 +53,32 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _launch(device, fn, *args):
+    """fn(*args, stream) with `device` current, on its current stream (asked for by its raw handle: the Stream object
+    costs thirty times as much, and these calls are as short as their host code)."""
+    if torch._C._cuda_getDevice() == device:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device))
+    if rc != 0:
+        check(rc, fn.__name__)
 
 
-class _On:
-    """Makes the tensor's device current for the launches inside."""
-    __slots__ = ("index", "before")
-
-    def __init__(self, t):
-        self.index = t.get_device()
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.index:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *_):
-        if self.before != self.index:
-            torch.cuda.set_device(self.before)
-        return False
+def _new(t):
+    """An uninitialised contiguous tensor like t."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 # ---- dropout --------------------------------------------------------------------------------------------------------
-def _generator(p, seed, offset, device):
+def _generator(p, seed, offset, x):
     """(threshold, scale, seed, offset, rng pointer) of a mask."""
     if not 0.0 <= p <= 1.0:
         _fail("the dropout probability must lie in [0, 1]")
     threshold = int(round(p * 65536))
     scale = 65536.0 / (65536 - threshold) if threshold < 65536 else 0.0
     if isinstance(seed, Tensor):
-        if seed.dtype != torch.int64 or seed.device != device or seed.numel() != 2 or not seed.is_contiguous():
+        if seed.dtype != torch.int64 or seed.device != x.device or seed.numel() != 2 or not seed.is_contiguous():
             _fail("a seed tensor must hold two contiguous int64 values (seed, offset) on the inputs' device")
         return threshold, scale, 0, 0, seed.data_ptr()
     return threshold, scale, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, None
@@ -92,15 +86,17 @@ def _generator(p, seed, offset, device):
 
 def _dropout(x, p, seed, offset, residual):
     code = _elements(x, "x")
-    threshold, scale, seed, offset, rng = _generator(p, seed, offset, x.device)
-    x = x.contiguous()
+    threshold, scale, seed, offset, rng = _generator(p, seed, offset, x)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    at = None
     if residual is not None:
         _like(residual, x, "residual", x.shape)
         residual = residual.contiguous()
+        at = residual.data_ptr()
     out = torch.empty_like(x)
-    spec = _capi.Dropout(x.data_ptr(), _ptr(residual), out.data_ptr(), x.numel(), code, threshold, scale, seed, offset, rng)
-    with _On(x):
-        check(_capi.lib().psgd_dropout(ctypes.byref(spec), _stream(x)), "psgd_dropout")
+    spec = _capi.Dropout(x.data_ptr(), at, out.data_ptr(), x.numel(), code, threshold, scale, seed, offset, rng)
+    _launch(x.get_device(), _capi.lib().psgd_dropout, ctypes.byref(spec))
     return out
 
 
@@ -146,75 +142,81 @@ class ResidualNormGrads(NamedTuple):
     dgate: Optional[Tensor]
 
 
-def _rows(t, d, name):
-    """t as rows of d elements with a unit stride inside (a copy only where its strides allow no such view)."""
+def _rows(t, d):
+    """(t, stride of its rows): t as rows of d elements with a unit stride inside (a copy only where its strides allow no
+    such view)."""
+    if t.is_contiguous():
+        return t, d
     if t.dim() != 2:
         t = t.reshape(-1, d)
-    if t.stride(1) != 1 and d > 1 or t.stride(0) < d and t.shape[0] > 1:
+    if (t.stride(1) != 1 and d > 1) or (t.stride(0) < d and t.shape[0] > 1):
         t = t.contiguous()
-    return t
+    return t, max(t.stride(0), d)
 
 
 def _joint_spec(x, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps, dropout_p, seed, offset):
-    """(spec, rows, tensors to keep until the launch) of a joint of x (the residual, or its output) and y."""
-    code = _elements(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > _capi.JOINT_MAX_D:
-        _fail(f"rows must have 1 to {_capi.JOINT_MAX_D} elements")
-    if norm not in _NORMS:
+    """(spec, rows, type of the parameters, tensors to keep until the launch) of a joint of x (the residual, or its output)
+    and y."""
+    dtype, device, shape = x.dtype, x.get_device(), x.shape
+    code, kind = _TYPES.get(dtype), _NORMS.get(norm)
+    if code is None or device < 0:
+        _fail("x must be an fp32, bf16 or fp16 CUDA tensor")
+    if kind is None:
         _fail("norm must be 'rms' or 'layer'")
-    _like(y, x, "y", x.shape)
-    d = x.shape[-1]
-    params, kept = None, []
-    for t, name in ((weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias")):
-        if t is None:
-            continue
-        _elements(t, name)
-        if t.shape != (d,) or t.device != x.device:
-            _fail(f"{name} must hold {d} values on the inputs' device")
-        if params is None:
-            params = t.dtype
-        if t.dtype != params or params not in (x.dtype, torch.float32):
-            _fail("weights and biases must share one type: that of x, or fp32")
+    d = shape[-1] if shape else 0
+    if not 1 <= d <= _capi.JOINT_MAX_D:
+        _fail(f"rows must have 1 to {_capi.JOINT_MAX_D} elements")
+    if y.dtype != dtype or y.shape != shape or y.get_device() != device:
+        _fail("y must have the type, shape and device of the first argument")
     if not post_norm and (post_weight is not None or post_bias is not None):
         _fail("post_weight and post_bias need post_norm")
-    if norm == "rms" and (bias is not None or post_bias is not None):
+    if kind == 0 and (bias is not None or post_bias is not None):
         _fail("an rms norm has no bias")
     if not eps > 0.0:
         _fail("eps must be positive")
-    vectors = [t if t is None or t.is_contiguous() else t.contiguous() for t in (weight, bias, post_weight, post_bias)]
-    x2, y2 = _rows(x, d, "x"), _rows(y, d, "y")
-    rows = x2.shape[0]
-    gates = 0
+    params, pointers, kept = None, [None] * 4, []
+    for k, t in enumerate((weight, bias, post_weight, post_bias)):
+        if t is None:
+            continue
+        if params is None:
+            params = t.dtype
+        if t.dtype != params or (params != dtype and params != torch.float32) or t.get_device() != device or \
+                t.dim() != 1 or t.numel() != d:
+            _fail(f"weights and biases must hold {d} values of one type, that of x or fp32, on the inputs' device")
+        if not t.is_contiguous():
+            t = t.contiguous()
+            kept.append(t)
+        pointers[k] = t.data_ptr()
+    (x, ld_x), (y, ld_y) = _rows(x, d), _rows(y, d)
+    rows, gates, gate_at = x.numel() // d, 0, None
     if gate is not None:
-        _like(gate, x, "gate")
-        gates = _gates(gate, x, rows)
+        if gate.dtype != dtype or gate.get_device() != device:
+            _fail("gate must have the type and device of the first argument")
+        gates = _gates(gate, shape, rows)
         gate = gate.contiguous()
-    threshold, keep, seed, offset, rng = _generator(dropout_p, seed, offset, x.device)
-    s = _capi.Joint()
-    s.x, s.y, s.ld_x, s.ld_y = x2.data_ptr(), y2.data_ptr(), x2.stride(0), y2.stride(0)
-    s.weight, s.bias, s.post_weight, s.post_bias = (_ptr(t) for t in vectors)
-    s.gate, s.gates, s.rows, s.d, s.dtype = _ptr(gate), gates, rows, d, code
-    s.param_dtype = _TYPES[params or torch.float32]
-    s.kind, s.post, s.scale, s.eps = _NORMS[norm], int(post_norm), scale, eps
-    s.threshold, s.keep_scale, s.seed, s.offset, s.rng = threshold, keep, seed, offset, rng
-    return s, rows, (x2, y2, vectors, gate)
+        gate_at = gate.data_ptr()
+    threshold, keep, seed, offset, rng = _generator(dropout_p, seed, offset, x) if dropout_p else (0, 1.0, 0, 0, None)
+    s = _capi.Joint(x.data_ptr(), y.data_ptr(), None, None, None, *pointers, gate_at, None, None, None, None, None, None,
+                    None, None, None, ld_x, ld_y, d, d, rows, gates, d, code, _TYPES[params or torch.float32], kind,
+                    post_norm, scale, eps, threshold, keep, seed, offset, rng)
+    return s, rows, params or torch.float32, (x, y, kept, gate)
 
 
-def _gates(gate, x, rows):
+def _gates(gate, shape, rows):
     """How many rows of d the gate has: its leading dimensions are the first dimensions of x (ones after them), so that
     each of its rows serves consecutive rows of x; for a two-dimensional gate, any number that divides them."""
-    d = x.shape[-1]
+    d = shape[-1]
     if gate.dim() < 1 or gate.shape[-1] != d:
         _fail(f"gate must have rows of {d} values")
     lead, count = tuple(gate.shape[:-1]), gate.numel() // d
     if gate.dim() <= 2:
         if count >= 1 and (rows == 0 or rows % count == 0):
             return count
-    elif gate.dim() == x.dim():
+    elif gate.dim() == len(shape):
         k = len(lead)
         while k and lead[k - 1] == 1:
             k -= 1
-        if lead[:k] == tuple(x.shape[:k]) and count:
+        if lead[:k] == tuple(shape[:k]) and count:
             return count
     _fail("gate must be (d), (g, d) with g dividing the rows, or x's shape with ones after its first dimensions")
 
@@ -223,14 +225,12 @@ def residual_norm_forward(x: Tensor, y: Tensor, *, norm: str = "rms", post_norm:
                           post_weight=None, post_bias=None, gate=None, scale: float = 1.0, eps: float = 1e-6,
                           dropout_p: float = 0.0, seed=0, offset: int = 0):
     """(out, normed, stats) of residual_norm; stats (rows, 4) in fp32 is what residual_norm_grad needs besides out and y."""
-    s, rows, keep = _joint_spec(x, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps, dropout_p,
-                                seed, offset)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    normed = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(rows, 4, dtype=torch.float32, device=x.device)
+    s, rows, _, keep = _joint_spec(x, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps, dropout_p,
+                                   seed, offset)
+    out, normed = _new(x), _new(x)
+    stats = x.new_empty((rows, 4), dtype=torch.float32)
     s.out, s.normed, s.stats = out.data_ptr(), normed.data_ptr(), stats.data_ptr()
-    with _On(x):
-        check(_capi.lib().psgd_joint_forward(ctypes.byref(s), _stream(x)), "psgd_joint_forward")
+    _launch(x.get_device(), _capi.lib().psgd_joint_forward, ctypes.byref(s))
     return out, normed, stats
 
 
@@ -240,37 +240,41 @@ def residual_norm_grad(d_out: Optional[Tensor], d_normed: Optional[Tensor], out:
                        offset: int = 0) -> ResidualNormGrads:
     """Gradients of residual_norm's inputs from those of its outputs (None: zero), its output `out`, its input y and the
     stats of the forward call with the same options."""
-    s, rows, keep = _joint_spec(out, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps, dropout_p,
-                                seed, offset)
-    if stats.shape != (rows, 4) or stats.dtype != torch.float32 or stats.device != out.device or not stats.is_contiguous():
+    s, rows, pd, keep = _joint_spec(out, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps,
+                                    dropout_p, seed, offset)
+    d, device, shape = s.d, out.get_device(), out.shape
+    if stats.shape != (rows, 4) or stats.dtype != torch.float32 or stats.get_device() != device or not stats.is_contiguous():
         _fail("stats must be what residual_norm_forward returned")
-    d, device = s.d, out.device
-    pd = next((t.dtype for t in (weight, bias, post_weight, post_bias) if t is not None), torch.float32)
-    ups = []
-    for t, name in ((d_out, "d_out"), (d_normed, "d_normed")):
-        if t is not None:
-            _like(t, out, name, out.shape)
-            t = _rows(t, d, name)
-        ups.append(t)
-    s.stats, s.d_out, s.d_normed = stats.data_ptr(), _ptr(ups[0]), _ptr(ups[1])
-    s.ld_d_out, s.ld_d_normed = (d if t is None else t.stride(0) for t in ups)
+    s.stats = stats.data_ptr()
+    if d_out is not None:
+        _like(d_out, out, "d_out", shape)
+        d_out, s.ld_d_out = _rows(d_out, d)
+        s.d_out = d_out.data_ptr()
+    if d_normed is not None:
+        _like(d_normed, out, "d_normed", shape)
+        d_normed, s.ld_d_normed = _rows(d_normed, d)
+        s.d_normed = d_normed.data_ptr()
     layer = s.kind == _capi.PSGD_NORM_LAYER
 
-    def vector(there):
-        make = torch.empty if rows else torch.zeros
-        return make(d, dtype=pd, device=device) if there else None
+    def vector(there, like):
+        if not there:
+            return None
+        if rows and like is not None:
+            return _new(like)
+        return (out.new_empty if rows else out.new_zeros)((d,), dtype=pd)
 
-    dx, dy = (torch.empty(out.shape, dtype=out.dtype, device=device) for _ in range(2))
-    dweight, dbias, dpw, dpb = (vector(b) for b in (True, layer, post_norm, post_norm and layer))
-    dgate = None if gate is None else (torch.empty if rows else torch.zeros)(gate.shape, dtype=gate.dtype, device=device)
+    dx, dy = _new(out), _new(out)
+    dweight, dbias = vector(True, weight), vector(layer, bias)
+    dpw, dpb = vector(post_norm, post_weight), vector(post_norm and layer, post_bias)
+    dgate = None if gate is None else _new(gate) if rows else torch.zeros_like(gate)
     s.dx, s.dy, s.dgate = dx.data_ptr(), dy.data_ptr(), _ptr(dgate)
-    s.dweight, s.dbias, s.dpost_weight, s.dpost_bias = (_ptr(t) for t in (dweight, dbias, dpw, dpb))
-    with _On(out):
-        L = _capi.lib()
-        size = L.psgd_joint_workspace(ctypes.byref(s))
-        check(min(size, 0), "psgd_joint_workspace")
-        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=device)
-        check(L.psgd_joint_backward(ctypes.byref(s), ws.data_ptr(), size, _stream(out)), "psgd_joint_backward")
+    s.dweight, s.dbias, s.dpost_weight, s.dpost_bias = dweight.data_ptr(), _ptr(dbias), _ptr(dpw), _ptr(dpb)
+    L = _capi.lib()
+    size = L.psgd_joint_workspace(ctypes.byref(s))
+    if size < 0:
+        check(size, "psgd_joint_workspace")
+    ws = out.new_empty((size + 16,), dtype=torch.uint8)
+    _launch(device, L.psgd_joint_backward, ctypes.byref(s), ws.data_ptr(), size)
     return ResidualNormGrads(dx, dy, dweight if weight is not None else None, dbias if bias is not None else None,
                              dpw if post_weight is not None else None, dpb if post_bias is not None else None, dgate)
 
@@ -315,6 +319,46 @@ def residual_norm(x: Tensor, y: Tensor, *, norm: str = "rms", post_norm: bool = 
 
 
 # ---- the loss of a large vocabulary ----------------------------------------------------------------------------------
+class _ErrorWords:
+    """A word of pinned host memory for each device, which the kernels write when something is wrong and the host reads
+    at any time, without a copy or an event: the calls that follow (or check_errors) raise."""
+
+    def __init__(self):
+        self.words = {}
+
+    def get(self, device):
+        w = self.words.get(device)
+        if w is None:
+            t = torch.zeros(1, dtype=torch.int32).pin_memory()
+            w = self.words[device] = (t, ctypes.c_int.from_address(t.data_ptr()), t.data_ptr())
+        if w[1].value:
+            _fail(f"an earlier linear_cross_entropy reported: {_capi.describe_err(w[1].value)}")
+        return w[2]
+
+    def check(self):
+        for device in list(self.words):
+            torch.cuda.synchronize(device)
+            self.get(device)
+
+    def reset(self):
+        for device, w in self.words.items():
+            torch.cuda.synchronize(device)
+            w[1].value = 0
+
+
+_ERRORS = _ErrorWords()
+
+
+def check_errors():
+    """Waits for the devices' work and raises RuntimeError if a kernel of this module reported an error."""
+    _ERRORS.check()
+
+
+def reset_errors():
+    """Waits and clears what was reported, so that later calls run again."""
+    _ERRORS.reset()
+
+
 def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes):
     code = _elements(h, "h")
     if reduction not in _REDUCTIONS:
@@ -322,38 +366,37 @@ def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduc
     if w.dim() != 2 or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
         _fail("h (..., d) and w (v, d) must share d")
     _like(w, h, "w")
-    if target.shape != h.shape[:-1] or target.dtype != torch.int64 or target.device != h.device:
+    if target.shape != h.shape[:-1] or target.dtype != torch.int64 or not target.is_cuda or target.get_device() != h.get_device():
         _fail("target must hold one int64 value for each row of h, on its device")
     if not 0.0 <= label_smoothing <= 1.0:
         _fail("label_smoothing must lie in [0, 1]")
     v, d = w.shape
-    h2, w2, t = _rows(h, d, "h"), _rows(w, d, "w"), target.contiguous()
-    n = h2.shape[0]
+    (h2, ld_h), (w2, ld_w), t = _rows(h, d), _rows(w, d), target.contiguous()
+    n = h2.numel() // d
     none = reduction == "none"
     if grad is not None:
-        if grad.dtype != torch.float32 or grad.device != h.device or grad.shape != (target.shape if none else ()):
+        if grad.dtype != torch.float32 or grad.get_device() != h.get_device() or grad.shape != (target.shape if none else ()):
             _fail("grad must be fp32 on the inputs' device: a scalar, or one value for each row with reduction 'none'")
         grad = grad.contiguous()
-    loss = torch.empty(target.shape if none else (), dtype=torch.float32, device=h.device)
-    dh = torch.empty(h.shape, dtype=h.dtype, device=h.device) if grads else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=h.device) if grads else None
+    loss = target.new_empty(target.shape if none else (), dtype=torch.float32)
+    dh, dw = (_new(h), _new(w)) if grads else (None, None)
     if n == 0:
         for x in (loss, dw):
             if x is not None:
                 x.zero_()
         return loss, dh, dw
-    s = _capi.Lce()
-    s.h, s.w, s.target, s.grad, s.loss, s.dh, s.dw = (_ptr(x) for x in (h2, w2, t, grad, loss, dh, dw))
-    s.ld_h, s.ld_w, s.n, s.d, s.v, s.dtype = max(h2.stride(0), d), max(w2.stride(0), d), n, d, v, code
-    s.reduction, s.grads, s.ignore_index = _REDUCTIONS[reduction], int(grads), ignore_index
-    s.label_smoothing, s.z_loss, s.piece_bytes = label_smoothing, z_loss, piece_bytes
-    with _On(h), ops._call(h) as err:
-        L = _capi.lib()
-        size = L.psgd_lce_workspace(ctypes.byref(s))
-        check(min(size, 0), "psgd_lce_workspace")
-        ws = torch.empty(size, dtype=torch.uint8, device=h.device)
-        s.workspace, s.workspace_bytes = ws.data_ptr(), size
-        check(L.psgd_lce(ctypes.byref(s), err.data_ptr(), _stream(h)), "psgd_lce")
+    index = h.get_device()
+    err = _ERRORS.get(index)
+    s = _capi.Lce(h2.data_ptr(), w2.data_ptr(), t.data_ptr(), _ptr(grad), loss.data_ptr(), _ptr(dh), _ptr(dw), None,
+                  ld_h, ld_w, ignore_index, 0, piece_bytes, n, d, v, code,
+                  _REDUCTIONS[reduction], grads, label_smoothing, z_loss)
+    L = _capi.lib()
+    size = L.psgd_lce_workspace(ctypes.byref(s))
+    if size < 0:
+        check(size, "psgd_lce_workspace")
+    ws = h.new_empty((size,), dtype=torch.uint8)
+    s.workspace, s.workspace_bytes = ws.data_ptr(), size
+    _launch(index, L.psgd_lce, ctypes.byref(s), err)
     return loss, dh, dw
 
 
