@@ -82,19 +82,19 @@ PSGD_DEVI void store_any(void* p, int dtype, long long i, float v) {
 // at least the threshold T = round(65536 p). Sixteen bits an element halve the generator's work against one word an
 // element; the kept values are scaled by 1 / (1 - T / 65536), the inverse of the probability that is really used.
 struct Keep {
-  uint32_t o0, o1, threshold;
-  PhiloxKeys keys;
+  uint32_t o0, o1, k0, k1, threshold;
   PSGD_DEVI Keep(unsigned long long seed, unsigned long long offset, const long long* rng, uint32_t t) : threshold(t) {
     if (rng) {
       seed = (unsigned long long)rng[0];
       offset = (unsigned long long)rng[1];
     }
-    keys = philox_keys((uint32_t)seed, (uint32_t)(seed >> 32));
+    k0 = (uint32_t)seed;
+    k1 = (uint32_t)(seed >> 32);
     o0 = (uint32_t)offset;
     o1 = (uint32_t)(offset >> 32);
   }
   PSGD_DEVI uint4 block(unsigned long long b) const {
-    return philox4x32_10(make_uint4((uint32_t)b, (uint32_t)(b >> 32), o0, o1), keys);
+    return philox4x32_10(make_uint4((uint32_t)b, (uint32_t)(b >> 32), o0, o1), k0, k1);
   }
   // bit f: field f of the block is kept
   PSGD_DEVI uint32_t mask8(unsigned long long b) const {

@@ -21,17 +21,17 @@ constexpr int JOINT_MAX_D = PSGD_JOINT_MAX_D;
 constexpr int JOINT_MAX_GROUPS = 8;  // of a block
 constexpr int JOINT_MAX_THREADS = 512;
 // Kernels by the elements that a thread has of a row and the threads of a block: 8 (rows of up to 256 elements, a warp
-// each), 16 (up to 4096, 256 threads), 16 (beyond, 512 threads, whose registers no longer hold a layer norm's sums).
-enum JointWidth { W8 = 0, W16 = 1, W16_512 = 2 };
+// each), 16 (up to 2048 elements: 128 threads; up to 4096: 256; beyond: 512, whose registers do not hold all the sums).
+enum JointWidth { W8 = 0, W16 = 1, W16_256 = 2, W16_512 = 3 };
 PSGD_HD constexpr int width_nv(int w) { return w == W8 ? 1 : 2; }
-PSGD_HD constexpr int width_threads(int w) { return w == W16_512 ? 512 : 256; }
+PSGD_HD constexpr int width_threads(int w) { return w == W16_512 ? 512 : w == W16_256 ? 256 : 128; }
 
 // How rows are dealt out to blocks: consecutive ones, `per_block` each. With a gate a block holds whole gate groups
 // (chunks = 0: a group of threads takes a gate group at a time and writes its gradient itself) or a chunk of one gate
 // group (`chunks` to a gate group). A group of threads takes every blockDim.y-th row (gate group) of its block.
 struct JointPlan {
   int blocks, per_block, chunks, per_gate;
-  int tpr, groups, vec, nv, wide, stages, smem;
+  int tpr, groups, vec, nv, wide, stages, ring, smem;  // ring: bytes of shared memory before the backward pass's columns
   int slot[5];  // of dweight, dbias, dpost_weight, dpost_bias, dgate in `part` [slot][block][d up to 8], or -1
   int slots;
 };
@@ -194,6 +194,7 @@ PSGD_DEVI F2 select2(F2 a, uint32_t mask, int k) {  // elements k, k + 1 of 8, z
 // places of warps that are not there stay zero.
 template <int N, int WARPS>
 struct GroupSum {
+  static_assert(WARPS % 4 == 0, "sums are read four at a time");
   static constexpr int FLOATS = 2 * JOINT_MAX_GROUPS * WARPS * N;
   float* at;
   int tpr, turn;
@@ -294,10 +295,12 @@ struct Ring16 {
 // ---- forward ----------------------------------------------------------------------------------------------------------
 constexpr int F_POST = 1, F_GATE = 2, F_LAYER = 4, F_DROP = 8, F_DIRECT = 16, F_RUNTIME = 32;
 
+PSGD_HD constexpr int joint_forward_blocks(int w, int f) { return w == W8 ? 7 : w == W16 ? ((f & F_LAYER) || (f & F_RUNTIME) ? 3 : 4) : 1; }
+
 // What is constant along a column is formed once: f = scale gate post_weight (and with it the post norm's bias), with the
 // gate where it has one row; other gates multiply row by row.
 template <typename T, bool VEC, int W, int F>
-__global__ void __launch_bounds__(width_threads(W), W == W8 ? 3 : 1) joint_forward_kernel(const PsgdJoint j, const JointPlan p) {
+__global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) joint_forward_kernel(const PsgdJoint j, const JointPlan p) {
   constexpr int NV = width_nv(W), P = NV * 4;
   const bool post = F & F_RUNTIME ? j.post != 0 : bool(F & F_POST);
   const bool layer = F & F_RUNTIME ? j.kind == PSGD_NORM_LAYER : bool(F & F_LAYER);
@@ -474,10 +477,35 @@ struct JointRows {  // a group's rows: every groups-th one, or (direct) every gr
   }
 };
 
-// Blocks that an SM has to hold: three of 256 threads where what a thread keeps fits in 84 registers.
+// Blocks that an SM has to hold, as many as the registers that a thread needs allow.
 PSGD_HD constexpr int joint_min_blocks(int w, int f) {
-  return w == W16_512 ? 1 : w == W16 ? 1 : (f & F_RUNTIME) ? 2 : (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER)) ? 2 : 3;
+  const bool heavy = (f & F_RUNTIME) || (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER));
+  return w == W8 ? (heavy ? 4 : 6) : w == W16 ? (heavy ? 2 : (f & F_POST) || (f & F_GATE) ? 3 : 4) : 1;
 }
+
+// A thread's own copies of column vectors in shared memory: what each row needs once costs a load there, not registers.
+template <int P>
+struct Columns {
+  uint32_t base, apart;
+  PSGD_DEVI Columns(uint32_t at, int index) {
+    apart = blockDim.x * blockDim.y * 16;
+    base = at + index * (P / 2) * apart + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+  }
+  PSGD_DEVI void put(int i, const F2* v) const {  // the four pairs of vector i
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("st.shared.v2.b64 [%0], {%1, %2};" ::"r"(base + (i * 2 + k) * apart), "l"(v[2 * k].v), "l"(v[2 * k + 1].v)
+                   : "memory");
+  }
+  PSGD_DEVI void get(int i, F2* v) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];"
+                   : "=l"(v[2 * k].v), "=l"(v[2 * k + 1].v)
+                   : "r"(base + (i * 2 + k) * apart)
+                   : "memory");
+  }
+};
 
 template <typename T, bool VEC, int W, int F>
 __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
@@ -499,7 +527,8 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
   Sum sum(red);
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
-  Ring16<T, NV, 4> ring(smem, p.stages);
+  constexpr int ARRAYS = RT || (F & (F_POST | F_GATE)) ? 4 : 3;  // d_normed, d_out, out and, where it is needed, y
+  Ring16<T, NV, ARRAYS> ring(smem, p.stages);
 
   JointRows it;
   it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
@@ -544,13 +573,20 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
     rows[3] = use_y ? reinterpret_cast<const T*>(j.y) + row * ld_y : nullptr;
   };
 
-  F2 dw[P], db[P], A[P], B[P], dpw[P], dpb[P], w[P], f[P];
+  F2 dw[P], db[P], A[P], B[P], dpw[P], dpb[P];
+  const bool scaled = post || gate;  // f is not one number
+  const Columns<P> ws(smem_u32(smem) + p.ring, 0), fs(smem_u32(smem) + p.ring, 1);
 #pragma unroll
   for (int k = 0; k < P; ++k) dw[k] = db[k] = A[k] = B[k] = dpw[k] = dpb[k] = f2(0.f);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    at.template param<T>(j.weight, j.param_dtype, 1.f, i, w + i * 4);
-    if (!direct) column_factor(gate_row, i, f + i * 4);
+    F2 v[4];
+    at.template param<T>(j.weight, j.param_dtype, 1.f, i, v);
+    ws.put(i, v);
+    if (scaled && !direct) {
+      column_factor(gate_row, i, v);
+      fs.put(i, v);
+    }
   }
 
   JointRows ahead = it;
@@ -604,13 +640,19 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
     {
       const F2 r = f2(st.w), m = f2(-st.z * st.w);
 #pragma unroll
-      for (int k = 0; k < P; ++k) {
-        hat[k] = layer ? fma2(hat[k], r, m) : mul2(hat[k], r);
-        dw[k] = fma2(dn[k], hat[k], dw[k]);
-        if (layer) db[k] = add2(db[k], dn[k]);
-        dn[k] = mul2(dn[k], w[k]);
-        s0 = fma2(dn[k], hat[k], s0);
-        if (layer) s1 = add2(s1, dn[k]);
+      for (int i = 0; i < NV; ++i) {
+        F2 w[4];
+        ws.get(i, w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = i * 4 + e;
+          hat[k] = layer ? fma2(hat[k], r, m) : mul2(hat[k], r);
+          dw[k] = fma2(dn[k], hat[k], dw[k]);
+          if (layer) db[k] = add2(db[k], dn[k]);
+          dn[k] = mul2(dn[k], w[e]);
+          s0 = fma2(dn[k], hat[k], s0);
+          if (layer) s1 = add2(s1, dn[k]);
+        }
       }
     }
     float s[2] = {sum2(s0), sum2(s1)};
@@ -628,7 +670,11 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
     }
     if (direct && fresh) {
 #pragma unroll
-      for (int i = 0; i < NV; ++i) column_factor(it.g, i, f + i * 4);
+      for (int i = 0; i < NV; ++i) {
+        F2 v[4];
+        column_factor(it.g, i, v);
+        fs.put(i, v);
+      }
     }
     const F2 r = f2(st.w), c1 = f2(-s[0] * inv_d), c2 = f2(layer ? -s[1] * inv_d : 0.f);
     const F2 ry = f2(st.y), my = f2(-st.x * st.y);
@@ -645,6 +691,11 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
         dx[n] = fma2(r, t, dx[n]);
       }
       at.store(reinterpret_cast<T*>(j.dx) + (long long)row * d, i, dx + i * 4);
+      F2 f[4];
+      if (scaled) fs.get(i, f);
+      else
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = f2(c);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int n = i * 4 + k;
@@ -660,7 +711,7 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
           A[n] = fma2(m, y[n], A[n]);
         }
         if (post && layer) B[n] = add2(B[n], m);
-        dx[n] = mul2(m, f[n]);
+        dx[n] = mul2(m, f[k]);
         if (post) {
           s0 = fma2(dx[n], y[n], s0);
           if (layer) s1 = add2(s1, dx[n]);
@@ -821,6 +872,9 @@ int joint_forward_of(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream
     case W8: return p.vec ? joint_forward_pick<T, W8>(f, j, p, stream) : joint_forward_launch<T, false, W8, F_RUNTIME>(j, p, stream);
     case W16:
       return p.vec ? joint_forward_pick<T, W16>(f, j, p, stream) : joint_forward_launch<T, false, W16, F_RUNTIME>(j, p, stream);
+    case W16_256:
+      return p.vec ? joint_forward_pick<T, W16_256>(f, j, p, stream)
+                   : joint_forward_launch<T, false, W16_256, F_RUNTIME>(j, p, stream);
     default:
       return p.vec ? joint_forward_launch<T, true, W16_512, F_RUNTIME>(j, p, stream)
                    : joint_forward_launch<T, false, W16_512, F_RUNTIME>(j, p, stream);
@@ -837,6 +891,9 @@ int joint_backward_of(const PsgdJoint& j, const JointPlan& p, float* part, cudaS
     case W16:
       return p.vec ? joint_backward_pick<T, W16>(f, j, p, part, stream)
                    : joint_backward_launch<T, false, W16, F_RUNTIME>(j, p, part, stream);
+    case W16_256:
+      return p.vec ? joint_backward_pick<T, W16_256>(f, j, p, part, stream)
+                   : joint_backward_launch<T, false, W16_256, F_RUNTIME>(j, p, part, stream);
     default:
       return p.vec ? joint_backward_launch<T, true, W16_512, F_RUNTIME>(j, p, part, stream)
                    : joint_backward_launch<T, false, W16_512, F_RUNTIME>(j, p, part, stream);

@@ -66,20 +66,18 @@ bool valid(const PsgdJoint& j) {
 
 // The block's shape, and as many groups as fill a block of 128 threads.
 void shape(int d, JointPlan& p) {
-  p.wide = d <= 256 ? W8 : d <= 4096 ? W16 : W16_512;
+  p.wide = d <= 256 ? W8 : d <= 2048 ? W16 : d <= 4096 ? W16_256 : W16_512;
   p.nv = width_nv(p.wide);
   p.tpr = round_up((d + 8 * p.nv - 1) / (8 * p.nv), 32);
   p.groups = 128 / p.tpr;
   p.groups = p.groups < 1 ? 1 : p.groups > JOINT_MAX_GROUPS ? JOINT_MAX_GROUPS : p.groups;
 }
 
-// Blocks that an SM holds at once, by the shared memory and registers that a thread takes.
-int per_sm(const JointPlan& p, int regs) {
-  const int threads = p.tpr * p.groups;
-  int n = 65536 / (threads * regs);
-  const int by_smem = 220 * 1024 / (p.smem + 3 * 1024);
-  n = n < by_smem ? n : by_smem;
-  n = n < 2048 / threads ? n : 2048 / threads;
+// Blocks that an SM holds at once: as many as the kernel was compiled for, and as the shared memory allows.
+int per_sm(const JointPlan& p, int compiled) {
+  const int threads = p.tpr * p.groups, by_regs = compiled * width_threads(p.wide) / threads;
+  const int by_smem = 220 * 1024 / (p.smem + 2 * 1024);
+  const int n = by_regs < by_smem ? by_regs : by_smem;
   return n < 1 ? 1 : n;
 }
 
@@ -92,7 +90,7 @@ JointPlan plan_forward(const PsgdJoint& j) {
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
   p.smem = p.vec ? p.stages * 2 * p.nv * p.tpr * p.groups * 8 * size_of(j.dtype) : 0;
   p.per_gate = j.gate ? (int)(j.rows / j.gates) : 1;
-  const int want = ((int)j.rows + p.groups - 1) / p.groups, most = per_sm(p, p.wide == W8 ? 64 : 112) * psgd_num_sms();
+  const int want = ((int)j.rows + p.groups - 1) / p.groups, most = per_sm(p, joint_forward_blocks(p.wide, joint_flags(j, p))) * psgd_num_sms();
   p.blocks = want < most ? want : most;
   return p;
 }
@@ -109,15 +107,18 @@ JointPlan plan_backward(const PsgdJoint& j) {
   const bool layer = j.kind == PSGD_NORM_LAYER;
   const bool there[5] = {true, layer, j.post != 0, j.post && layer, j.gate != nullptr};
   for (int a = 0; a < 5; ++a) p.slot[a] = there[a] ? p.slots++ : -1;
+  // Rows ahead: two for 16-bit types, one for fp32, as far as shared memory goes.
+  const int f = (joint_flags(j, p) & ~F_DIRECT) | (p.vec ? 0 : F_RUNTIME), blocks = joint_min_blocks(p.wide, f);
+  const int threads = p.tpr * p.groups, columns = threads * p.nv * 64;
+  const int arrays = p.wide == W16_512 || j.post || j.gate ? 4 : 3;
+  const int row = arrays * p.nv * threads * 8 * size_of(j.dtype), room = 216 * 1024 / blocks - columns - 2 * 1024;
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
-  const int row = 4 * p.nv * p.tpr * p.groups * 8 * size_of(j.dtype);
-  while (p.stages > 1 && p.stages * row > 200 * 1024) --p.stages;  // (fp32 rows of over 6144 elements: one row at a time)
-  p.smem = p.vec ? p.stages * row : 0;
+  while (p.stages > 1 && p.stages * row > room) --p.stages;
+  p.ring = p.vec ? p.stages * row : 0;
+  p.smem = p.ring + columns;
   const int share = (p.groups - 1) * round_up(j.d, 8) * 4;
   if (p.smem < share) p.smem = share;
-  const int f = joint_flags(j, p) & ~F_DIRECT;
-  const int regs = p.wide == W8 && p.vec ? 65536 / (256 * joint_min_blocks(W8, f)) : p.wide == W16 ? 168 : 128;
-  const int most = psgd_num_sms() * per_sm(p, regs), rows = (int)j.rows;
+  const int most = psgd_num_sms() * per_sm(p, blocks), rows = (int)j.rows;
   p.per_block = (rows + most - 1) / most;
   if (p.per_block < p.groups) p.per_block = p.groups;
   p.per_gate = 1;

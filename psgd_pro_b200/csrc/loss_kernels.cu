@@ -252,8 +252,9 @@ PSGD_DEVI LceUnit lce_unit(const LceProblem& p, const LceShape& s, int u) {
   const int in = t - band * L_GROUP_M * s.tiles_n;
   x.tn = in / h;
   x.tm = m0 + in - x.tn * h;
-  x.k0 = (int)((long long)s.kblocks * x.split / p.splits);
-  x.k1 = (int)((long long)s.kblocks * (x.split + 1) / p.splits);
+  const int more = s.kblocks - s.unit_kblocks * p.splits;  // splits of unit_kblocks, the first ones of one more
+  x.k0 = x.split * s.unit_kblocks + min(x.split, more);
+  x.k1 = x.k0 + s.unit_kblocks + (x.split < more);
   return x;
 }
 
