@@ -5,55 +5,78 @@
 namespace psgd {
 namespace {
 
-constexpr int DROP_THREADS = 256;
+constexpr int DROP_THREADS = 256, DROP_UNROLL = 2, DROP_BLOCKS = 4;  // (blocks of an SM)
 
-// One generator block (8 elements) a thread and turn. VEC: every pointer is 16-byte aligned, so whole blocks move as
-// vectors; the last, partial block (and every block without VEC) goes element by element.
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(DROP_THREADS) dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual,
-                                                               T* __restrict__ out, long long n, uint32_t threshold,
-                                                               float scale, unsigned long long seed,
-                                                               unsigned long long offset, const long long* rng) {
+// A generator block (8 elements) at a time, DROP_UNROLL of them DROP_THREADS apart so that their loads are under way
+// together. VEC: every pointer is 16-byte aligned and whole blocks move as vectors; the last, partial block (and all
+// without VEC) goes element by element.
+template <typename T, bool VEC, bool RESIDUAL>
+__global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS)
+    dropout_kernel(const T* __restrict__ x, const T* __restrict__ residual, T* __restrict__ out, long long n,
+                   uint32_t threshold, float scale, unsigned long long seed, unsigned long long offset,
+                   const long long* rng) {
+  constexpr int H = sizeof(T) / 2;  // 16-byte pieces to 8 elements
   const Keep keep(seed, offset, rng, threshold);
-  const long long blocks = (n + 7) / 8;
-  for (long long b = (long long)blockIdx.x * DROP_THREADS + threadIdx.x; b < blocks;
-       b += (long long)gridDim.x * DROP_THREADS) {
-    const uint32_t m = keep.mask8((unsigned long long)b);
-    const long long at = 8 * b;
-    if (VEC && at + 8 <= n) {
-      float v[8], r[8];
-      load_vec<T, 8>(x + at, v);
-      if (residual) load_vec<T, 8>(residual + at, r);
+  const long long whole = VEC ? n / 8 : 0, step = (long long)gridDim.x * DROP_THREADS * DROP_UNROLL;
+  for (long long b0 = (long long)blockIdx.x * DROP_THREADS * DROP_UNROLL + threadIdx.x; b0 < whole; b0 += step) {
+    uint4 v[DROP_UNROLL][H], r[DROP_UNROLL][H];
+#pragma unroll
+    for (int u = 0; u < DROP_UNROLL; ++u) {
+      const long long b = b0 + u * DROP_THREADS;
+      if (b < whole)
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          v[u][h] = reinterpret_cast<const uint4*>(x)[b * H + h];
+          if (RESIDUAL) r[u][h] = reinterpret_cast<const uint4*>(residual)[b * H + h];
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < DROP_UNROLL; ++u) {
+      const long long b = b0 + u * DROP_THREADS;
+      if (b >= whole) break;
+      const uint4 words = keep.block((unsigned long long)b);
+      float f[8], add[8];
+      unpack_pieces<T>(v[u], f);
+      if (RESIDUAL) unpack_pieces<T>(r[u], add);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        v[i] = (m >> i) & 1u ? v[i] * scale : 0.f;
-        if (residual) v[i] += r[i];
+        const uint32_t w = word_of(words, i / 2);
+        f[i] = (i & 1 ? keep.high(w) : keep.low(w)) ? f[i] * scale : 0.f;
+        if (RESIDUAL) f[i] += add[i];
       }
-      store_vec<T, 8>(out + at, v);
-    } else {
-      for (int i = 0; i < 8 && at + i < n; ++i) {
-        float v = (m >> i) & 1u ? to_f32(x[at + i]) * scale : 0.f;
-        if (residual) v += to_f32(residual[at + i]);
-        out[at + i] = from_f32<T>(v);
-      }
+      store_vec<T, 8>(out + 8 * b, f);
     }
   }
+  const long long blocks = (n + 7) / 8;
+  for (long long b = whole + (long long)blockIdx.x * DROP_THREADS + threadIdx.x; b < blocks;
+       b += (long long)gridDim.x * DROP_THREADS) {
+    const uint4 words = keep.block((unsigned long long)b);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const long long at = 8 * b + i;
+      if (at >= n) break;
+      const uint32_t w = word_of(words, i / 2);
+      float f = (i & 1 ? keep.high(w) : keep.low(w)) ? to_f32(x[at]) * scale : 0.f;
+      if (RESIDUAL) f += to_f32(residual[at]);
+      out[at] = from_f32<T>(f);
+    }
+  }
+}
+
+template <typename T, bool VEC, bool RESIDUAL>
+int start(const PsgdDropout& d, cudaStream_t stream) {
+  const long long want = ((d.n + 7) / 8 + DROP_THREADS - 1) / DROP_THREADS, most = (long long)DROP_BLOCKS * psgd_num_sms();
+  dropout_kernel<T, VEC, RESIDUAL><<<(int)(want < most ? want : most), DROP_THREADS, 0, stream>>>(
+      reinterpret_cast<const T*>(d.x), reinterpret_cast<const T*>(d.residual), reinterpret_cast<T*>(d.out), d.n, d.threshold,
+      d.scale, d.seed, d.offset, d.rng);
+  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
 }
 
 template <typename T>
 int launch(const PsgdDropout& d, cudaStream_t stream) {
   const bool vec = aligned16(d.x) && aligned16(d.out) && aligned16(d.residual);
-  const long long blocks = (d.n + 7) / 8, want = (blocks + DROP_THREADS - 1) / DROP_THREADS;
-  const long long most = 8LL * psgd_num_sms();
-  const int grid = (int)(want < most ? want : most);
-  const T* x = reinterpret_cast<const T*>(d.x);
-  const T* r = reinterpret_cast<const T*>(d.residual);
-  T* out = reinterpret_cast<T*>(d.out);
-  if (vec)
-    dropout_kernel<T, true><<<grid, DROP_THREADS, 0, stream>>>(x, r, out, d.n, d.threshold, d.scale, d.seed, d.offset, d.rng);
-  else
-    dropout_kernel<T, false><<<grid, DROP_THREADS, 0, stream>>>(x, r, out, d.n, d.threshold, d.scale, d.seed, d.offset, d.rng);
-  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+  if (d.residual) return vec ? start<T, true, true>(d, stream) : start<T, false, true>(d, stream);
+  return vec ? start<T, true, false>(d, stream) : start<T, false, false>(d, stream);
 }
 
 }  // namespace

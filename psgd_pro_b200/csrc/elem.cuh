@@ -52,6 +52,24 @@ PSGD_DEVI void load_vec(const T* __restrict__ p, float* v) {
     }
   }
 }
+// Eight elements from their 16-byte pieces (one, or two of fp32).
+template <typename T>
+PSGD_DEVI void unpack_pieces(const uint4* p, float* v) {
+#pragma unroll
+  for (int h = 0; h < (int)sizeof(T) / 2; ++h) {
+    const uint32_t w[4] = {p[h].x, p[h].y, p[h].z, p[h].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        v[4 * h + i] = __uint_as_float(w[i]);
+      } else {
+        const float2 f = unpack2(w[i], T());
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+}
 template <typename T, int V>
 PSGD_DEVI void store_vec(T* p, const float* v) {
   if constexpr (V == 1) {
@@ -82,8 +100,9 @@ PSGD_DEVI void store_any(void* p, int dtype, long long i, float v) {
 // at least the threshold T = round(65536 p). Sixteen bits an element halve the generator's work against one word an
 // element; the kept values are scaled by 1 / (1 - T / 65536), the inverse of the probability that is really used.
 struct Keep {
-  uint32_t o0, o1, k0, k1, threshold;
-  PSGD_DEVI Keep(unsigned long long seed, unsigned long long offset, const long long* rng, uint32_t t) : threshold(t) {
+  uint32_t o0, o1, k0, k1, limit;  // limit: T << 16, which a word is compared with for its high field, shifted for its low one
+  bool none;                       // T = 65536: nothing is kept (words of zeros stay below every limit)
+  PSGD_DEVI Keep(unsigned long long seed, unsigned long long offset, const long long* rng, uint32_t threshold) {
     if (rng) {
       seed = (unsigned long long)rng[0];
       offset = (unsigned long long)rng[1];
@@ -92,24 +111,36 @@ struct Keep {
     k1 = (uint32_t)(seed >> 32);
     o0 = (uint32_t)offset;
     o1 = (uint32_t)(offset >> 32);
+    none = threshold > 65535u;
+    limit = none ? 0xFFFFFFFFu : threshold << 16;
   }
   PSGD_DEVI uint4 block(unsigned long long b) const {
+    if (none) return make_uint4(0u, 0u, 0u, 0u);
     return philox4x32_10(make_uint4((uint32_t)b, (uint32_t)(b >> 32), o0, o1), k0, k1);
   }
-  // bit f: field f of the block is kept
-  PSGD_DEVI uint32_t mask8(unsigned long long b) const {
-    const uint4 r = block(b);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    uint32_t m = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      m |= ((w[i] & 0xFFFFu) >= threshold ? 1u : 0u) << (2 * i);
-      m |= ((w[i] >> 16) >= threshold ? 1u : 0u) << (2 * i + 1);
-    }
-    return m;
+  PSGD_DEVI bool low(uint32_t word) const { return (word << 16) >= limit; }   // fields 0, 2, 4, 6
+  PSGD_DEVI bool high(uint32_t word) const { return word >= limit; }          // fields 1, 3, 5, 7
+  PSGD_DEVI bool one(unsigned long long i) const {
+    const uint4 r = block(i >> 3);
+    const uint32_t k = (uint32_t)i & 7u, w = k < 2 ? r.x : k < 4 ? r.y : k < 6 ? r.z : r.w;
+    return k & 1u ? high(w) : low(w);
   }
-  PSGD_DEVI bool one(unsigned long long i) const { return (mask8(i >> 3) >> (i & 7)) & 1u; }
 };
+PSGD_DEVI uint32_t word_of(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+
+// A launch that may start while the one before it ends (its kernel waits for that one by pdl_wait before it reads anything).
+template <typename... P, typename... A>
+int pdl_launch(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t stream, A&&... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = smem, c.stream = stream;
+  cudaLaunchAttribute at = {};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &at, c.numAttrs = 1;
+  if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess) return PSGD_OK;
+  cudaGetLastError();  // else it would be taken for a later launch's
+  return PSGD_ELAUNCH;
+}
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

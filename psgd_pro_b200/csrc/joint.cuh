@@ -18,7 +18,7 @@
 namespace psgd {
 
 constexpr int JOINT_MAX_D = PSGD_JOINT_MAX_D;
-constexpr int JOINT_MAX_GROUPS = 8;  // of a block
+constexpr int JOINT_MAX_GROUPS = 8;  // of a block, where a group has more than a warp
 constexpr int JOINT_MAX_THREADS = 512;
 // Kernels by the elements that a thread has of a row and the threads of a block: 8 (rows of up to 256 elements, a warp
 // each), 16 (up to 2048 elements: 128 threads; up to 4096: 256; beyond: 512, whose registers do not hold all the sums).
@@ -28,7 +28,7 @@ PSGD_HD constexpr int width_threads(int w) { return w == W16_512 ? 512 : w == W1
 
 // How rows are dealt out to blocks: consecutive ones, `per_block` each. With a gate a block holds whole gate groups
 // (chunks = 0: a group of threads takes a gate group at a time and writes its gradient itself) or a chunk of one gate
-// group (`chunks` to a gate group). A group of threads takes every blockDim.y-th row (gate group) of its block.
+// group (`chunks` to a gate group, whose gradient a block writes itself if there is one). A group of threads takes every blockDim.y-th row (gate group) of its block.
 struct JointPlan {
   int blocks, per_block, chunks, per_gate;
   int tpr, groups, vec, nv, wide, stages, ring, smem;  // ring: bytes of shared memory before the backward pass's columns
@@ -170,24 +170,30 @@ struct Place {
       load(reinterpret_cast<const T*>(p), i, v);
     }
   }
-  // Bit k: element k is kept by dropout.
-  PSGD_DEVI uint32_t kept(const Keep& keep, long long row, int i) const {
+  // v with what dropout does not keep set to zero.
+  PSGD_DEVI void drop(const Keep& keep, long long row, int i, F2* v) const {
     const unsigned long long at0 = (unsigned long long)row * d;
     if constexpr (VEC) {
-      return keep.mask8((at0 + e(i)) >> 3);
+      const uint4 words = keep.block((at0 + e(i)) >> 3);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t w = word_of(words, k);
+        const float2 f = un2(v[k]);
+        v[k] = f2(keep.low(w) ? f.x : 0.f, keep.high(w) ? f.y : 0.f);
+      }
     } else {
       uint32_t m = 0;
 #pragma unroll 1
       for (int k = 0; k < 8; ++k)
         if (has(i, k)) m |= (uint32_t)keep.one(at0 + at(i, k)) << k;
-      return m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = un2(v[k]);
+        v[k] = f2((m >> (2 * k)) & 1u ? f.x : 0.f, (m >> (2 * k + 1)) & 1u ? f.y : 0.f);
+      }
     }
   }
 };
-PSGD_DEVI F2 select2(F2 a, uint32_t mask, int k) {  // elements k, k + 1 of 8, zero where dropped
-  const float2 f = un2(a);
-  return f2((mask >> k) & 1u ? f.x : 0.f, (mask >> (k + 1)) & 1u ? f.y : 0.f);
-}
 
 // Sum of v[0..N) over the threads of a group of at most WARPS warps. `red` holds two buffers taken in turn: a thread writes
 // one again only after the barrier of the other's sum, which every thread reaches after its reads of the first. The
@@ -426,11 +432,7 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
 #pragma unroll
         for (int k = 0; k < 4; ++k) ui[k] = mul2(ui[k], v[k]);
       }
-      if (drop) {
-        const uint32_t m = at.kept(keep, row, i);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) ui[k] = select2(ui[k], m, 2 * k);
-      }
+      if (drop) at.drop(keep, row, i, ui);
 #pragma unroll
       for (int k = 0; k < 4; ++k) x[i * 4 + k] = add2(x[i * 4 + k], ui[k]);
       at.store(po, i, x + i * 4);
@@ -458,8 +460,8 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
 //   dy = f m, through the post norm as above;  A = sum m yh and B = sum m over rows give
 //   dpost_weight = c gate A, dpost_bias = c gate B, dgate = c (post_weight A + post_bias B): one multiply-add a row for
 //   three gradients. dweight = sum d_normed hat, dbias = sum d_normed.
-// The sums over rows are kept in registers and written once a block, as rows of `part`, which joint_reduce_kernel adds in
-// a fixed order.
+// The sums over rows are kept in registers and written once a block, as rows of `part`, which
+// joint_reduce_kernel adds in a fixed order.
 struct JointRows {  // a group's rows: every groups-th one, or (direct) every groups-th gate group's
   int row, g, end, per_gate, groups;
   bool direct;
@@ -477,10 +479,15 @@ struct JointRows {  // a group's rows: every groups-th one, or (direct) every gr
   }
 };
 
-// Blocks that an SM has to hold, as many as the registers that a thread needs allow.
-PSGD_HD constexpr int joint_min_blocks(int w, int f) {
-  const bool heavy = (f & F_RUNTIME) || (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER));
-  return w == W8 ? (heavy ? 4 : 6) : w == W16 ? (heavy ? 2 : (f & F_POST) || (f & F_GATE) ? 3 : 4) : 1;
+// Threads of a block, and blocks that an SM holds, by the registers that a thread needs. Fewer and larger blocks leave fewer
+// sums over rows to the last step, smaller ones even out the SMs (8192 x 2048, rms: 128 threads 49.5 us, 256 47.3, 512 47.2;
+// 16384 x 1024, layer norm with dropout: 44.8, 45.1, 48.7).
+PSGD_HD constexpr bool joint_heavy(int f) { return (f & F_RUNTIME) || (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER)); }
+PSGD_HD constexpr int joint_backward_threads(int w, int f) {
+  return w == W8 ? 256 : w == W16 ? ((f & F_LAYER) && (f & F_GATE) && !joint_heavy(f) ? 384 : 256) : width_threads(w);
+}
+PSGD_HD constexpr int joint_backward_blocks(int w, int f) {
+  return w == W8 ? (joint_heavy(f) ? 2 : 3) : w == W16 && !joint_heavy(f) && !((f & F_LAYER) && (f & F_GATE)) ? 2 : 1;
 }
 
 // A thread's own copies of column vectors in shared memory: what each row needs once costs a load there, not registers.
@@ -508,7 +515,7 @@ struct Columns {
 };
 
 template <typename T, bool VEC, int W, int F>
-__global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
+__global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_blocks(W, F))
     joint_backward_kernel(const PsgdJoint j, const JointPlan p, float* part) {
   constexpr int NV = width_nv(W), P = NV * 4;
   constexpr bool RT = F & F_RUNTIME;
@@ -524,6 +531,7 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
   __shared__ __align__(16) float red[Sum::FLOATS];
   const int d = j.d, dp = (d + 7) & ~7;
   const Place<VEC> at(d);
+  pdl_trigger();
   Sum sum(red);
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
@@ -681,8 +689,6 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
     s0 = s1 = f2(0.f);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      uint32_t kept = 0xFFu;
-      if (drop && at.any(i)) kept = at.kept(keep, row, i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int n = i * 4 + k;
@@ -696,10 +702,11 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
       else
 #pragma unroll
         for (int k = 0; k < 4; ++k) f[k] = f2(c);
+      if (drop && at.any(i)) at.drop(keep, row, i, dx + i * 4);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int n = i * 4 + k;
-        F2 m = drop ? select2(dx[n], kept, 2 * k) : dx[n];
+        F2 m = dx[n];
         if (!VEC) {  // beyond d, where a layer norm's dx is not zero
           const float2 v = un2(m);
           m = f2(at.has(i, 2 * k) ? v.x : 0.f, at.has(i, 2 * k + 1) ? v.y : 0.f);
@@ -788,31 +795,27 @@ __global__ void __launch_bounds__(width_threads(W), joint_min_blocks(W, F))
       }
     }
   }
-  // The groups' shares are added in their order, through shared memory (the ring is done with).
+  // The groups' shares are added in their order through shared memory, in two buffers in turn, so that one barrier a vector
+  // is enough (a buffer is written again only after the barrier of the vector between, which follows every read of it).
+  // The ring is done with.
   asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
   float* share = reinterpret_cast<float*>(smem);
+  int turn = 0;
   auto write = [&](int a, const F2* v) {
     if (p.slot[a] < 0) return;
-    if (blockDim.y > 1) {
-      __syncthreads();
-      if (threadIdx.y > 0)
+    float* mine = share + turn * blockDim.y * dp;
+    turn ^= 1;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) at.store(share + (threadIdx.y - 1) * dp, i, v + i * 4);
-      __syncthreads();
-      if (threadIdx.y > 0) return;
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      F2 t[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) t[k] = v[i * 4 + k];
-      for (int g = 1; g < (int)blockDim.y; ++g) {
-        F2 o[4];
-        at.load(share + (g - 1) * dp, i, o);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) t[k] = add2(t[k], o[k]);
-      }
-      at.store(part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp, i, t);
+    for (int i = 0; i < NV; ++i) at.store(mine + threadIdx.y * dp, i, v + i * 4);
+    __syncthreads();
+    float* to = part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp;
+    T* whole = a == 4 && p.chunks == 1 ? reinterpret_cast<T*>(j.dgate) + (long long)gate_row * d : nullptr;
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < d; c += blockDim.x * blockDim.y) {
+      float t = mine[c];
+      for (int g = 1; g < (int)blockDim.y; ++g) t += mine[g * dp + c];
+      if (whole) whole[c] = from_f32<T>(t);
+      else to[c] = t;
     }
   };
   write(0, dw);

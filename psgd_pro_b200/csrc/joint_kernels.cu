@@ -23,6 +23,7 @@ __global__ void __launch_bounds__(1024) joint_reduce_kernel(const PsgdJoint j, c
     to = (long long)g * j.d;
   }
   float s[8] = {};
+  pdl_wait();
   if (col < j.d) {
     const float* from = part + (size_t)p.slot[a] * p.blocks * dp + col;
     int b = b0 + threadIdx.y;
@@ -42,6 +43,8 @@ __global__ void __launch_bounds__(1024) joint_reduce_kernel(const PsgdJoint j, c
     else store_any(j.dgate, j.dtype, to + c, v);
   }
 }
+
+constexpr int JOINT_DIRECT_ROWS = 32;
 
 int size_of(int dtype) { return dtype == PSGD_F32 ? 4 : 2; }
 
@@ -64,13 +67,14 @@ bool valid(const PsgdJoint& j) {
   return true;
 }
 
-// The block's shape, and as many groups as fill a block of 128 threads.
-void shape(int d, JointPlan& p) {
+// The kernel for rows of d elements, and as many groups as make up a block of `threads` (of the kernel's width for 0).
+void shape(int d, JointPlan& p, int threads) {
   p.wide = d <= 256 ? W8 : d <= 2048 ? W16 : d <= 4096 ? W16_256 : W16_512;
   p.nv = width_nv(p.wide);
   p.tpr = round_up((d + 8 * p.nv - 1) / (8 * p.nv), 32);
-  p.groups = 128 / p.tpr;
-  p.groups = p.groups < 1 ? 1 : p.groups > JOINT_MAX_GROUPS ? JOINT_MAX_GROUPS : p.groups;
+  p.groups = (threads ? threads : width_threads(p.wide)) / p.tpr;
+  if (p.groups < 1) p.groups = 1;
+  if (p.tpr > 32 && p.groups > JOINT_MAX_GROUPS) p.groups = JOINT_MAX_GROUPS;
 }
 
 // Blocks that an SM holds at once: as many as the kernel was compiled for, and as the shared memory allows.
@@ -86,7 +90,7 @@ JointPlan plan_forward(const PsgdJoint& j) {
   p.vec = j.d % 8 == 0 && params_aligned(j) && rows_aligned(j.x, j.ld_x, j.dtype) && rows_aligned(j.y, j.ld_y, j.dtype) &&
           rows_aligned(j.out, j.d, j.dtype) && rows_aligned(j.normed, j.d, j.dtype) &&
           (!j.gate || rows_aligned(j.gate, j.d, j.dtype));
-  shape(j.d, p);
+  shape(j.d, p, 0);
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
   p.smem = p.vec ? p.stages * 2 * p.nv * p.tpr * p.groups * 8 * size_of(j.dtype) : 0;
   p.per_gate = j.gate ? (int)(j.rows / j.gates) : 1;
@@ -103,33 +107,36 @@ JointPlan plan_backward(const PsgdJoint& j) {
           (!j.d_normed || rows_aligned(j.d_normed, j.ld_d_normed, j.dtype)) &&
           (!(j.post || j.gate) || rows_aligned(j.y, j.ld_y, j.dtype)) &&
           (!j.gate || (rows_aligned(j.gate, j.d, j.dtype) && rows_aligned(j.dgate, j.d, j.dtype)));
-  shape(j.d, p);
+  // Gate groups of few rows are a thread group's each (direct); longer ones are dealt out in chunks.
+  p.per_gate = j.gate ? (int)(j.rows / j.gates) : 1;
+  p.chunks = j.gate && p.per_gate > JOINT_DIRECT_ROWS;  // (how many: below)
+  shape(j.d, p, 0);
+  const int f = joint_flags(j, p) | (p.vec && p.wide != W16_512 ? 0 : F_RUNTIME);
+  shape(j.d, p, joint_backward_threads(p.wide, f));
+  const int rows = (int)j.rows, per_sm = joint_backward_blocks(p.wide, f), most = per_sm * psgd_num_sms();
+  const int fair = (rows + most - 1) / most;
+  if (p.chunks) p.chunks = (p.per_gate + fair - 1) / fair;
   const bool layer = j.kind == PSGD_NORM_LAYER;
   const bool there[5] = {true, layer, j.post != 0, j.post && layer, j.gate != nullptr};
   for (int a = 0; a < 5; ++a) p.slot[a] = there[a] ? p.slots++ : -1;
   // Rows ahead: two for 16-bit types, one for fp32, as far as shared memory goes.
-  const int f = (joint_flags(j, p) & ~F_DIRECT) | (p.vec ? 0 : F_RUNTIME), blocks = joint_min_blocks(p.wide, f);
   const int threads = p.tpr * p.groups, columns = threads * p.nv * 64;
   const int arrays = p.wide == W16_512 || j.post || j.gate ? 4 : 3;
-  const int row = arrays * p.nv * threads * 8 * size_of(j.dtype), room = 216 * 1024 / blocks - columns - 2 * 1024;
+  const int row = arrays * p.nv * threads * 8 * size_of(j.dtype), room = 220 * 1024 / per_sm - columns;
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
   while (p.stages > 1 && p.stages * row > room) --p.stages;
   p.ring = p.vec ? p.stages * row : 0;
   p.smem = p.ring + columns;
-  const int share = (p.groups - 1) * round_up(j.d, 8) * 4;
+  const int share = 2 * p.groups * round_up(j.d, 8) * 4;
   if (p.smem < share) p.smem = share;
-  const int most = psgd_num_sms() * per_sm(p, blocks), rows = (int)j.rows;
-  p.per_block = (rows + most - 1) / most;
-  if (p.per_block < p.groups) p.per_block = p.groups;
-  p.per_gate = 1;
-  if (j.gate) {
-    p.per_gate = (int)(j.rows / j.gates);
-    if (p.per_gate <= p.per_block) {
-      p.per_block = (p.per_block + p.per_gate - 1) / p.per_gate * p.per_gate;
-    } else {
-      p.chunks = (p.per_gate + p.per_block - 1) / p.per_block;
-      p.per_block = (p.per_gate + p.chunks - 1) / p.chunks;
-    }
+  if (p.chunks) {
+    p.per_block = (p.per_gate + p.chunks - 1) / p.chunks;
+  } else if (j.gate) {
+    int held = fair / p.per_gate;  // gate groups of a block: a multiple of its thread groups where there are enough
+    held = held < 1 ? 1 : held > p.groups ? (held + p.groups - 1) / p.groups * p.groups : held;
+    p.per_block = held * p.per_gate;
+  } else {
+    p.per_block = fair < p.groups ? p.groups : fair;
   }
   p.blocks = p.chunks ? (int)j.gates * p.chunks : (rows + p.per_block - 1) / p.per_block;
   return p;
@@ -169,7 +176,6 @@ extern "C" int psgd_joint_backward(const PsgdJoint* j, void* workspace, long lon
   if (((j->post || j->gate) && !j->y) || (p.slot[1] >= 0 && !j->dbias) || (p.slot[2] >= 0 && !j->dpost_weight) ||
       (p.slot[3] >= 0 && !j->dpost_bias) || (p.slot[4] >= 0 && !j->dgate))
     return PSGD_EINVAL;
-  if (p.chunks && j->gates > 65000) return PSGD_EINVAL;  // (their rows would be over 2^30)
   if (bytes < (long long)p.slots * p.blocks * round_up(j->d, 8) * 4) return PSGD_ESPACE;
   float* part = reinterpret_cast<float*>(workspace);
   int rc;
@@ -179,7 +185,7 @@ extern "C" int psgd_joint_backward(const PsgdJoint* j, void* workspace, long lon
     default: rc = joint_backward_f16(*j, p, part, stream);
   }
   if (rc) return rc;
-  const dim3 grid((j->d + 31) / 32, p.slots - (p.slot[4] >= 0) + (p.chunks ? (int)j->gates : 0));
-  joint_reduce_kernel<<<grid, dim3(32, 32), 0, stream>>>(*j, p, part);
-  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+  // (a gate group of several chunks has over 32 rows to a chunk on 148 SMs: their number stays within the grid's limit)
+  const dim3 grid((j->d + 31) / 32, p.slots - (p.slot[4] >= 0) + (p.chunks > 1 ? (int)j->gates : 0));
+  return pdl_launch(joint_reduce_kernel, grid, dim3(32, 32), 0, stream, *j, p, (const float*)part);
 }

@@ -987,20 +987,6 @@ bool valid(const PsgdLce& a) {
          a.reduction >= 0 && a.reduction <= 2 && a.piece_bytes >= 0 && a.n <= (1 << 30) && a.v <= (1 << 30);
 }
 
-// A launch that may start while the one before it ends (it waits for it in the kernel: pdl_wait).
-template <typename... P, typename... A>
-int launch(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream_t stream, A&&... args) {
-  cudaLaunchConfig_t c = {};
-  c.gridDim = grid, c.blockDim = block, c.dynamicSmemBytes = smem, c.stream = stream;
-  cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  c.attrs = &at, c.numAttrs = 1;
-  if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess) return PSGD_OK;
-  cudaGetLastError();  // else it would be taken for a later launch's
-  return PSGD_ELAUNCH;
-}
-
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
 int product(const LceArgs& args, cudaStream_t stream) {
   using C = LceCfg<LIMBS, BN>;
@@ -1009,7 +995,7 @@ int product(const LceArgs& args, cudaStream_t stream) {
     cudaGetLastError();
     return PSGD_ELAUNCH;
   }
-  return launch(k, dim3(psgd_num_sms() / 2 * 2), dim3(L_THREADS), C::SMEM, stream, args);
+  return pdl_launch(k, dim3(psgd_num_sms() / 2 * 2), dim3(L_THREADS), C::SMEM, stream, args);
 }
 template <typename OP, typename OUT, int LIMBS, bool LOGITS>
 int product_bn(int bn, const LceArgs& args, cudaStream_t stream) {
@@ -1044,7 +1030,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
                           nullptr, a.v, l.stage_w ? (a.v + 7) / 8 : 0};
   const bool vec = a.d % 8 == 0 && aligned16(a.h) && a.ld_h * sizeof(T) % 16 == 0 && aligned16(sh.dh) &&
                    (!l.stage_w || (aligned16(a.w) && a.ld_w * sizeof(T) % 16 == 0));
-  if (int rc = launch(vec ? lce_stage_kernel<T, true> : lce_stage_kernel<T, false>, dim3(sh.blocks + sw.blocks), dim3(256),
+  if (int rc = pdl_launch(vec ? lce_stage_kernel<T, true> : lce_stage_kernel<T, false>, dim3(sh.blocks + sw.blocks), dim3(256),
                       0, stream, sh, sw, a.d, (const LceState*)state))
     return rc;
 
@@ -1086,7 +1072,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     r.smoothing = a.label_smoothing, r.z = a.z_loss, r.stat = l.stat;
     int cols = a.grads ? (2 * psgd_num_sms() + rows64 - 1) / rows64 : 1;
     if (cols > (a.v + 2047) / 2048) cols = (a.v + 2047) / 2048;
-    if (int rc = launch(lce_rows_kernel<KT, OP>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state)) return rc;
+    if (int rc = pdl_launch(lce_rows_kernel<KT, OP>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state)) return rc;
     if (!a.grads) continue;
 
     const uint16_t* gm = reinterpret_cast<const uint16_t*>(ws + l.g);
@@ -1119,14 +1105,14 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     if (l.splits > 1) {
       const bool four = a.d % 8 == 0 && aligned16(a.dh);
       const long long n = (long long)rows * a.d / (four ? 8 : 1), want = (n + 255) / 256, most = 8LL * psgd_num_sms();
-      if (int rc = launch(four ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
+      if (int rc = pdl_launch(four ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
                           dim3(256), 0, stream, (const float*)ph.part, l.splits, rows, a.d, row0, (const int*)row_of,
                           reinterpret_cast<T*>(a.dh), (const LceState*)state))
         return rc;
     }
   }
   if (!none && !a.grads)
-    return launch(lce_loss_kernel, dim3(1), dim3(1024), 0, stream, (const float*)loss_rows, (const LceState*)state, (int)mean,
+    return pdl_launch(lce_loss_kernel, dim3(1), dim3(1024), 0, stream, (const float*)loss_rows, (const LceState*)state, (int)mean,
                   a.loss);
   return PSGD_OK;
 }

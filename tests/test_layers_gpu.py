@@ -141,6 +141,8 @@ JOINTS = [
     (9, 8192, "fp32", "layer", True, 1, 0.1, "fp32"),
     (5, 8191, "bf16", "layer", True, 5, 0.1, "fp32"),
     (3000, 24, "bf16", "layer", True, 1, 0.0, "fp32"),
+    (12000, 32, "bf16", "layer", True, 300, 0.0, "fp32"),
+    (3000, 40, "fp16", "rms", False, 30, 0.1, "fp32"),
 ]
 
 
