@@ -45,33 +45,61 @@ PSGD_DEVI void report(int* err, int bits) {
 }
 
 // ---- plan ------------------------------------------------------------------------------------------------------------
+struct LcePlan {
+  const long long* target;
+  long long ignore;
+  const float* grad;
+  int *rank, *row_of, *row_target;
+  float* loss;
+  LceState* state;
+  int* err;
+  int n, v, reduction, half;
+  PSGD_DEVI bool counts(long long x, bool& bad) const {
+    const bool yes = x != ignore && x >= 0 && x < v;
+    bad |= x != ignore && !yes;
+    return yes;
+  }
+  PSGD_DEVI bool none() const { return reduction == PSGD_REDUCE_NONE; }
+  // A row's entries; r: its number among the counted rows (or any, if it does not count).
+  PSGD_DEVI void enter(int i, long long x, bool counted, int r) const {
+    if (counted) {
+      row_of[r] = i;
+      row_target[r] = (int)x;
+    } else if (none()) {
+      loss[i] = 0.f;
+    }
+  }
+  PSGD_DEVI void finish(int total, float top) const {
+    state->counted = total;
+    // fp16 gradients: per-row upstream values are taken relative to the largest, so that g stays in range
+    const float unit = half && none() && grad && top > 0.f ? top : 1.f;
+    state->row_unit = unit;
+    float alpha = half ? unit / L_HALF_SCALE : 1.f;
+    if (!none() && grad) alpha *= *grad;
+    if (reduction == PSGD_REDUCE_MEAN) alpha /= (float)max(total, 1);
+    state->alpha = alpha;
+  }
+};
+
 // One block numbers the counted rows in their order. 65536 targets at a time: every warp counts its groups of 32, the
 // counts are scanned, and each row's number is its group's start plus its place in the group.
 constexpr int PLAN_GROUPS = 64;  // groups of 32 targets that a warp has at a time
-__global__ void __launch_bounds__(1024) lce_plan_kernel(const long long* __restrict__ target, int n, int v,
-                                                        long long ignore, int reduction, int half,
-                                                        const float* __restrict__ grad, int* __restrict__ rank,
-                                                        int* __restrict__ row_of, int* __restrict__ row_target,
-                                                        float* __restrict__ loss, LceState* state, int* err) {
+__global__ void __launch_bounds__(1024) lce_plan_kernel(const LcePlan a) {
   __shared__ int count[PLAN_GROUPS * 32];
   __shared__ int warp_total[32];
   __shared__ float tops[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  const bool none = reduction == PSGD_REDUCE_NONE;
   float top = 0.f;
   bool bad = false;
   int total = 0;
   pdl_trigger();
-  pdl_wait();
-  for (int base = 0; base < n; base += 1024 * PLAN_GROUPS) {
-    const int groups = min(PLAN_GROUPS, (n - base + 1023) / 1024);
+  for (int base = 0; base < a.n; base += 1024 * PLAN_GROUPS) {
+    const int groups = min(PLAN_GROUPS, (a.n - base + 1023) / 1024);
 #pragma unroll 8
     for (int g = 0; g < groups; ++g) {
       const int i = base + g * 1024 + t;
-      const long long x = i < n ? target[i] : ignore;
-      const bool counted = x != ignore && x >= 0 && x < v;
-      bad |= x != ignore && !counted;
-      if (none && grad && counted) top = fmaxf(top, fabsf(grad[i]));
+      const bool counted = a.counts(i < a.n ? a.target[i] : a.ignore, bad);
+      if (a.none() && a.grad && counted) top = fmaxf(top, fabsf(a.grad[i]));
       const uint32_t m = __ballot_sync(0xffffffffu, counted);
       if (lane == 0) count[g * 32 + warp] = __popc(m);
     }
@@ -100,35 +128,23 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const long long* __restr
 #pragma unroll 8
     for (int g = 0; g < groups; ++g) {
       const int i = base + g * 1024 + t;
-      const long long x = i < n ? target[i] : ignore;
-      const bool counted = x != ignore && x >= 0 && x < v;
+      const long long x = i < a.n ? a.target[i] : a.ignore;
+      const bool counted = a.counts(x, bad);
       const uint32_t m = __ballot_sync(0xffffffffu, counted);
       const int r = count[g * 32 + warp] + __popc(m & ((1u << lane) - 1u));
-      if (i >= n) continue;
-      rank[i] = counted ? r : -1;
-      if (counted) {
-        row_of[r] = i;
-        row_target[r] = (int)x;
-      } else if (none) {
-        loss[i] = 0.f;
-      }
+      if (i >= a.n) continue;
+      a.rank[i] = counted ? r : -1;
+      a.enter(i, x, counted, r);
     }
     __syncthreads();
   }
-  if (bad) report(err, ERR_BAD_TARGET);
+  if (bad) report(a.err, ERR_BAD_TARGET);
   top = warp_max(top);
   if (lane == 0) tops[warp] = top;
   __syncthreads();
   if (t == 0) {
     for (int w = 1; w < 32; ++w) top = fmaxf(top, tops[w]);
-    state->counted = total;
-    // fp16 gradients: per-row upstream values are taken relative to the largest, so that g stays in range
-    const float unit = half && none && grad && top > 0.f ? top : 1.f;
-    state->row_unit = unit;
-    float alpha = half ? unit / L_HALF_SCALE : 1.f;
-    if (!none && grad) alpha *= *grad;
-    if (reduction == PSGD_REDUCE_MEAN) alpha /= (float)max(total, 1);
-    state->alpha = alpha;
+    a.finish(total, top);
   }
 }
 
@@ -141,34 +157,71 @@ PSGD_DEVI void limbs3(float x, float* l) {
   l[2] = r - l[1];
 }
 
-// Tensor-core operands from matrices: row i of src to row rank[i] (i without ranks), itself or its bf16 limbs `plane`
-// elements apart. Rows whose rank is -1 zero their row of dh instead. Blocks beyond the rows zero the operand's rows from
+// Tensor-core operands from matrices: row i of h to its number among the counted rows, row i of w to row i, itself or its
+// bf16 limbs `plane` elements apart. Rows that do not count zero their row of dh instead. Blocks beyond the rows zero the operand's rows from
 // the count to the next multiple of 64, which a reduction over rows reads.
 template <typename T>
 struct LceStage {
   const T* src;
   long long ld, ld_out, plane;
-  const int* rank;
   uint16_t* out;
   T* dh;
   int n, blocks;  // (8 rows a block)
 };
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, const LceStage<T> w, int d,
-                                                        const LceState* state) {
+// INLINE: there was no plan launch; every block counts the rows before its own (up to PLAN_INLINE of them: the reads are
+// shorter than a launch), and the last one of h finishes the plan.
+constexpr int PLAN_INLINE = 2048;
+template <typename T, bool VEC, bool INLINE>
+__global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, const LceStage<T> w, int d, const LcePlan plan) {
   constexpr int V = VEC ? 8 : 1;
+  __shared__ int before[8];
+  __shared__ float tops[8];
   pdl_trigger();
-  pdl_wait();
+  if (!INLINE) pdl_wait();
   const bool first = (int)blockIdx.x < h.blocks;
   const LceStage<T>& a = first ? h : w;
-  const int lane = threadIdx.x & 31, i = (blockIdx.x - (first ? 0 : h.blocks)) * 8 + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i0 = (blockIdx.x - (first ? 0 : h.blocks)) * 8, i = i0 + warp;
   long long r = i;
+  int counted = INLINE ? 0 : plan.state->counted;
+  if (INLINE && first) {
+    const bool last = (int)blockIdx.x == h.blocks - 1;  // (beyond every row: it counts them all)
+    const int upto = min(i0, plan.n);
+    int mine = 0;
+    float top = 0.f;
+    bool bad = false;
+#pragma unroll 4
+    for (int k = threadIdx.x; k < upto; k += 256) {
+      const bool yes = plan.counts(plan.target[k], bad);
+      mine += yes;
+      if (last && yes && plan.none() && plan.grad) top = fmaxf(top, fabsf(plan.grad[k]));
+    }
+    mine = __reduce_add_sync(0xffffffffu, mine);
+    top = warp_max(top);
+    if (lane == 0) before[warp] = mine, tops[warp] = top;
+    __syncthreads();
+    counted = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) counted += before[k], top = fmaxf(top, tops[k]);
+    if (last && threadIdx.x == 0) plan.finish(counted, top);
+    if (last && bad) report(plan.err, ERR_BAD_TARGET);
+    if (i0 < plan.n) {  // this block's rows; a warp a row, each with the targets of all eight
+      const long long x = lane < 8 && i0 + lane < plan.n ? plan.target[i0 + lane] : plan.ignore;
+      const uint32_t m = __ballot_sync(0xffffffffu, plan.counts(x, bad));
+      r = (m >> warp) & 1u ? counted + __popc(m & ((1u << warp) - 1u)) : -1;
+      if (lane == warp && i < plan.n) plan.enter(i, x, r >= 0, (int)r);
+    }
+  }
   if (i >= a.n) {
-    if (!a.rank || i >= a.n + 64) return;
-    r = state->counted + (i - a.n);
-    if (r >= ((state->counted + 63) & ~63)) return;
-  } else if (a.rank) {
-    r = a.rank[i];
+    if (!first || i >= a.n + 64) return;
+    if (INLINE && i0 < a.n) {  // the block with the last rows: the count includes those
+      const long long x = lane < 8 && i0 + lane < plan.n ? plan.target[i0 + lane] : plan.ignore;
+      bool bad = false;
+      counted += __popc(__ballot_sync(0xffffffffu, plan.counts(x, bad)));
+    }
+    r = counted + (i - a.n);
+    if (r >= ((counted + 63) & ~63)) return;
+  } else if (!INLINE && first) {
+    r = plan.rank[i];
   }
   if (r < 0) {
     if (a.dh)
@@ -501,6 +554,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     mbar_init(drain, 1);
     *abort = 0;
     fence_barrier_init();
+  }
+  if (warp == 0 && lane < 2 * args.nproblems * LIMBS) {  // (the maps are arguments: no launch before writes them)
+    const LceProblem& p = args.p[lane / (2 * LIMBS)];
+    const int m = lane % (2 * LIMBS);
+    prefetch_tmap(m < LIMBS ? &p.ta[m] : &p.tb[m - LIMBS]);
   }
   pdl_trigger();
   __syncthreads();
@@ -1021,18 +1079,25 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
   const long long ld_w = l.stage_w ? l.ld_w : a.ld_w;
   const bool none = a.reduction == PSGD_REDUCE_NONE, mean = a.reduction == PSGD_REDUCE_MEAN;
 
-  lce_plan_kernel<<<1, 1024, 0, stream>>>(a.target, a.n, a.v, a.ignore_index, a.reduction, half, a.grad, rank, row_of,
-                                          row_target, a.loss, state, err);
-  if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
-  const LceStage<T> sh = {reinterpret_cast<const T*>(a.h), a.ld_h, l.ld_h, l.h_plane, rank, h,
-                          reinterpret_cast<T*>(a.grads ? a.dh : nullptr), a.n, (int)((a.n + 64LL + 7) / 8)};
-  const LceStage<T> sw = {reinterpret_cast<const T*>(a.w), a.ld_w, l.ld_w, l.w_plane, nullptr, const_cast<uint16_t*>(w),
+  const LcePlan plan = {a.target, a.ignore_index, a.grad, rank, row_of, row_target, a.loss, state, err, a.n, a.v, a.reduction, half};
+  const LceStage<T> sh = {reinterpret_cast<const T*>(a.h), a.ld_h, l.ld_h, l.h_plane, h,
+                          reinterpret_cast<T*>(a.grads ? a.dh : nullptr), a.n, (int)((a.n + 7LL) / 8 + 8)};
+  const LceStage<T> sw = {reinterpret_cast<const T*>(a.w), a.ld_w, l.ld_w, l.w_plane, const_cast<uint16_t*>(w),
                           nullptr, a.v, l.stage_w ? (a.v + 7) / 8 : 0};
   const bool vec = a.d % 8 == 0 && aligned16(a.h) && a.ld_h * sizeof(T) % 16 == 0 && aligned16(sh.dh) &&
                    (!l.stage_w || (aligned16(a.w) && a.ld_w * sizeof(T) % 16 == 0));
-  if (int rc = pdl_launch(vec ? lce_stage_kernel<T, true> : lce_stage_kernel<T, false>, dim3(sh.blocks + sw.blocks), dim3(256),
-                      0, stream, sh, sw, a.d, (const LceState*)state))
-    return rc;
+  const dim3 stage_grid(sh.blocks + sw.blocks);
+  if (a.n <= PLAN_INLINE) {
+    auto k = vec ? lce_stage_kernel<T, true, true> : lce_stage_kernel<T, false, true>;
+    k<<<stage_grid, 256, 0, stream>>>(sh, sw, a.d, plan);
+    if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
+  } else {
+    lce_plan_kernel<<<1, 1024, 0, stream>>>(plan);
+    if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
+    if (int rc = pdl_launch(vec ? lce_stage_kernel<T, true, false> : lce_stage_kernel<T, false, false>, stage_grid, dim3(256),
+                            0, stream, sh, sw, a.d, plan))
+      return rc;
+  }
 
   LceArgs args = {};
   args.state = state;
