@@ -23,7 +23,8 @@ constexpr int L_THREADS = 384;      // a warpgroup for copies and products, two 
 // Registers a thread: 168 at launch (384 threads); 3 * 168 = 56 + 2 * 224.
 constexpr int L_REGS_LOW = 56, L_REGS_HIGH = 224;
 constexpr int L_LIMBS = 3;          // of an fp32 operand
-constexpr int L_GROUP_M = 4;        // row tiles that walk the column tiles together (L2 reuse of both operands)
+constexpr int L_GROUP_M = 4;         // row tiles that walk the column tiles together (L2 reuse of both operands)
+constexpr int L_UNIT = 8;            // what a unit costs besides its K blocks (its last step), in K blocks: about 2.5 us
 // Kept exponentials are fp16 of 2^15 exp(l - m), exp(l - m) in [0, 1]: 11 significant bits down to 2^-29 of the row's
 // maximum in these 256 columns, so that the one rounding to 16 bits that matters is that of g.
 constexpr float L_KEEP_SCALE = 32768.f;
@@ -273,9 +274,10 @@ struct LceProblem {
   const int* row_of;
   void* out;
   long long ld_out;
-  float* part;       // splits > 1: [split][M][N], joined by lce_join_kernel
-  const float* acc;  // earlier pieces' sums, added
+  float* part;       // splits > 1: [split][M][ld_part], joined by lce_join_kernel
+  const float* acc;  // earlier pieces' sums [M][ld_acc], added
   float* acc_out;    // sums so far, fp32, instead of out
+  long long ld_part, ld_acc;
 };
 struct LceShape {
   int M, K, tiles_m, tiles_n, kblocks, units, unit_kblocks;
@@ -323,7 +325,7 @@ struct LceDeal {
     u1 = two ? s1.units : 0;
     rem = u0 % n;
     h = u0 / n + (c < rem);
-    extra = two && rem && s1.unit_kblocks ? s0.unit_kblocks / s1.unit_kblocks : 0;
+    extra = two && rem && s0.unit_kblocks > s1.unit_kblocks ? (s0.unit_kblocks + L_UNIT) / (s1.unit_kblocks + L_UNIT) : 0;
     base = (n - rem) * extra;
   }
   // Unit k of this cluster: (problem, index), or false.
@@ -367,13 +369,13 @@ struct __align__(64) LceArgs {
 };
 
 // Shared memory of a stage: KS blocks of 64 of K, each LIMBS tiles of A (this CTA's 128 rows) and of B (its half of BN).
-template <int LIMBS, int BN>
+template <int LIMBS, int BN, bool LOGITS>
 struct LceCfg {
   static constexpr int KS = LIMBS == 1 ? 2 : 1;
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = LIMBS == 1 || LOGITS ? 3 : 2;
   static constexpr int A = 128 * LK * 2, B = (BN / 2) * LK * 2;
   static constexpr int BLOCK = LIMBS * (A + B), STAGE = KS * BLOCK;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + 512;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + 512 + (LOGITS ? 0 : 8 * 32 * 33 * 4);  // (grad_row's blocks)
   static constexpr int COLS = BN / 2;                  // accumulator columns of an epilogue thread
   static constexpr int ACC = (LIMBS == 1 ? 1 : 2) * BN;  // TMEM columns of an accumulator (fp32: the small products apart)
   static constexpr int TMEM = 2 * ACC < 512 ? 256 : 512;
@@ -465,41 +467,64 @@ PSGD_DEVI void logits_row(const LceProblem& p, const LceShape& sh, const LceLogi
   }
 }
 
-// The gradients' epilogue: this thread's COLS columns of one row.
+// The gradients' epilogue: this thread's COLS columns of one row (all lanes of a warp call it: `live` says whether the row
+// is there). Rows that 32-byte stores do not fit (an odd number of columns) go through `turn`, 32 x 33 floats of the
+// warp, so that a store covers neighbours of one row.
 template <typename T, int COLS>
-PSGD_DEVI void grad_row(const LceProblem& p, const LceShape& sh, int split, long long row, int n0, float* v, float alpha) {
-  if (row >= sh.M) return;
-  const int width = min(COLS, p.N - n0);
-  const long long flat = row * p.N + n0;
-  const float* from = p.acc ? p.acc + flat : nullptr;
-  if (from) {
+PSGD_DEVI void grad_row(const LceProblem& p, const LceShape& sh, int split, long long row, int n0, float* v, float alpha,
+                        float* turn) {
+  const bool live = row < sh.M;
+  const int width = min(COLS, p.N - n0), lane = threadIdx.x & 31;
+  if (p.acc && live) {
+    const float* from = p.acc + row * p.ld_acc + n0;
 #pragma unroll
     for (int k = 0; k < COLS; ++k)
       if (k < width) v[k] += from[k];
   }
-  float* wide = p.part ? p.part + (long long)split * p.M * p.N + flat : p.acc_out ? p.acc_out + flat : nullptr;
-  if (wide) {
-    if (width == COLS && p.N % 8 == 0 && (reinterpret_cast<uintptr_t>(wide) & 31) == 0) {
+  if (p.part) {  // (rows of whole sectors)
+    if (!live) return;
+    float* to = p.part + ((long long)split * p.M + row) * p.ld_part + n0;
 #pragma unroll
-      for (int k = 0; k < COLS; k += 8) store_row32<float>(wide + k, v + k);
-    } else {
+    for (int k = 0; k < COLS; k += 8)
+      if (k < width) store_row32<float>(to + k, v + k);
+    return;
+  }
+  if (p.acc_out) {
+    if (!live) return;
+    float* to = p.acc_out + row * p.ld_acc + n0;
 #pragma unroll
-      for (int k = 0; k < COLS; ++k)
-        if (k < width) wide[k] = v[k];
-    }
+    for (int k = 0; k < COLS; ++k)
+      if (k < width) to[k] = v[k];
     return;
   }
   constexpr int S = 32 / sizeof(T);
-  T* out = reinterpret_cast<T*>(p.out) + (p.row_of ? p.row_of[p.row0 + row] : row) * p.ld_out + n0;
 #pragma unroll
   for (int k = 0; k < COLS; ++k) v[k] *= alpha;
-  if (width == COLS && p.ld_out % S == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0) {
+  const int at = live ? (p.row_of ? p.row_of[p.row0 + row] : (int)row) : -1;
+  T* base = reinterpret_cast<T*>(p.out) + n0;
+  if (p.ld_out % S == 0 && (reinterpret_cast<uintptr_t>(p.out) & 31) == 0) {  // (N is ld_out: whole sectors to its end)
+    T* out = base + at * p.ld_out;
 #pragma unroll
-    for (int k = 0; k < COLS; k += S) store_row32<T>(out + k, v + k);
-  } else {
+    for (int k = 0; k < COLS; k += S)
+      if (live && k < width) store_row32<T>(out + k, v + k);
+    return;
+  }
+  for (int c = 0; c < COLS; c += 32) {
+    if (c >= width) break;
+    __syncwarp();
 #pragma unroll
-    for (int k = 0; k < COLS; ++k)
-      if (k < width) out[k] = from_f32<T>(v[k]);
+    for (int k = 0; k < 32; ++k) {
+      // (v's index has to be known where it is compiled: one of COLS / 32 blocks is taken)
+      float x = v[k];
+#pragma unroll
+      for (int b = 32; b < COLS; b += 32) x = c == b ? v[b + k] : x;
+      turn[lane * 33 + k] = x;
+    }
+    __syncwarp();
+    for (int r = 0; r < 32; ++r) {
+      const int to = __shfl_sync(0xffffffffu, at, r);
+      if (to >= 0 && c + lane < width) base[to * p.ld_out + c + lane] = from_f32<T>(turn[r * 33 + lane]);
+    }
   }
 }
 
@@ -526,7 +551,7 @@ PSGD_DEVI void add_columns(uint32_t at, float* v) {
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     lce_product_kernel(const __grid_constant__ LceArgs args) {
-  using C = LceCfg<LIMBS, BN>;
+  using C = LceCfg<LIMBS, BN, LOGITS>;
   constexpr int S = C::STAGES, COLS = C::COLS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -711,6 +736,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
         *args.loss = args.mean ? sum / (float)max(n, 1) : sum;
       }
     }
+    float* turn = reinterpret_cast<float*>(smem + S * C::STAGE + 512) + (warp - 4) * (32 * 33);
     const uint32_t lead0 = mapa_shared(&tempty[0], 0), lead1 = mapa_shared(&tempty[1], 0);
     const float alpha = args.state->alpha;
     uint32_t i = 0;
@@ -730,10 +756,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
         tc_fence_after();
         return tmem_base + ((uint32_t)(q * 32) << 16) + acc * C::ACC + half * COLS;
       };
+      // (Its columns are in registers: nothing in memory is handed over, and a releasing arrive would wait for this warp's
+      // stores of the tile before.)
       auto give_back = [&]() {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(i & 1 ? lead1 : lead0);
+        if (lane == 0) mbar_arrive_cluster_relaxed(i & 1 ? lead1 : lead0);
         ++i;
       };
       if constexpr (!LOGITS && LIMBS == 1) {  // one sum over all of K: no more than 32 columns in registers
@@ -747,7 +775,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
           if (u.k0 >= u.k1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) f[e] = 0.f;
-          grad_row<OUT, 32>(p, sh, u.split, row, n0 + c, f, alpha);
+          grad_row<OUT, 32>(p, sh, u.split, row, n0 + c, f, alpha, turn);
         }
         give_back();
       } else {
@@ -772,7 +800,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
           for (int e = 0; e < COLS; ++e) f[e] = 0.f;
         if (n0 < p.N) {
           if constexpr (LOGITS) logits_row<OUT, COLS>(p, sh, args.logits, row, n0, f);
-          else grad_row<OUT, COLS>(p, sh, u.split, row, n0, f, alpha);
+          else grad_row<OUT, COLS>(p, sh, u.split, row, n0, f, alpha, turn);
         }
       }
     }
@@ -825,20 +853,25 @@ struct LceRows {
   int stat;  // columns to a statistic
 };
 
-// One block a row (and 1 / gridDim.y of its columns). KT / GT: types of the kept exponentials and of g.
-template <typename KT, typename GT>
+// One block a row (and 1 / gridDim.y of its columns), or (WARP) one warp a row, where a row is short. KT / GT: types of
+// the kept exponentials and of g.
+template <typename KT, typename GT, bool WARP>
 __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const LceState* state) {
   __shared__ float red[8];
   pdl_trigger();
   pdl_wait();
-  const int row = blockIdx.x, there = min(a.rows, max(0, state->counted - a.row0));
+  constexpr int STEP = WARP ? 32 : 256;
+  const int t = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const int row = WARP ? blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x, there = min(a.rows, max(0, state->counted - a.row0));
+  auto sum_all = [&](float v) { return WARP ? warp_sum(v) : block_sum(v, red); };
+  auto max_all = [&](float v) { return WARP ? warp_max(v) : block_max(v, red); };
   KT* kept = reinterpret_cast<KT*>(a.kept) + (a.kept ? row * a.ld_kept : 0);
   const int vecs = (a.v + 7) / 8, per = (vecs + gridDim.y - 1) / gridDim.y;
   const int v0 = blockIdx.y * per, v1 = min(vecs, v0 + per);
   if (row >= there) {  // rows up to the next multiple of 64 enter the reduction over rows: zero
     if (!a.kept || row >= ((there + 63) & ~63)) return;
     const float zero[8] = {};
-    for (int i = v0 + threadIdx.x; i < v1; i += 256) {
+    for (int i = v0 + t; i < v1; i += STEP) {
       if constexpr (sizeof(KT) == 4) {
         for (int q = 0; q < 3; ++q)
           store_vec<__nv_bfloat16, 8>(reinterpret_cast<__nv_bfloat16*>(a.limbs) + q * a.plane + row * a.ld_kept + i * 8, zero);
@@ -850,19 +883,19 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   }
   const float2* st = a.stats + (long long)row * a.tiles;
   float top = -INFINITY;
-  for (int i = threadIdx.x; i < a.tiles; i += 256) top = fmaxf(top, st[i].x);
-  top = block_max(top, red);
+  for (int i = t; i < a.tiles; i += STEP) top = fmaxf(top, st[i].x);
+  top = max_all(top);
   const float ref = top == -INFINITY ? 0.f : top;
   float sum = 0.f, linear = 0.f;
-  for (int i = threadIdx.x; i < a.tiles; i += 256) {
+  for (int i = t; i < a.tiles; i += STEP) {
     sum += st[i].y * expf(st[i].x - ref);
     if (a.linear) linear += a.linear[(long long)row * a.tiles + i];
   }
-  sum = block_sum(sum, red);
-  if (a.linear) linear = block_sum(linear, red);
+  sum = sum_all(sum);
+  if (a.linear) linear = sum_all(linear);
   const float lse = ref + logf(sum), lt = a.target_logit[row];
   const int target = a.row_target[a.row0 + row];
-  if (threadIdx.x == 0 && blockIdx.y == 0) {
+  if (t == 0 && blockIdx.y == 0) {
     float loss = a.smoothing == 0.f ? lse - lt : (1.f - a.smoothing) * (lse - lt) + a.smoothing * (lse - linear / (float)a.v);
     if (a.z != 0.f) loss += a.z * lse * lse;
     if (a.none) a.loss[a.row_of[a.row0 + row]] = loss;
@@ -876,7 +909,7 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   const float scale = sizeof(KT) == 4 ? 1.f : 1.f / L_KEEP_SCALE;
   // the target's element from its fp32 logit: p - 1 without cancellation
   const float at_target = c * (expm1f(lt - lse) + (pull - 1.f) * expf(lt - lse) + a.smoothing - uniform);
-  for (int i = v0 + threadIdx.x; i < v1; i += 256) {
+  for (int i = v0 + t; i < v1; i += STEP) {
     const float f = expf(st[(i * 8) >> shift].x - lse) * scale * pull;
     float g[8];
     load_vec<KT, 8>(kept + i * 8, g);
@@ -914,28 +947,29 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float* __restrict_
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
-// Joins the splits of dh: out[row_of[r]] = alpha * sum over splits, in their order. V: values at a time (N a multiple).
+// Joins the splits of a gradient: out[row] = alpha * sum over splits, in their order. Rows are the counted ones through
+// row_of, or all M of them as they are. V: values at a time (N a multiple, or 1).
 template <typename T, int V>
-__global__ void __launch_bounds__(256) lce_join_kernel(const float* __restrict__ part, int splits, int M, int N, int row0,
-                                                       const int* __restrict__ row_of, T* __restrict__ out,
-                                                       const LceState* state) {
+__global__ void __launch_bounds__(256) lce_join_kernel(const float* __restrict__ part, int splits, int M, int N,
+                                                       long long ld_part, int row0, const int* __restrict__ row_of,
+                                                       T* __restrict__ out, const LceState* state) {
   pdl_wait();
-  const int there = min(M, max(0, state->counted - row0)), per_row = N / V;
-  const long long n = (long long)there * per_row, plane = (long long)M * N;
+  const int there = row_of ? min(M, max(0, state->counted - row0)) : M, per_row = N / V;
+  const long long n = (long long)there * per_row, plane = M * ld_part;
   const float alpha = state->alpha;
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * V;
     float s[V] = {};
 #pragma unroll 4
     for (int k = 0; k < splits; ++k) {
       float x[V];
-      load_vec<float, V>(part + k * plane + i * V, x);
+      load_vec<float, V>(part + k * plane + r * ld_part + c, x);
 #pragma unroll
       for (int e = 0; e < V; ++e) s[e] += x[e];
     }
 #pragma unroll
     for (int e = 0; e < V; ++e) s[e] *= alpha;
-    const int r = (int)(i / per_row);
-    store_vec<T, V>(out + (long long)row_of[row0 + r] * N + (i - (long long)r * per_row) * V, s);
+    store_vec<T, V>(out + (long long)(row_of ? row_of[row0 + r] : r) * N + c, s);
   }
 }
 
@@ -970,10 +1004,10 @@ int encode(CUtensorMap* m, const void* p, bool half, long long rows, long long c
 
 // Where everything lies in the workspace; the same from a size query and from the call.
 struct Layout {
-  int limbs, tiles, piece, pieces, splits, bn, bn_grads, stat;
+  int limbs, tiles, piece, pieces, splits, splits_w, bn, bn_grads, stat;
   bool stage_w;
-  long long ld_h, ld_w, ld_kept, h_plane, w_plane, g_plane;
-  size_t state, rank, row_of, row_target, loss_rows, target_logit, stats, linear, h, w, kept, g, part, acc, bytes;
+  long long ld_h, ld_w, ld_kept, ld_part, h_plane, w_plane, g_plane;
+  size_t state, rank, row_of, row_target, loss_rows, target_logit, stats, linear, h, w, kept, g, part, part_w, acc, bytes;
 };
 
 Layout layout(const PsgdLce& a) {
@@ -986,7 +1020,9 @@ Layout layout(const PsgdLce& a) {
   const long long wide_tiles = (((long long)a.n + LM - 1) / LM) * ((a.v + 255) / 256);
   l.bn = wide || wide_tiles < 2 * clusters ? 128 : 256;
   const long long wide_grads = (((long long)a.n + LM - 1) / LM + (a.v + LM - 1) / LM) * ((a.d + 255) / 256);
-  l.bn_grads = wide || wide_grads < 2 * clusters ? 128 : 256;
+  // (and for widths that fill their last wide tile to less than half: 4 / 3 of the products of narrow ones, or twice)
+  l.bn_grads = wide || wide_grads < 2 * clusters || (a.d <= 384 && (a.d + 127) / 128 % 2) ? 128 : 256;
+  l.ld_part = up(a.d, 8);
   l.stat = l.bn / 2;
   l.tiles = (a.v + l.stat - 1) / l.stat;
   l.ld_h = up(a.d, 8);
@@ -1000,17 +1036,20 @@ Layout layout(const PsgdLce& a) {
   if (piece > up(a.n, LM)) piece = up(a.n, LM);
   l.piece = (int)piece;
   l.pieces = (int)((a.n + piece - 1) / piece);
-  // dh has few tiles and a long reduction over the vocabulary. It and dw need the same number of products, so a unit
-  // of at most a quarter of a cluster's share of both keeps the shares even.
-  const long long tiles_h = ((piece + LM - 1) / LM) * ((a.d + l.bn_grads - 1) / l.bn_grads);
-  const long long tiles_w = (((long long)a.v + LM - 1) / LM) * ((a.d + l.bn_grads - 1) / l.bn_grads);
+  // dh reduces over the vocabulary, dw over the tokens, and either may have few tiles. They need the same number of
+  // products: splits until a unit is at most a quarter of a cluster's share of both keep the shares even.
+  const long long tiles_n = (a.d + l.bn_grads - 1) / l.bn_grads;
+  const long long tiles_h = ((piece + LM - 1) / LM) * tiles_n, tiles_w = (((long long)a.v + LM - 1) / LM) * tiles_n;
   const long long kb_h = (a.v + LK - 1) / LK, kb_w = (piece + LK - 1) / LK;
-  const long long quarter = (tiles_h * kb_h + tiles_w * kb_w) / (4 * clusters) + 1;
-  long long splits = (kb_h + quarter - 1) / quarter;
-  if (splits > (kb_h + 7) / 8) splits = (kb_h + 7) / 8;
-  if (splits > 16) splits = 16;
-  if (tiles_h >= 4 * clusters) splits = 1;  // (the units are even enough, and partial sums are not free)
-  l.splits = splits < 1 ? 1 : (int)splits;
+  const long long quarter = (tiles_h * (kb_h + L_UNIT) + tiles_w * (kb_w + L_UNIT)) / (4 * clusters) + 1;
+  auto split = [&](long long tiles, long long kb) -> int {
+    long long n = (kb + quarter - 1) / quarter;
+    if (n > (kb + 7) / 8) n = (kb + 7) / 8;
+    if (n > 16) n = 16;
+    return tiles >= 4 * clusters ? 1 : (int)n;  // (many units are even enough, and partial sums are not free)
+  };
+  l.splits = split(tiles_h, kb_h);
+  l.splits_w = l.pieces > 1 ? 1 : split(tiles_w, kb_w);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t p = at;
@@ -1033,8 +1072,9 @@ Layout layout(const PsgdLce& a) {
   if (a.grads) {
     l.kept = take((wide ? 4ull : 2ull) * l.g_plane);
     l.g = wide ? take(2ull * l.limbs * l.g_plane) : l.kept;
-    l.part = take(l.splits > 1 ? 4ull * l.splits * piece * a.d : 0);
-    l.acc = take(l.pieces > 1 && !wide ? 4ull * a.v * a.d : 0);
+    l.part = take(l.splits > 1 ? 4ull * l.splits * piece * l.ld_part : 0);
+    l.part_w = take(l.splits_w > 1 ? 4ull * l.splits_w * a.v * l.ld_part : 0);
+    l.acc = take(l.pieces > 1 && !wide ? 4ull * a.v * l.ld_part : 0);
   }
   l.bytes = at;
   return l;
@@ -1047,7 +1087,7 @@ bool valid(const PsgdLce& a) {
 
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
 int product(const LceArgs& args, cudaStream_t stream) {
-  using C = LceCfg<LIMBS, BN>;
+  using C = LceCfg<LIMBS, BN, LOGITS>;
   auto k = lce_product_kernel<OP, OUT, LIMBS, BN, LOGITS>;
   if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
     cudaGetLastError();
@@ -1137,7 +1177,10 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     r.smoothing = a.label_smoothing, r.z = a.z_loss, r.stat = l.stat;
     int cols = a.grads ? (2 * psgd_num_sms() + rows64 - 1) / rows64 : 1;
     if (cols > (a.v + 2047) / 2048) cols = (a.v + 2047) / 2048;
-    if (int rc = pdl_launch(lce_rows_kernel<KT, OP>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state)) return rc;
+    const bool by_warp = a.v <= 2048 && rows64 >= 2 * psgd_num_sms();  // (one warp's trip over a row is then no longer)
+    if (int rc = by_warp ? pdl_launch(lce_rows_kernel<KT, OP, true>, dim3(rows64 / 8), dim3(256), 0, stream, r, (const LceState*)state)
+                         : pdl_launch(lce_rows_kernel<KT, OP, false>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state))
+      return rc;
     if (!a.grads) continue;
 
     const uint16_t* gm = reinterpret_cast<const uint16_t*>(ws + l.g);
@@ -1150,31 +1193,37 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     ph.b_mn = 1, ph.M = rows, ph.N = a.d, ph.K = a.v, ph.dyn = 1, ph.row0 = row0, ph.splits = l.splits;
     ph.row_of = row_of, ph.out = a.dh, ph.ld_out = a.d;
     ph.part = l.splits > 1 ? reinterpret_cast<float*>(ws + l.part) : nullptr;
+    ph.ld_part = l.ld_part;
     LceProblem& pw = args.p[1];  // dw = g^T h: both with rows of K = tokens
     pw = LceProblem{};
     for (int i = 0; i < l.limbs; ++i) {
       if (int rc = encode(&pw.ta[i], gm + i * l.g_plane, half, rows64, a.v, l.ld_kept, 64)) return rc;
       if (int rc = encode(&pw.tb[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows64, a.d, l.ld_h, 64)) return rc;
     }
-    pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = 1;
-    pw.out = a.dw, pw.ld_out = a.d;
+    pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = l.splits_w;
+    pw.part = l.splits_w > 1 ? reinterpret_cast<float*>(ws + l.part_w) : nullptr;
+    pw.ld_part = l.ld_part, pw.out = a.dw, pw.ld_out = a.d;
     if (l.pieces > 1) {
       float* acc = sizeof(T) == 4 ? reinterpret_cast<float*>(a.dw) : reinterpret_cast<float*>(ws + l.acc);
       pw.acc = piece > 0 ? acc : nullptr;
       pw.acc_out = piece + 1 < l.pieces ? acc : nullptr;
+      pw.ld_acc = sizeof(T) == 4 ? a.d : l.ld_part;
     }
     args.nproblems = 2;
     args.chunk = LIMBS == 1 ? 1 << 20 : 8;  // (a 16-bit gradient's own rounding is a hundred times the truncation)
     if (!none && piece + 1 == l.pieces) args.loss_rows = loss_rows, args.loss = a.loss, args.mean = mean;
     if (int rc = product_bn<OP, T, LIMBS, false>(l.bn_grads, args, stream)) return rc;
-    if (l.splits > 1) {
-      const bool four = a.d % 8 == 0 && aligned16(a.dh);
-      const long long n = (long long)rows * a.d / (four ? 8 : 1), want = (n + 255) / 256, most = 8LL * psgd_num_sms();
-      if (int rc = pdl_launch(four ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
-                          dim3(256), 0, stream, (const float*)ph.part, l.splits, rows, a.d, row0, (const int*)row_of,
-                          reinterpret_cast<T*>(a.dh), (const LceState*)state))
-        return rc;
-    }
+    auto join = [&](const LceProblem& p, void* out) {
+      const bool eight = a.d % 8 == 0 && aligned16(out);
+      const long long n = (long long)p.M * a.d / (eight ? 8 : 1), want = (n + 255) / 256, most = 8LL * psgd_num_sms();
+      return pdl_launch(eight ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
+                        dim3(256), 0, stream, (const float*)p.part, p.splits, p.M, a.d, p.ld_part, row0, p.row_of,
+                        reinterpret_cast<T*>(out), (const LceState*)state);
+    };
+    if (l.splits > 1)
+      if (int rc = join(ph, a.dh)) return rc;
+    if (l.splits_w > 1)
+      if (int rc = join(pw, a.dw)) return rc;
   }
   if (!none && !a.grads)
     return pdl_launch(lce_loss_kernel, dim3(1), dim3(1024), 0, stream, (const float*)loss_rows, (const LceState*)state, (int)mean,

@@ -328,6 +328,13 @@ LOSSES = [
     (300, 515, 2003, "bf16", 0.1, 0.1, 0.0),
     (513, 264, 5003, "bf16", 0.0, 0.0, 0.0),
     (1025, 520, 4100, "bf16", 0.2, 0.0, 1e-4),
+    # few classes and many tokens (dw is split over the tokens), rows that 32-byte stores do not fit, few tokens
+    (4100, 136, 10, "bf16", 0.3, 0.0, 0.0),
+    (3000, 100, 33, "fp16", 0.9, 0.1, 0.0),
+    (2500, 67, 5, "fp32", 0.2, 0.0, 0.0),
+    (700, 301, 3001, "bf16", 0.0, 0.0, 0.0),
+    (700, 301, 1501, "fp32", 0.0, 0.0, 0.0),
+    (3, 1000, 9001, "fp16", 0.0, 0.0, 0.0),
 ]
 
 
