@@ -7,8 +7,30 @@ namespace {
 
 constexpr int DROP_THREADS = 256, DROP_UNROLL = 2, DROP_BLOCKS = 4;  // (blocks of an SM)
 
+// Eight elements: 16 bytes, or 32 at once (two 16-byte loads would take half a sector each, twice).
+template <int H>
+PSGD_DEVI void load_pieces(const void* p, uint4* v) {
+  if constexpr (H == 1) {
+    v[0] = *reinterpret_cast<const uint4*>(p);
+  } else {
+    asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(v[0].x), "=r"(v[0].y), "=r"(v[0].z), "=r"(v[0].w), "=r"(v[1].x), "=r"(v[1].y), "=r"(v[1].z), "=r"(v[1].w)
+                 : "l"(p));
+  }
+}
+template <typename T>
+PSGD_DEVI void store_pieces(T* p, const float* f) {
+  if constexpr (sizeof(T) == 2) {
+    store_vec<T, 8>(p, f);
+  } else {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(f[0]), "f"(f[1]), "f"(f[2]),
+                 "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7])
+                 : "memory");
+  }
+}
+
 // A generator block (8 elements) at a time, DROP_UNROLL of them DROP_THREADS apart so that their loads are under way
-// together. VEC: every pointer is 16-byte aligned and whole blocks move as vectors; the last, partial block (and all
+// together. VEC: every pointer is aligned to a block's bytes and whole blocks move as vectors; the last, partial block (and all
 // without VEC) goes element by element.
 template <typename T, bool VEC, bool RESIDUAL>
 __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS)
@@ -23,12 +45,10 @@ __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS)
 #pragma unroll
     for (int u = 0; u < DROP_UNROLL; ++u) {
       const long long b = b0 + u * DROP_THREADS;
-      if (b < whole)
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          v[u][h] = reinterpret_cast<const uint4*>(x)[b * H + h];
-          if (RESIDUAL) r[u][h] = reinterpret_cast<const uint4*>(residual)[b * H + h];
-        }
+      if (b < whole) {
+        load_pieces<H>(x + 8 * b, v[u]);
+        if (RESIDUAL) load_pieces<H>(residual + 8 * b, r[u]);
+      }
     }
 #pragma unroll
     for (int u = 0; u < DROP_UNROLL; ++u) {
@@ -44,7 +64,7 @@ __global__ void __launch_bounds__(DROP_THREADS, DROP_BLOCKS)
         f[i] = (i & 1 ? keep.high(w) : keep.low(w)) ? f[i] * scale : 0.f;
         if (RESIDUAL) f[i] += add[i];
       }
-      store_vec<T, 8>(out + 8 * b, f);
+      store_pieces<T>(out + 8 * b, f);
     }
   }
   const long long blocks = (n + 7) / 8;
@@ -74,7 +94,8 @@ int start(const PsgdDropout& d, cudaStream_t stream) {
 
 template <typename T>
 int launch(const PsgdDropout& d, cudaStream_t stream) {
-  const bool vec = aligned16(d.x) && aligned16(d.out) && aligned16(d.residual);
+  auto aligned = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & (8 * sizeof(T) - 1)) == 0; };
+  const bool vec = aligned(d.x) && aligned(d.out) && aligned(d.residual);
   if (d.residual) return vec ? start<T, true, true>(d, stream) : start<T, false, true>(d, stream);
   return vec ? start<T, true, false>(d, stream) : start<T, false, false>(d, stream);
 }

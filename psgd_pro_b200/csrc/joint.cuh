@@ -89,7 +89,7 @@ PSGD_DEVI float sum2(F2 a) {
   return f.x + f.y;
 }
 
-// Eight elements as four pairs.
+// Eight 16-bit elements as four pairs.
 template <typename T>
 PSGD_DEVI void unpack8(uint4 a, F2* v) {
   const uint32_t w[4] = {a.x, a.y, a.z, a.w};
@@ -99,44 +99,47 @@ PSGD_DEVI void unpack8(uint4 a, F2* v) {
     v[i] = f2(f.x, f.y);
   }
 }
-template <typename T>
-PSGD_DEVI void load8(const T* p, F2* v) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-    v[0] = f2(a.x, a.y), v[1] = f2(a.z, a.w), v[2] = f2(b.x, b.y), v[3] = f2(b.z, b.w);
-  } else {
-    unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
-  }
-}
-template <typename T>
-PSGD_DEVI void store8(T* p, const F2* v) {
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 a = un2(v[i]);
-    f[2 * i] = a.x, f[2 * i + 1] = a.y;
-  }
-  store_vec<T, 8>(p, f);
-}
 
-// The elements of a row that are this thread's: vector i is at e(i) (VEC), or its elements at e(i), e(i) + tpr, ...
-template <bool VEC>
+// The elements of a row that are this thread's, eight to a vector. VEC: a vector is H pieces of 16 bytes (T of 16 bits: one
+// of 8 elements; fp32: two of 4), a piece at e(i, h), neighbouring threads' pieces side by side. Otherwise the elements are
+// tpr apart.
+template <typename T, bool VEC>
 struct Place {
+  static constexpr int H = VEC ? (int)sizeof(T) / 2 : 1, E = 8 / H;  // pieces to a vector, elements to a piece
   int d, tpr, t;
   PSGD_DEVI Place(int d_) : d(d_), tpr(blockDim.x), t(threadIdx.x) {}
-  PSGD_DEVI int e(int i) const { return VEC ? (i * tpr + t) * 8 : i * 8 * tpr + t; }
-  PSGD_DEVI bool any(int i) const { return e(i) < d; }
-  PSGD_DEVI int at(int i, int k) const { return VEC ? e(i) + k : e(i) + k * tpr; }
-  PSGD_DEVI bool has(int i, int k) const { return VEC ? any(i) : at(i, k) < d; }
-  template <typename T>
-  PSGD_DEVI void load(const T* row, int i, F2* v) const {
+  PSGD_DEVI int e(int i, int h) const { return VEC ? ((i * H + h) * tpr + t) * E : i * 8 * tpr + t; }
+  PSGD_DEVI bool piece(int i, int h) const { return e(i, h) < d; }
+  PSGD_DEVI bool any(int i) const { return piece(i, 0); }
+  PSGD_DEVI int at(int i, int k) const { return VEC ? e(i, k / E) + k % E : e(i, 0) + k * tpr; }
+  PSGD_DEVI bool has(int i, int k) const { return VEC ? piece(i, k / E) : at(i, k) < d; }
+  PSGD_DEVI F2 only(F2 v, int i, int k) const {  // elements 2 k, 2 k + 1 of vector i, zero where there are none
     if constexpr (VEC) {
-      if (any(i)) {
-        load8<T>(row + e(i), v);
-        return;
-      }
+      return has(i, 2 * k) ? v : f2(0.f);
+    } else {
+      const float2 f = un2(v);
+      return f2(has(i, 2 * k) ? f.x : 0.f, has(i, 2 * k + 1) ? f.y : 0.f);
+    }
+  }
+  template <typename S>  // S: T, or fp32 (a parameter, a sum) in T's places
+  PSGD_DEVI void load(const S* row, int i, F2* v) const {
+    if constexpr (VEC) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
+      for (int h = 0; h < H; ++h) {
+        F2* to = v + h * (E / 2);
+        if (!piece(i, h)) {
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) to[k] = f2(0.f);
+        } else if constexpr (sizeof(S) == 4) {
+#pragma unroll
+          for (int q = 0; q < E / 4; ++q) {
+            const float4 a = reinterpret_cast<const float4*>(row + e(i, h))[q];
+            to[2 * q] = f2(a.x, a.y), to[2 * q + 1] = f2(a.z, a.w);
+          }
+        } else {
+          unpack8<S>(*reinterpret_cast<const uint4*>(row + e(i, h)), to);
+        }
+      }
     } else {
       float f[8];
 #pragma unroll
@@ -145,21 +148,36 @@ struct Place {
       for (int k = 0; k < 4; ++k) v[k] = f2(f[2 * k], f[2 * k + 1]);
     }
   }
-  template <typename T>
-  PSGD_DEVI void store(T* row, int i, const F2* v) const {
+  template <typename S>
+  PSGD_DEVI void store(S* row, int i, const F2* v) const {
     if constexpr (VEC) {
-      if (any(i)) store8<T>(row + e(i), v);
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        if (piece(i, h)) {
+          float f[E];
+#pragma unroll
+          for (int k = 0; k < E / 2; ++k) {
+            const float2 a = un2(v[h * (E / 2) + k]);
+            f[2 * k] = a.x, f[2 * k + 1] = a.y;
+          }
+          if constexpr (sizeof(S) == 4) {
+#pragma unroll
+            for (int q = 0; q < E / 4; ++q)
+              reinterpret_cast<float4*>(row + e(i, h))[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
+          } else {
+            store_vec<S, 8>(row + e(i, h), f);
+          }
+        }
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 f = un2(v[k]);
-        if (has(i, 2 * k)) row[at(i, 2 * k)] = from_f32<T>(f.x);
-        if (has(i, 2 * k + 1)) row[at(i, 2 * k + 1)] = from_f32<T>(f.y);
+        if (has(i, 2 * k)) row[at(i, 2 * k)] = from_f32<S>(f.x);
+        if (has(i, 2 * k + 1)) row[at(i, 2 * k + 1)] = from_f32<S>(f.y);
       }
     }
   }
   // A parameter vector of fp32 or of T, `otherwise` where there is none.
-  template <typename T>
   PSGD_DEVI void param(const void* p, int dtype, float otherwise, int i, F2* v) const {
     if (!p) {
 #pragma unroll
@@ -173,13 +191,18 @@ struct Place {
   // v with what dropout does not keep set to zero.
   PSGD_DEVI void drop(const Keep& keep, long long row, int i, F2* v) const {
     const unsigned long long at0 = (unsigned long long)row * d;
-    if constexpr (VEC) {
-      const uint4 words = keep.block((at0 + e(i)) >> 3);
+    if constexpr (VEC) {  // (d is a multiple of 8: a piece lies in one block of the generator)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t w = word_of(words, k);
-        const float2 f = un2(v[k]);
-        v[k] = f2(keep.low(w) ? f.x : 0.f, keep.high(w) ? f.y : 0.f);
+      for (int h = 0; h < H; ++h) {
+        const unsigned long long first = at0 + e(i, h);
+        const uint4 words = keep.block(first >> 3);
+        const bool upper = H == 2 && (first & 4);
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) {
+          const uint32_t w = upper ? word_of(words, k + 2) : word_of(words, k);
+          const float2 f = un2(v[h * (E / 2) + k]);
+          v[h * (E / 2) + k] = f2(keep.low(w) ? f.x : 0.f, keep.high(w) ? f.y : 0.f);
+        }
       }
     } else {
       uint32_t m = 0;
@@ -248,19 +271,18 @@ struct Ring16 {
     all = stage * s;
     base = smem_u32(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
   }
-  PSGD_DEVI void fetch(const Place<true>& at, const T* const* rows, bool there) {
+  PSGD_DEVI void fetch(const Place<T, true>& at, const T* const* rows, bool there) {
     if (there)
 #pragma unroll
       for (int a = 0; a < ARR; ++a)
         if (rows[a])
 #pragma unroll
           for (int i = 0; i < NV; ++i)
-            if (at.any(i))
 #pragma unroll
-              for (int h = 0; h < H; ++h)
+            for (int h = 0; h < H; ++h)
+              if (at.piece(i, h))
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                             ::"r"(base + put + apart * ((a * NV + i) * H + h)),
-                             "l"(reinterpret_cast<const uint4*>(rows[a] + at.e(i)) + h)
+                             ::"r"(base + put + apart * ((a * NV + i) * H + h)), "l"(rows[a] + at.e(i, h))
                              : "memory");
     asm volatile("cp.async.commit_group;" ::: "memory");
     put += stage;
@@ -271,25 +293,21 @@ struct Ring16 {
     else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
-  PSGD_DEVI void read(const Place<true>& at, int a, int i, F2* v) const {
-    if (at.any(i)) {
+  PSGD_DEVI void read(const Place<T, true>& at, int a, int i, F2* v) const {
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        uint4 x;
+    for (int h = 0; h < H; ++h) {
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (at.piece(i, h))
         asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
                      : "r"(base + get + apart * ((a * NV + i) * H + h))
                      : "memory");
-        if constexpr (H == 2) {
-          v[2 * h] = f2(__uint_as_float(x.x), __uint_as_float(x.y));
-          v[2 * h + 1] = f2(__uint_as_float(x.z), __uint_as_float(x.w));
-        } else {
-          unpack8<T>(x, v);
-        }
+      if constexpr (H == 2) {
+        v[2 * h] = f2(__uint_as_float(x.x), __uint_as_float(x.y));
+        v[2 * h + 1] = f2(__uint_as_float(x.z), __uint_as_float(x.w));
+      } else {
+        unpack8<T>(x, v);
       }
-    } else {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
     }
   }
   PSGD_DEVI void next() {
@@ -315,7 +333,7 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
   using Sum = GroupSum<1, width_threads(W) / 32>;
   __shared__ __align__(16) float red[Sum::FLOATS];
   const int d = j.d;
-  const Place<VEC> at(d);
+  const Place<T, VEC> at(d);
   Sum sum(red);
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d;
@@ -339,10 +357,10 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const F2 c = f2(j.scale * (drop ? j.keep_scale : 1.f));
-    at.template param<T>(j.weight, j.param_dtype, 1.f, i, w + i * 4);
-    if (layer) at.template param<T>(j.bias, j.param_dtype, 0.f, i, b + i * 4);
-    at.template param<T>(post ? j.post_weight : nullptr, j.param_dtype, 1.f, i, f + i * 4);
-    if (post && layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, fb + i * 4);
+    at.param(j.weight, j.param_dtype, 1.f, i, w + i * 4);
+    if (layer) at.param(j.bias, j.param_dtype, 0.f, i, b + i * 4);
+    at.param(post ? j.post_weight : nullptr, j.param_dtype, 1.f, i, f + i * 4);
+    if (post && layer) at.param(j.post_bias, j.param_dtype, 0.f, i, fb + i * 4);
     F2 g[4] = {c, c, c, c};
     if (one_gate) {
       at.load(reinterpret_cast<const T*>(j.gate), i, g);
@@ -372,11 +390,7 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
         if (at.any(i))
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            F2 c = add2(a[i * 4 + k], m);
-            if (!VEC) {
-              const float2 x = un2(c);
-              c = f2(at.has(i, 2 * k) ? x.x : 0.f, at.has(i, 2 * k + 1) ? x.y : 0.f);
-            }
+            const F2 c = at.only(add2(a[i * 4 + k], m), i, k);
             q = fma2(c, c, q);
           }
     } else {
@@ -530,7 +544,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
   using Sum = GroupSum<NS, width_threads(W) / 32>;
   __shared__ __align__(16) float red[Sum::FLOATS];
   const int d = j.d, dp = (d + 7) & ~7;
-  const Place<VEC> at(d);
+  const Place<T, VEC> at(d);
   pdl_trigger();
   Sum sum(red);
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
@@ -560,7 +574,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 
   // f, per column, of a gate group
   auto column_factor = [&](int g, int i, F2* f) {
-    if (post) at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, f);
+    if (post) at.param(j.post_weight, j.param_dtype, 1.f, i, f);
     else
 #pragma unroll
       for (int k = 0; k < 4; ++k) f[k] = f2(1.f);
@@ -589,7 +603,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     F2 v[4];
-    at.template param<T>(j.weight, j.param_dtype, 1.f, i, v);
+    at.param(j.weight, j.param_dtype, 1.f, i, v);
     ws.put(i, v);
     if (scaled && !direct) {
       column_factor(gate_row, i, v);
@@ -706,13 +720,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int n = i * 4 + k;
-        F2 m = dx[n];
-        if (!VEC) {  // beyond d, where a layer norm's dx is not zero
-          const float2 v = un2(m);
-          m = f2(at.has(i, 2 * k) ? v.x : 0.f, at.has(i, 2 * k + 1) ? v.y : 0.f);
-        } else if (!at.any(i)) {
-          m = f2(0.f);
-        }
+        const F2 m = at.only(dx[n], i, k);  // (beyond d a layer norm's dx is not zero)
         if (use_y) {
           if (post) y[n] = layer ? fma2(y[n], ry, my) : mul2(y[n], ry);
           A[n] = fma2(m, y[n], A[n]);
@@ -752,8 +760,8 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
           F2 g[4], pw[4], pb[4], v[4];
           at.load(pg, i, g);
           if (post) {
-            at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, pw);
-            if (layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, pb);
+            at.param(j.post_weight, j.param_dtype, 1.f, i, pw);
+            if (layer) at.param(j.post_bias, j.param_dtype, 0.f, i, pb);
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -781,8 +789,8 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
       for (int k = 0; k < 4; ++k) g[k] = f2(1.f);
       if (gate) at.load(pg, i, g);
       if (gate && post) {
-        at.template param<T>(j.post_weight, j.param_dtype, 1.f, i, pw);
-        if (layer) at.template param<T>(j.post_bias, j.param_dtype, 0.f, i, pb);
+        at.param(j.post_weight, j.param_dtype, 1.f, i, pw);
+        if (layer) at.param(j.post_bias, j.param_dtype, 0.f, i, pb);
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
