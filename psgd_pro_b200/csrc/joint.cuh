@@ -833,6 +833,301 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
   if (gate && !direct) write(4, A);
 }
 
+// Rows of over 4096 elements: 512 threads have 128 registers each, which the sums over rows half fill. The row stays in
+// shared memory (without VEC: is read again) and each step of it goes through the thread's elements eight at a time,
+// forming again what the step before had; everything else is as above.
+template <typename T, bool VEC, bool DIRECT>
+__global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJoint j, const JointPlan p, float* part) {
+  constexpr int W = W16_512, F = F_RUNTIME;
+  constexpr int NV = width_nv(W), P = NV * 4;
+  constexpr bool RT = F & F_RUNTIME;
+  const bool post = RT ? j.post != 0 : bool(F & F_POST);
+  const bool gate = RT ? j.gate != nullptr : bool(F & F_GATE);
+  const bool layer = RT ? j.kind == PSGD_NORM_LAYER : bool(F & F_LAYER);
+  const bool drop = RT ? j.threshold != 0 : bool(F & F_DROP);
+  const bool direct = DIRECT;
+  const bool use_y = post || gate;
+  extern __shared__ uint4 smem[];
+  constexpr int NS = RT || (F & F_LAYER) ? 2 : 1;
+  using Sum = GroupSum<NS, width_threads(W) / 32>;
+  __shared__ __align__(16) float red[Sum::FLOATS];
+  const int d = j.d, dp = (d + 7) & ~7;
+  const Place<T, VEC> at(d);
+  pdl_trigger();
+  Sum sum(red);
+  const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
+  const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
+  constexpr int ARRAYS = RT || (F & (F_POST | F_GATE)) ? 4 : 3;  // d_normed, d_out, out and, where it is needed, y
+  Ring16<T, NV, ARRAYS> ring(smem, p.stages);
+
+  JointRows it;
+  it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
+  int gate_row = 0;  // of a block that holds (part of) one gate group
+  if (direct) {
+    const int held = p.per_block / p.per_gate, g0 = blockIdx.x * held;
+    it.g = g0 + threadIdx.y;
+    it.end = min(g0 + held, (int)j.gates);
+    it.row = it.g * p.per_gate;
+  } else if (p.chunks) {
+    gate_row = blockIdx.x / p.chunks;
+    const int r0 = gate_row * p.per_gate + (blockIdx.x - gate_row * p.chunks) * p.per_block;
+    it.row = r0 + threadIdx.y;
+    it.end = min(r0 + p.per_block, (gate_row + 1) * p.per_gate);
+    it.g = 0;
+  } else {
+    it.row = blockIdx.x * p.per_block + threadIdx.y;
+    it.end = (int)min((blockIdx.x + 1LL) * p.per_block, j.rows);
+    it.g = 0;
+  }
+
+  // f, per column, of a gate group
+  auto column_factor = [&](int g, int i, F2* f) {
+    if (post) at.param(j.post_weight, j.param_dtype, 1.f, i, f);
+    else
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = f2(1.f);
+    if (gate) {
+      F2 v[4];
+      at.load(reinterpret_cast<const T*>(j.gate) + (long long)g * d, i, v);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f[k] = mul2(f[k], v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) f[k] = mul2(f[k], f2(c));
+  };
+  const int ld_dn = (int)j.ld_d_normed, ld_do = (int)j.ld_d_out, ld_x = (int)j.ld_x, ld_y = (int)j.ld_y;
+  auto sources = [&](long long row, const T** rows) {
+    rows[0] = j.d_normed ? reinterpret_cast<const T*>(j.d_normed) + row * ld_dn : nullptr;
+    rows[1] = j.d_out ? reinterpret_cast<const T*>(j.d_out) + row * ld_do : nullptr;
+    rows[2] = reinterpret_cast<const T*>(j.x) + row * ld_x;
+    rows[3] = use_y ? reinterpret_cast<const T*>(j.y) + row * ld_y : nullptr;
+  };
+
+  F2 dw[P], db[P], A[P], B[P], dpw[P], dpb[P];
+  const bool scaled = post || gate;  // f is not one number
+  const Columns<P> ws(smem_u32(smem) + p.ring, 0), fs(smem_u32(smem) + p.ring, 1);
+#pragma unroll
+  for (int k = 0; k < P; ++k) dw[k] = db[k] = A[k] = B[k] = dpw[k] = dpb[k] = f2(0.f);
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    F2 v[4];
+    at.param(j.weight, j.param_dtype, 1.f, i, v);
+    ws.put(i, v);
+    if (scaled && !direct) {
+      column_factor(gate_row, i, v);
+      fs.put(i, v);
+    }
+  }
+
+  JointRows ahead = it;
+  if constexpr (VEC) {
+    for (int s = 0; s + 1 < p.stages; ++s) {
+      const T* rows[4];
+      const bool there = ahead.there();
+      sources(ahead.row, rows);
+      ring.fetch(at, rows, there);
+      if (there) ahead.next();
+    }
+  }
+  bool fresh = true;  // the gate group's factor is to be formed
+  for (; it.there(); it.next()) {
+    const int row = it.row;
+    const float4 st = reinterpret_cast<const float4*>(j.stats)[row];
+    const T* now[4];
+    sources(row, now);
+    if constexpr (VEC) {
+      const T* rows[4];
+      const bool there = ahead.there();
+      sources(ahead.row, rows);
+      ring.fetch(at, rows, there);
+      if (there) ahead.next();
+      ring.wait();
+    }
+    auto get = [&](int a, int i, F2* v) {
+      if (!now[a]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
+      } else if constexpr (VEC) {
+        ring.read(at, a, i, v);
+      } else {
+        at.load(now[a], i, v);
+      }
+    };
+    const F2 r = f2(st.w), m0 = f2(layer ? -st.z * st.w : 0.f), ry = f2(st.y), my = f2(layer ? -st.x * st.y : 0.f);
+    auto hats = [&](int i, F2* dh, F2* hat) {  // d_normed and hat of vector i
+      get(0, i, dh);
+      get(2, i, hat);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) hat[k] = fma2(hat[k], r, m0);
+    };
+    F2 s0 = f2(0.f), s1 = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 dh[4], hat[4], w[4];
+      hats(i, dh, hat);
+      ws.get(i, w);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        dw[i * 4 + k] = fma2(dh[k], hat[k], dw[i * 4 + k]);
+        db[i * 4 + k] = add2(db[i * 4 + k], dh[k]);
+        dh[k] = mul2(dh[k], w[k]);
+        s0 = fma2(dh[k], hat[k], s0);
+        s1 = add2(s1, dh[k]);
+      }
+    }
+    float s[2] = {sum2(s0), sum2(s1)};
+    sum(s);
+    const F2 c1 = f2(-s[0] * inv_d), c2 = f2(layer ? -s[1] * inv_d : 0.f);
+    if (direct && fresh) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        F2 v[4];
+        column_factor(it.g, i, v);
+        fs.put(i, v);
+      }
+    }
+    // dx of vector i, and with it what reaches dy before the post norm, and yh (or y)
+    auto back = [&](int i, F2* dx, F2* m, F2* y) {
+      F2 dh[4], hat[4], w[4];
+      hats(i, dh, hat);
+      ws.get(i, w);
+      get(1, i, dx);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        dx[k] = fma2(r, add2(fma2(hat[k], c1, mul2(dh[k], w[k])), c2), dx[k]);
+        m[k] = dx[k];
+      }
+      if (drop && at.any(i)) at.drop(keep, row, i, m);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) m[k] = at.only(m[k], i, k);
+      if (use_y) get(3, i, y);
+      if (post)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[k] = fma2(y[k], ry, my);
+    };
+    auto factor = [&](int i, F2* f) {
+      if (scaled) fs.get(i, f);
+      else
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = f2(c);
+    };
+    s0 = s1 = f2(0.f);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 dx[4], m[4], y[4], f[4];
+      back(i, dx, m, y);
+      factor(i, f);
+      at.store(reinterpret_cast<T*>(j.dx) + (long long)row * d, i, dx);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (use_y) A[i * 4 + k] = fma2(m[k], y[k], A[i * 4 + k]);
+        B[i * 4 + k] = add2(B[i * 4 + k], m[k]);
+        m[k] = mul2(m[k], f[k]);
+        if (post) {
+          s0 = fma2(m[k], y[k], s0);
+          s1 = add2(s1, m[k]);
+        }
+      }
+      if (!post) at.store(reinterpret_cast<T*>(j.dy) + (long long)row * d, i, m);
+    }
+    if (post) {
+      s[0] = sum2(s0), s[1] = sum2(s1);
+      sum(s);
+      const F2 c3 = f2(-s[0] * inv_d), c4 = f2(layer ? -s[1] * inv_d : 0.f);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        F2 dx[4], m[4], y[4], f[4];
+        back(i, dx, m, y);
+        factor(i, f);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m[k] = mul2(ry, add2(fma2(y[k], c3, mul2(m[k], f[k])), c4));
+        at.store(reinterpret_cast<T*>(j.dy) + (long long)row * d, i, m);
+      }
+    }
+    if constexpr (VEC) ring.next();
+    if (direct) {
+      fresh = it.last_of_gate();
+      if (fresh) {  // the gate group ends here, and with it its gradient
+        const T* pg = reinterpret_cast<const T*>(j.gate) + (long long)it.g * d;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (!at.any(i)) continue;
+          F2 g[4], pw[4], pb[4], v[4];
+          at.load(pg, i, g);
+          if (post) {
+            at.param(j.post_weight, j.param_dtype, 1.f, i, pw);
+            if (layer) at.param(j.post_bias, j.param_dtype, 0.f, i, pb);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int n = i * 4 + k;
+            const F2 a = mul2(A[n], f2(c)), b = mul2(B[n], f2(c));
+            v[k] = post ? mul2(a, pw[k]) : a;
+            if (post && layer) v[k] = fma2(b, pb[k], v[k]);
+            if (post) dpw[n] = fma2(a, g[k], dpw[n]);
+            if (post && layer) dpb[n] = fma2(b, g[k], dpb[n]);
+            A[n] = B[n] = f2(0.f);
+          }
+          at.store(reinterpret_cast<T*>(j.dgate) + (long long)it.g * d, i, v);
+        }
+      }
+    }
+  }
+
+  // What this group has of the block's rows of `part`: dweight, dbias, then from A and B.
+  if (!direct) {
+    const T* pg = gate ? reinterpret_cast<const T*>(j.gate) + (long long)gate_row * d : nullptr;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      F2 g[4], pw[4], pb[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) g[k] = f2(1.f);
+      if (gate) at.load(pg, i, g);
+      if (gate && post) {
+        at.param(j.post_weight, j.param_dtype, 1.f, i, pw);
+        if (layer) at.param(j.post_bias, j.param_dtype, 0.f, i, pb);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = i * 4 + k;
+        const F2 a = mul2(A[n], f2(c)), b = mul2(B[n], f2(c));
+        dpw[n] = gate ? mul2(a, g[k]) : a;
+        if (layer) dpb[n] = gate ? mul2(b, g[k]) : b;
+        A[n] = post && gate ? mul2(a, pw[k]) : a;
+        if (post && gate && layer) A[n] = fma2(b, pb[k], A[n]);
+      }
+    }
+  }
+  // The groups' shares are added in their order through shared memory, in two buffers in turn, so that one barrier a vector
+  // is enough (a buffer is written again only after the barrier of the vector between, which follows every read of it).
+  // The ring is done with.
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float* share = reinterpret_cast<float*>(smem);
+  int turn = 0;
+  auto write = [&](int a, const F2* v) {
+    if (p.slot[a] < 0) return;
+    float* mine = share + turn * blockDim.y * dp;
+    turn ^= 1;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) at.store(mine + threadIdx.y * dp, i, v + i * 4);
+    __syncthreads();
+    float* to = part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp;
+    T* whole = a == 4 && p.chunks == 1 ? reinterpret_cast<T*>(j.dgate) + (long long)gate_row * d : nullptr;
+    for (int c = threadIdx.y * blockDim.x + threadIdx.x; c < d; c += blockDim.x * blockDim.y) {
+      float t = mine[c];
+      for (int g = 1; g < (int)blockDim.y; ++g) t += mine[g * dp + c];
+      if (whole) whole[c] = from_f32<T>(t);
+      else to[c] = t;
+    }
+  };
+  write(0, dw);
+  if (layer) write(1, db);
+  if (post) write(2, dpw);
+  if (post && layer) write(3, dpb);
+  if (gate && !direct) write(4, A);
+}
+
 // ---- launches of one element type -------------------------------------------------------------------------------------
 template <typename T, bool VEC, int W, int F>
 int joint_forward_launch(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
@@ -841,12 +1136,16 @@ int joint_forward_launch(const PsgdJoint& j, const JointPlan& p, cudaStream_t st
   k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p);
   return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
 }
-template <typename T, bool VEC, int W, int F>
-int joint_backward_launch(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
-  auto k = joint_backward_kernel<T, VEC, W, F>;
+template <typename K>
+int joint_backward_start(K k, const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
   if (int rc = joint_allow_smem(k, p.smem)) return rc;
   k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p, part);
   return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+}
+
+template <typename T, bool VEC, int W, int F>
+int joint_backward_launch(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
+  return joint_backward_start(joint_backward_kernel<T, VEC, W, F>, j, p, part, stream);
 }
 
 inline int joint_flags(const PsgdJoint& j, const JointPlan& p) {
@@ -855,24 +1154,24 @@ inline int joint_flags(const PsgdJoint& j, const JointPlan& p) {
 }
 
 // The kernel compiled for the flags f (F and up that can occur; the forward kernels take the gate at run time).
-template <typename T, int W, int F = 0>
+template <typename T, bool VEC, int W, int F = 0>
 int joint_forward_pick(int f, const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
   if constexpr (F >= F_DIRECT) {
     return PSGD_EINVAL;
   } else {
     if constexpr (!(F & F_GATE))
-      if (f == F) return joint_forward_launch<T, true, W, F>(j, p, stream);
-    return joint_forward_pick<T, W, F + 1>(f, j, p, stream);
+      if (f == F) return joint_forward_launch<T, VEC, W, F>(j, p, stream);
+    return joint_forward_pick<T, VEC, W, F + 1>(f, j, p, stream);
   }
 }
-template <typename T, int W, int F = 0>
+template <typename T, bool VEC, int W, int F = 0>
 int joint_backward_pick(int f, const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
   if constexpr (F >= F_RUNTIME) {
     return PSGD_EINVAL;
   } else {
     if constexpr (!(F & F_DIRECT) || (F & F_GATE))
-      if (f == F) return joint_backward_launch<T, true, W, F>(j, p, part, stream);
-    return joint_backward_pick<T, W, F + 1>(f, j, p, part, stream);
+      if (f == F) return joint_backward_launch<T, VEC, W, F>(j, p, part, stream);
+    return joint_backward_pick<T, VEC, W, F + 1>(f, j, p, part, stream);
   }
 }
 
@@ -880,11 +1179,10 @@ template <typename T>
 int joint_forward_of(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
   const int f = joint_flags(j, p) & ~(F_GATE | F_DIRECT);
   switch (p.wide) {
-    case W8: return p.vec ? joint_forward_pick<T, W8>(f, j, p, stream) : joint_forward_launch<T, false, W8, F_RUNTIME>(j, p, stream);
-    case W16:
-      return p.vec ? joint_forward_pick<T, W16>(f, j, p, stream) : joint_forward_launch<T, false, W16, F_RUNTIME>(j, p, stream);
+    case W8: return p.vec ? joint_forward_pick<T, true, W8>(f, j, p, stream) : joint_forward_pick<T, false, W8>(f, j, p, stream);
+    case W16: return p.vec ? joint_forward_pick<T, true, W16>(f, j, p, stream) : joint_forward_pick<T, false, W16>(f, j, p, stream);
     case W16_256:
-      return p.vec ? joint_forward_pick<T, W16_256>(f, j, p, stream)
+      return p.vec ? joint_forward_pick<T, true, W16_256>(f, j, p, stream)
                    : joint_forward_launch<T, false, W16_256, F_RUNTIME>(j, p, stream);
     default:
       return p.vec ? joint_forward_launch<T, true, W16_512, F_RUNTIME>(j, p, stream)
@@ -897,17 +1195,20 @@ int joint_backward_of(const PsgdJoint& j, const JointPlan& p, float* part, cudaS
   const int f = joint_flags(j, p);
   switch (p.wide) {
     case W8:
-      return p.vec ? joint_backward_pick<T, W8>(f, j, p, part, stream)
-                   : joint_backward_launch<T, false, W8, F_RUNTIME>(j, p, part, stream);
+      return p.vec ? joint_backward_pick<T, true, W8>(f, j, p, part, stream)
+                   : joint_backward_pick<T, false, W8>(f, j, p, part, stream);
     case W16:
-      return p.vec ? joint_backward_pick<T, W16>(f, j, p, part, stream)
-                   : joint_backward_launch<T, false, W16, F_RUNTIME>(j, p, part, stream);
+      return p.vec ? joint_backward_pick<T, true, W16>(f, j, p, part, stream)
+                   : joint_backward_pick<T, false, W16>(f, j, p, part, stream);
     case W16_256:
-      return p.vec ? joint_backward_pick<T, W16_256>(f, j, p, part, stream)
+      return p.vec ? joint_backward_pick<T, true, W16_256>(f, j, p, part, stream)
                    : joint_backward_launch<T, false, W16_256, F_RUNTIME>(j, p, part, stream);
     default:
-      return p.vec ? joint_backward_launch<T, true, W16_512, F_RUNTIME>(j, p, part, stream)
-                   : joint_backward_launch<T, false, W16_512, F_RUNTIME>(j, p, part, stream);
+      if (f & F_DIRECT)
+        return p.vec ? joint_backward_start(joint_backward_wide_kernel<T, true, true>, j, p, part, stream)
+                     : joint_backward_start(joint_backward_wide_kernel<T, false, true>, j, p, part, stream);
+      return p.vec ? joint_backward_start(joint_backward_wide_kernel<T, true, false>, j, p, part, stream)
+                   : joint_backward_start(joint_backward_wide_kernel<T, false, false>, j, p, part, stream);
   }
 }
 

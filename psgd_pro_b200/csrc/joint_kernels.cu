@@ -111,7 +111,8 @@ JointPlan plan_backward(const PsgdJoint& j) {
   p.per_gate = j.gate ? (int)(j.rows / j.gates) : 1;
   p.chunks = j.gate && p.per_gate > JOINT_DIRECT_ROWS;  // (how many: below)
   shape(j.d, p, 0);
-  const int f = joint_flags(j, p) | (p.vec && p.wide != W16_512 ? 0 : F_RUNTIME);
+  const bool compiled = p.wide == W8 || p.wide == W16 || (p.wide == W16_256 && p.vec);
+  const int f = joint_flags(j, p) | (compiled ? 0 : F_RUNTIME);
   shape(j.d, p, joint_backward_threads(p.wide, f));
   const int rows = (int)j.rows, per_sm = joint_backward_blocks(p.wide, f), most = per_sm * psgd_num_sms();
   const int fair = (rows + most - 1) / most;
