@@ -120,10 +120,13 @@ struct Keep {
   }
   PSGD_DEVI bool low(uint32_t word) const { return (word << 16) >= limit; }   // fields 0, 2, 4, 6
   PSGD_DEVI bool high(uint32_t word) const { return word >= limit; }          // fields 1, 3, 5, 7
-  PSGD_DEVI bool one(unsigned long long i) const {
-    const uint4 r = block(i >> 3);
-    const uint32_t k = (uint32_t)i & 7u, w = k < 2 ? r.x : k < 4 ? r.y : k < 6 ? r.z : r.w;
-    return k & 1u ? high(w) : low(w);
+  PSGD_DEVI uint32_t mask8(unsigned long long b) const {  // bit f: field f of the block is kept
+    const uint4 r = block(b);
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m |= (low(w[i]) ? 1u << (2 * i) : 0u) | (high(w[i]) ? 2u << (2 * i) : 0u);
+    return m;
   }
 };
 PSGD_DEVI uint32_t word_of(const uint4& r, int i) { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }

@@ -9,8 +9,7 @@
 // constant along a column is kept out of the rows' loop. The rows to come are copied to shared memory asynchronously,
 // each thread its own 16-byte pieces (which therefore need no barrier).
 //
-// A row belongs to a group of `tpr` threads (whole warps) and a thread to 8 * NV elements of it: with VEC (16-byte
-// aligned rows) vectors of 8 neighbours, tpr vectors apart; otherwise single elements, tpr apart. A block holds
+// A row belongs to a group of `tpr` threads (whole warps) and a thread to 8 * NV elements of it (Place). A block holds
 // blockDim.y groups, each with rows of its own, whose threads meet at a named barrier of the group.
 #pragma once
 #include "elem.cuh"
@@ -100,19 +99,38 @@ PSGD_DEVI void unpack8(uint4 a, F2* v) {
   }
 }
 
-// The elements of a row that are this thread's, eight to a vector. VEC: a vector is H pieces of 16 bytes (T of 16 bits: one
-// of 8 elements; fp32: two of 4), a piece at e(i, h), neighbouring threads' pieces side by side. Otherwise the elements are
-// tpr apart.
+// Bytes [by, by + 16) of the 32 bytes x, y (by < 16).
+PSGD_DEVI uint4 from_byte(const uint4& x, const uint4& y, uint32_t by) {
+  uint32_t z[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  if (by & 4u)
+#pragma unroll
+    for (int k = 0; k < 7; ++k) z[k] = z[k + 1];
+  if (by & 8u)
+#pragma unroll
+    for (int k = 0; k < 5; ++k) z[k] = z[k + 2];
+  const uint32_t bits = (by & 3u) * 8;
+  return make_uint4(__funnelshift_r(z[0], z[1], bits), __funnelshift_r(z[1], z[2], bits), __funnelshift_r(z[2], z[3], bits),
+                    __funnelshift_r(z[3], z[4], bits));
+}
+PSGD_DEVI uint4 shuffle_up(const uint4& v) {
+  return make_uint4(__shfl_up_sync(0xffffffffu, v.x, 1), __shfl_up_sync(0xffffffffu, v.y, 1),
+                    __shfl_up_sync(0xffffffffu, v.z, 1), __shfl_up_sync(0xffffffffu, v.w, 1));
+}
+// The elements of a row that are this thread's: vectors of eight, each H pieces of 16 bytes (T of 16 bits: one of 8
+// elements; fp32: two of 4), a piece at e(i, h), neighbouring threads' pieces side by side. VEC: every row starts on a
+// 16-byte boundary and d is a multiple of 8, so pieces are whole and aligned. Otherwise a piece straddles two aligned
+// ones, of which this thread moves one and a neighbour the other (see Ring16::read and store_row), and the last
+// piece may be cut off by the row's end.
 template <typename T, bool VEC>
 struct Place {
-  static constexpr int H = VEC ? (int)sizeof(T) / 2 : 1, E = 8 / H;  // pieces to a vector, elements to a piece
+  static constexpr int H = (int)sizeof(T) / 2, E = 8 / H;  // pieces to a vector, elements to a piece
   int d, tpr, t;
   PSGD_DEVI Place(int d_) : d(d_), tpr(blockDim.x), t(threadIdx.x) {}
-  PSGD_DEVI int e(int i, int h) const { return VEC ? ((i * H + h) * tpr + t) * E : i * 8 * tpr + t; }
+  PSGD_DEVI int e(int i, int h) const { return ((i * H + h) * tpr + t) * E; }
   PSGD_DEVI bool piece(int i, int h) const { return e(i, h) < d; }
+  PSGD_DEVI bool whole(int i, int h) const { return VEC ? piece(i, h) : e(i, h) + E <= d; }
   PSGD_DEVI bool any(int i) const { return piece(i, 0); }
-  PSGD_DEVI int at(int i, int k) const { return VEC ? e(i, k / E) + k % E : e(i, 0) + k * tpr; }
-  PSGD_DEVI bool has(int i, int k) const { return VEC ? piece(i, k / E) : at(i, k) < d; }
+  PSGD_DEVI bool has(int i, int k) const { return e(i, k / E) + (VEC ? 0 : k % E) < d; }
   PSGD_DEVI F2 only(F2 v, int i, int k) const {  // elements 2 k, 2 k + 1 of vector i, zero where there are none
     if constexpr (VEC) {
       return has(i, 2 * k) ? v : f2(0.f);
@@ -121,59 +139,95 @@ struct Place {
       return f2(has(i, 2 * k) ? f.x : 0.f, has(i, 2 * k + 1) ? f.y : 0.f);
     }
   }
-  template <typename S>  // S: T, or fp32 (a parameter, a sum) in T's places
+  // Vector i of a row of T or of fp32 (a parameter, a sum, a gate); zero beyond d. Aligned where VEC.
+  template <typename S>
   PSGD_DEVI void load(const S* row, int i, F2* v) const {
-    if constexpr (VEC) {
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        F2* to = v + h * (E / 2);
-        if (!piece(i, h)) {
+    for (int h = 0; h < H; ++h) {
+      F2* to = v + h * (E / 2);
+      if (!piece(i, h)) {
 #pragma unroll
-          for (int k = 0; k < E / 2; ++k) to[k] = f2(0.f);
-        } else if constexpr (sizeof(S) == 4) {
+        for (int k = 0; k < E / 2; ++k) to[k] = f2(0.f);
+      } else if constexpr (!VEC) {
+        float f[E];
 #pragma unroll
-          for (int q = 0; q < E / 4; ++q) {
-            const float4 a = reinterpret_cast<const float4*>(row + e(i, h))[q];
-            to[2 * q] = f2(a.x, a.y), to[2 * q + 1] = f2(a.z, a.w);
-          }
-        } else {
-          unpack8<S>(*reinterpret_cast<const uint4*>(row + e(i, h)), to);
+        for (int k = 0; k < E; ++k) f[k] = e(i, h) + k < d ? to_f32(row[e(i, h) + k]) : 0.f;
+#pragma unroll
+        for (int k = 0; k < E / 2; ++k) to[k] = f2(f[2 * k], f[2 * k + 1]);
+      } else if constexpr (sizeof(S) == 4) {
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          const float4 a = reinterpret_cast<const float4*>(row + e(i, h))[q];
+          to[2 * q] = f2(a.x, a.y), to[2 * q + 1] = f2(a.z, a.w);
         }
+      } else {
+        unpack8<S>(*reinterpret_cast<const uint4*>(row + e(i, h)), to);
       }
-    } else {
-      float f[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = has(i, k) ? to_f32(row[at(i, k)]) : 0.f;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = f2(f[2 * k], f[2 * k + 1]);
     }
   }
-  template <typename S>
-  PSGD_DEVI void store(S* row, int i, const F2* v) const {
+  // Vector i into a row of fp32 sums, aligned and as long as d rounded up to 8.
+  PSGD_DEVI void store_sums(float* row, int i, const F2* v) const {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+      if (piece(i, h))
+#pragma unroll
+        for (int q = 0; q < E / 4; ++q) {
+          const float2 a = un2(v[h * (E / 2) + 2 * q]), b = un2(v[h * (E / 2) + 2 * q + 1]);
+          reinterpret_cast<float4*>(row + e(i, h))[q] = make_float4(a.x, a.y, b.x, b.y);
+        }
+  }
+  PSGD_DEVI uint4 pack(int h, const F2* v) const {
+    float f[E];
+#pragma unroll
+    for (int k = 0; k < E / 2; ++k) {
+      const float2 a = un2(v[h * (E / 2) + k]);
+      f[2 * k] = a.x, f[2 * k + 1] = a.y;
+    }
+    if constexpr (H == 2) return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+    else return make_uint4(pack2(f[0], f[1], T()), pack2(f[2], f[3], T()), pack2(f[4], f[5], T()), pack2(f[6], f[7], T()));
+  }
+  PSGD_DEVI static T element(const uint4& w, int k) {  // k is known where it is compiled
+    const uint32_t x = k * (int)sizeof(T) / 4 == 0 ? w.x : k * (int)sizeof(T) / 4 == 1 ? w.y : k * (int)sizeof(T) / 4 == 2 ? w.z : w.w;
+    if constexpr (H == 2) {
+      return __uint_as_float(x);
+    } else {
+      const uint16_t half = (uint16_t)(k & 1 ? x >> 16 : x & 0xFFFFu);
+      return *reinterpret_cast<const T*>(&half);
+    }
+  }
+  // Vector i into a row of T; every thread of the warp calls it. Without VEC, where the row lies `off` bytes past a
+  // boundary, a thread stores the aligned 16 bytes that end in its piece: the last `off` bytes of the piece before and
+  // the first ones of its own. What a warp has no neighbour for, and the row's end, go element by element.
+  PSGD_DEVI void store(T* row, int i, const F2* v) const {
     if constexpr (VEC) {
 #pragma unroll
       for (int h = 0; h < H; ++h)
-        if (piece(i, h)) {
-          float f[E];
-#pragma unroll
-          for (int k = 0; k < E / 2; ++k) {
-            const float2 a = un2(v[h * (E / 2) + k]);
-            f[2 * k] = a.x, f[2 * k + 1] = a.y;
-          }
-          if constexpr (sizeof(S) == 4) {
-#pragma unroll
-            for (int q = 0; q < E / 4; ++q)
-              reinterpret_cast<float4*>(row + e(i, h))[q] = make_float4(f[4 * q], f[4 * q + 1], f[4 * q + 2], f[4 * q + 3]);
-          } else {
-            store_vec<S, 8>(row + e(i, h), f);
-          }
-        }
+        if (piece(i, h)) *reinterpret_cast<uint4*>(row + e(i, h)) = pack(h, v);
     } else {
+      const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+      const int lane = t & 31, back = (int)(off / sizeof(T));  // elements that the thread's own store leaves to the next
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = un2(v[k]);
-        if (has(i, 2 * k)) row[at(i, 2 * k)] = from_f32<S>(f.x);
-        if (has(i, 2 * k + 1)) row[at(i, 2 * k + 1)] = from_f32<S>(f.y);
+      for (int h = 0; h < H; ++h) {
+        const uint4 mine = pack(h, v);
+        const int at = e(i, h);
+        uint4 out = mine;
+        if (off) out = from_byte(shuffle_up(mine), mine, 16u - off);
+        const bool full = at - back + E <= d && (lane > 0 || off == 0);
+        if (full) *reinterpret_cast<uint4*>(row + at - back) = out;
+        // The first thread's own elements, the last one's left-over ones, and the row's end (which the last thread may meet
+        // before its left-over ones: those then lie beyond it).
+        const bool rest = full && lane == 31 && off;
+        if (!full || rest) {
+          const int first = full ? at : at - back, least = full ? E - back : lane > 0 ? 0 : back;
+          if (full) out = mine;
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (k >= least && first + k < d) row[first + k] = element(out, k);
+        }
+        if (!full && lane == 31 && off)
+#pragma unroll
+          for (int k = 0; k < E; ++k)
+            if (k >= E - back && at + k < d) row[at + k] = element(mine, k);
       }
     }
   }
@@ -191,10 +245,10 @@ struct Place {
   // v with what dropout does not keep set to zero.
   PSGD_DEVI void drop(const Keep& keep, long long row, int i, F2* v) const {
     const unsigned long long at0 = (unsigned long long)row * d;
-    if constexpr (VEC) {  // (d is a multiple of 8: a piece lies in one block of the generator)
 #pragma unroll
-      for (int h = 0; h < H; ++h) {
-        const unsigned long long first = at0 + e(i, h);
+    for (int h = 0; h < H; ++h) {
+      const unsigned long long first = at0 + e(i, h);
+      if constexpr (VEC) {  // (d is a multiple of 8: a piece lies in one block of the generator)
         const uint4 words = keep.block(first >> 3);
         const bool upper = H == 2 && (first & 4);
 #pragma unroll
@@ -203,16 +257,15 @@ struct Place {
           const float2 f = un2(v[h * (E / 2) + k]);
           v[h * (E / 2) + k] = f2(keep.low(w) ? f.x : 0.f, keep.high(w) ? f.y : 0.f);
         }
-      }
-    } else {
-      uint32_t m = 0;
-#pragma unroll 1
-      for (int k = 0; k < 8; ++k)
-        if (has(i, k)) m |= (uint32_t)keep.one(at0 + at(i, k)) << k;
+      } else {
+        const uint32_t o = (uint32_t)first & 7u;
+        uint32_t m = keep.mask8(first >> 3) >> o;
+        if (o + E > 8) m |= keep.mask8((first >> 3) + 1) << (8 - o);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float2 f = un2(v[k]);
-        v[k] = f2((m >> (2 * k)) & 1u ? f.x : 0.f, (m >> (2 * k + 1)) & 1u ? f.y : 0.f);
+        for (int k = 0; k < E / 2; ++k) {
+          const float2 f = un2(v[h * (E / 2) + k]);
+          v[h * (E / 2) + k] = f2((m >> (2 * k)) & 1u ? f.x : 0.f, (m >> (2 * k + 1)) & 1u ? f.y : 0.f);
+        }
       }
     }
   }
@@ -258,20 +311,30 @@ struct GroupSum {
 
 // ---- the rows to come -------------------------------------------------------------------------------------------------
 // A ring of `stages` rows' pieces, ARR arrays each, in shared memory: this thread's 16-byte pieces, a block's threads
-// side by side (no bank conflicts). fetch() starts a row's copies (null arrays are skipped, and stay zero where they
-// were cleared), wait() waits for the oldest row, read() unpacks a piece of it.
-template <typename T, int NV, int ARR>
+// side by side (no bank conflicts). fetch() starts a row's copies (null arrays are skipped), wait() waits for the oldest
+// row, read() unpacks a piece of it. Without VEC the copies are of the aligned 16 bytes in which the thread's piece
+// begins (never beyond the row's end), the last thread of a warp copies the next ones too, and read() takes the rest of
+// the piece from the next thread's; what lies beyond d reads as zero. Every thread of a warp calls all of them.
+template <typename T, bool VEC, int NV, int ARR>
 struct Ring16 {
-  static constexpr int H = sizeof(T) / 2;  // 16-byte pieces to 8 elements
-  uint32_t base, apart, stage, all, put, get;  // bytes: first piece, from piece to piece, of a stage, of the ring; turns
-  int stages;
-  PSGD_DEVI Ring16(void* smem, int s) : put(0), get(0), stages(s) {
-    apart = blockDim.x * blockDim.y * 16;
+  using At = Place<T, VEC>;
+  static constexpr int H = At::H;  // 16-byte pieces to 8 elements
+  uint32_t base, apart, extra, extra_apart, stage, extra_stage, put, get;  // bytes
+  int stages, put_turn, get_turn;
+  PSGD_DEVI Ring16(void* smem, int s) : put(0), get(0), stages(s), put_turn(0), get_turn(0) {
+    const uint32_t threads = blockDim.x * blockDim.y, thread = threadIdx.y * blockDim.x + threadIdx.x;
+    apart = threads * 16;
     stage = apart * (ARR * NV * H);
-    all = stage * s;
-    base = smem_u32(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+    base = smem_u32(smem) + thread * 16;
+    extra_apart = threads / 32 * 16;
+    extra_stage = extra_apart * (ARR * NV * H);
+    extra = smem_u32(smem) + stage * s + thread / 32 * 16;
   }
-  PSGD_DEVI void fetch(const Place<T, true>& at, const T* const* rows, bool there) {
+  PSGD_DEVI static void copy(uint32_t to, const void* p, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(p), "r"(n) : "memory");
+  }
+  PSGD_DEVI void fetch(const At& at, const T* const* rows, bool there) {
+    if (!VEC) __syncwarp();  // (the row that was there has been read by the thread before, too)
     if (there)
 #pragma unroll
       for (int a = 0; a < ARR; ++a)
@@ -279,40 +342,66 @@ struct Ring16 {
 #pragma unroll
           for (int i = 0; i < NV; ++i)
 #pragma unroll
-            for (int h = 0; h < H; ++h)
-              if (at.piece(i, h))
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;"
-                             ::"r"(base + put + apart * ((a * NV + i) * H + h)), "l"(rows[a] + at.e(i, h))
-                             : "memory");
+            for (int h = 0; h < H; ++h) {
+              const int n = (a * NV + i) * H + h;
+              if constexpr (VEC) {
+                if (at.piece(i, h))
+                  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + put + apart * n), "l"(rows[a] + at.e(i, h))
+                               : "memory");
+              } else {
+                const char* p = reinterpret_cast<const char*>(rows[a] + at.e(i, h));
+                const char* end = reinterpret_cast<const char*>(rows[a] + at.d);
+                const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(p) & 15u;
+                p -= off;
+                if (p < end) copy(base + put + apart * n, p, (int)min((long long)(end - p), 16LL));
+                p += 16;
+                if ((threadIdx.x & 31) == 31 && off && p < end)
+                  copy(extra + put_turn * extra_stage + extra_apart * n, p, (int)min((long long)(end - p), 16LL));
+              }
+            }
     asm volatile("cp.async.commit_group;" ::: "memory");
     put += stage;
-    if (put == all) put = 0;
+    if (++put_turn == stages) put = 0, put_turn = 0;
   }
   PSGD_DEVI void wait() {  // one group was committed for each of the stages - 1 rows after the oldest
     if (stages == 3) asm volatile("cp.async.wait_group 2;" ::: "memory");
     else if (stages == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
     else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    if (!VEC) __syncwarp();  // (the next thread's pieces are read, too)
   }
-  PSGD_DEVI void read(const Place<T, true>& at, int a, int i, F2* v) const {
+  PSGD_DEVI static uint4 word4(uint32_t at) {
+    uint4 x;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(at) : "memory");
+    return x;
+  }
+  // Vector i of array a, whose row is `row` (its address alone is used).
+  PSGD_DEVI void read(const At& at, const T* row, int a, int i, F2* v) const {
 #pragma unroll
     for (int h = 0; h < H; ++h) {
+      const int n = (a * NV + i) * H + h;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (at.piece(i, h))
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                     : "r"(base + get + apart * ((a * NV + i) * H + h))
-                     : "memory");
+      if constexpr (VEC) {
+        if (at.piece(i, h)) x = word4(base + get + apart * n);
+      } else {
+        const uint32_t off = (uint32_t)reinterpret_cast<uintptr_t>(row) & 15u;
+        x = word4(base + get + apart * n);
+        if (off)
+          x = from_byte(x, word4((threadIdx.x & 31) == 31 ? extra + get_turn * extra_stage + extra_apart * n : base + get + apart * n + 16), off);
+      }
       if constexpr (H == 2) {
         v[2 * h] = f2(__uint_as_float(x.x), __uint_as_float(x.y));
         v[2 * h + 1] = f2(__uint_as_float(x.z), __uint_as_float(x.w));
       } else {
         unpack8<T>(x, v);
       }
+      if (!VEC && !at.whole(i, h))
+#pragma unroll
+        for (int k = 0; k < At::E / 2; ++k) v[h * (At::E / 2) + k] = at.only(v[h * (At::E / 2) + k], i, h * (At::E / 2) + k);
     }
   }
   PSGD_DEVI void next() {
     get += stage;
-    if (get == all) get = 0;
+    if (++get_turn == stages) get = 0, get_turn = 0;
   }
 };
 
@@ -339,19 +428,17 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
   const float inv_d = 1.f / (float)d;
   const int step = gridDim.x * blockDim.y, rows_all = (int)j.rows, ld_x = (int)j.ld_x, ld_y = (int)j.ld_y;
   const bool one_gate = j.gate && p.per_gate == rows_all, row_gate = j.gate && !one_gate;
-  Ring16<T, NV, 2> ring(smem, p.stages);
+  Ring16<T, VEC, NV, 2> ring(smem, p.stages);
 
   auto sources = [&](int row, const T** rows) {
     rows[0] = reinterpret_cast<const T*>(j.x) + (long long)row * ld_x;
     rows[1] = reinterpret_cast<const T*>(j.y) + (long long)row * ld_y;
   };
   int row = blockIdx.x * blockDim.y + threadIdx.y, ahead = row;
-  if constexpr (VEC) {
-    for (int s = 0; s + 1 < p.stages; ++s, ahead += step) {
-      const T* rows[2];
-      sources(ahead, rows);
-      ring.fetch(at, rows, ahead < rows_all);
-    }
+  for (int s = 0; s + 1 < p.stages; ++s, ahead += step) {
+    const T* rows[2];
+    sources(ahead, rows);
+    ring.fetch(at, rows, ahead < rows_all);
   }
   F2 w[P], b[P], f[P], fb[P];
 #pragma unroll
@@ -404,27 +491,18 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
 
   for (; row < rows_all; row += step) {
     F2 u[P], x[P];
-    if constexpr (VEC) {
-      const T* rows[2];
-      sources(ahead, rows);
-      ring.fetch(at, rows, ahead < rows_all);
-      ahead += step;
-      ring.wait();
+    const T* rows[2];
+    sources(ahead, rows);
+    ring.fetch(at, rows, ahead < rows_all);
+    ahead += step;
+    ring.wait();
+    sources(row, rows);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        ring.read(at, 0, i, x + i * 4);
-        ring.read(at, 1, i, u + i * 4);
-      }
-      ring.next();
-    } else {
-      const T* rows[2];
-      sources(row, rows);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        at.load(rows[0], i, x + i * 4);
-        at.load(rows[1], i, u + i * 4);
-      }
+    for (int i = 0; i < NV; ++i) {
+      ring.read(at, rows[0], 0, i, x + i * 4);
+      ring.read(at, rows[1], 1, i, u + i * 4);
     }
+    ring.next();
     T* po = reinterpret_cast<T*>(j.out) + (long long)row * d;
     T* pn = reinterpret_cast<T*>(j.normed) + (long long)row * d;
     float mean_y = 0.f, r_y = 1.f, mean_o, r_o;
@@ -432,7 +510,6 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
     const F2 ry = f2(r_y), my = f2(-mean_y * r_y);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      if (!at.any(i)) continue;
       F2* ui = u + i * 4;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -550,7 +627,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
   constexpr int ARRAYS = RT || (F & (F_POST | F_GATE)) ? 4 : 3;  // d_normed, d_out, out and, where it is needed, y
-  Ring16<T, NV, ARRAYS> ring(smem, p.stages);
+  Ring16<T, VEC, NV, ARRAYS> ring(smem, p.stages);
 
   JointRows it;
   it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
@@ -612,51 +689,32 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
   }
 
   JointRows ahead = it;
-  if constexpr (VEC) {
-    for (int s = 0; s + 1 < p.stages; ++s) {
-      const T* rows[4];
-      const bool there = ahead.there();
-      sources(ahead.row, rows);
-      ring.fetch(at, rows, there);
-      if (there) ahead.next();
-    }
+  for (int s = 0; s + 1 < p.stages; ++s) {
+    const T* rows[4];
+    const bool there = ahead.there();
+    sources(ahead.row, rows);
+    ring.fetch(at, rows, there);
+    if (there) ahead.next();
   }
   bool fresh = true;  // the gate group's factor is to be formed
   for (; it.there(); it.next()) {
     const int row = it.row;
     const float4 st = reinterpret_cast<const float4*>(j.stats)[row];
     F2 dn[P], hat[P], dx[P], y[P];
-    if constexpr (VEC) {
-      const T* rows[4];
-      const bool there = ahead.there();
-      sources(ahead.row, rows);
-      ring.fetch(at, rows, there);
-      if (there) ahead.next();
-      ring.wait();
+    const T* rows[4];
+    const bool there = ahead.there();
+    sources(ahead.row, rows);
+    ring.fetch(at, rows, there);
+    if (there) ahead.next();
+    ring.wait();
+    sources(row, rows);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (j.d_normed) ring.read(at, 0, i, dn + i * 4);
-        else
+    for (int i = 0; i < NV; ++i) {
+      if (j.d_normed) ring.read(at, rows[0], 0, i, dn + i * 4);
+      else
 #pragma unroll
-          for (int k = 0; k < 4; ++k) dn[i * 4 + k] = f2(0.f);
-        ring.read(at, 2, i, hat + i * 4);
-      }
-    } else {
-      const T* rows[4];
-      sources(row, rows);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        at.load(rows[2], i, hat + i * 4);
-        if (rows[0]) at.load(rows[0], i, dn + i * 4);
-        else
-#pragma unroll
-          for (int k = 0; k < 4; ++k) dn[i * 4 + k] = f2(0.f);
-        if (rows[1]) at.load(rows[1], i, dx + i * 4);
-        else
-#pragma unroll
-          for (int k = 0; k < 4; ++k) dx[i * 4 + k] = f2(0.f);
-        if (use_y) at.load(rows[3], i, y + i * 4);
-      }
+        for (int k = 0; k < 4; ++k) dn[i * 4 + k] = f2(0.f);
+      ring.read(at, rows[2], 2, i, hat + i * 4);
     }
     F2 s0 = f2(0.f), s1 = f2(0.f);
     {
@@ -679,17 +737,16 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
     }
     float s[2] = {sum2(s0), sum2(s1)};
     sum(s);
-    if constexpr (VEC) {  // (read after the sum: what waits in shared memory needs no registers)
+    // (read after the sum: what waits in shared memory needs no registers)
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        if (j.d_out) ring.read(at, 1, i, dx + i * 4);
-        else
+    for (int i = 0; i < NV; ++i) {
+      if (j.d_out) ring.read(at, rows[1], 1, i, dx + i * 4);
+      else
 #pragma unroll
-          for (int k = 0; k < 4; ++k) dx[i * 4 + k] = f2(0.f);
-        if (use_y) ring.read(at, 3, i, y + i * 4);
-      }
-      ring.next();
+        for (int k = 0; k < 4; ++k) dx[i * 4 + k] = f2(0.f);
+      if (use_y) ring.read(at, rows[3], 3, i, y + i * 4);
     }
+    ring.next();
     if (direct && fresh) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
@@ -756,7 +813,6 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
         const T* pg = reinterpret_cast<const T*>(j.gate) + (long long)it.g * d;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          if (!at.any(i)) continue;
           F2 g[4], pw[4], pb[4], v[4];
           at.load(pg, i, g);
           if (post) {
@@ -815,7 +871,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
     float* mine = share + turn * blockDim.y * dp;
     turn ^= 1;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) at.store(mine + threadIdx.y * dp, i, v + i * 4);
+    for (int i = 0; i < NV; ++i) at.store_sums(mine + threadIdx.y * dp, i, v + i * 4);
     __syncthreads();
     float* to = part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp;
     T* whole = a == 4 && p.chunks == 1 ? reinterpret_cast<T*>(j.dgate) + (long long)gate_row * d : nullptr;
@@ -834,7 +890,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 }
 
 // Rows of over 4096 elements: 512 threads have 128 registers each, which the sums over rows half fill. The row stays in
-// shared memory (without VEC: is read again) and each step of it goes through the thread's elements eight at a time,
+// shared memory and each step of it goes through the thread's elements eight at a time,
 // forming again what the step before had; everything else is as above.
 template <typename T, bool VEC, bool DIRECT>
 __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJoint j, const JointPlan p, float* part) {
@@ -858,7 +914,7 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
   constexpr int ARRAYS = RT || (F & (F_POST | F_GATE)) ? 4 : 3;  // d_normed, d_out, out and, where it is needed, y
-  Ring16<T, NV, ARRAYS> ring(smem, p.stages);
+  Ring16<T, VEC, NV, ARRAYS> ring(smem, p.stages);
 
   JointRows it;
   it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
@@ -920,38 +976,29 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
   }
 
   JointRows ahead = it;
-  if constexpr (VEC) {
-    for (int s = 0; s + 1 < p.stages; ++s) {
-      const T* rows[4];
-      const bool there = ahead.there();
-      sources(ahead.row, rows);
-      ring.fetch(at, rows, there);
-      if (there) ahead.next();
-    }
+  for (int s = 0; s + 1 < p.stages; ++s) {
+    const T* rows[4];
+    const bool there = ahead.there();
+    sources(ahead.row, rows);
+    ring.fetch(at, rows, there);
+    if (there) ahead.next();
   }
   bool fresh = true;  // the gate group's factor is to be formed
   for (; it.there(); it.next()) {
     const int row = it.row;
     const float4 st = reinterpret_cast<const float4*>(j.stats)[row];
-    const T* now[4];
-    sources(row, now);
-    if constexpr (VEC) {
-      const T* rows[4];
-      const bool there = ahead.there();
-      sources(ahead.row, rows);
-      ring.fetch(at, rows, there);
-      if (there) ahead.next();
-      ring.wait();
-    }
+    const T* rows[4];
+    const bool there = ahead.there();
+    sources(ahead.row, rows);
+    ring.fetch(at, rows, there);
+    if (there) ahead.next();
+    ring.wait();
+    sources(row, rows);
     auto get = [&](int a, int i, F2* v) {
-      if (!now[a]) {
+      if (rows[a]) ring.read(at, rows[a], a, i, v);
+      else
 #pragma unroll
         for (int k = 0; k < 4; ++k) v[k] = f2(0.f);
-      } else if constexpr (VEC) {
-        ring.read(at, a, i, v);
-      } else {
-        at.load(now[a], i, v);
-      }
     };
     const F2 r = f2(st.w), m0 = f2(layer ? -st.z * st.w : 0.f), ry = f2(st.y), my = f2(layer ? -st.x * st.y : 0.f);
     auto hats = [&](int i, F2* dh, F2* hat) {  // d_normed and hat of vector i
@@ -1044,14 +1091,13 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
         at.store(reinterpret_cast<T*>(j.dy) + (long long)row * d, i, m);
       }
     }
-    if constexpr (VEC) ring.next();
+    ring.next();
     if (direct) {
       fresh = it.last_of_gate();
       if (fresh) {  // the gate group ends here, and with it its gradient
         const T* pg = reinterpret_cast<const T*>(j.gate) + (long long)it.g * d;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          if (!at.any(i)) continue;
           F2 g[4], pw[4], pb[4], v[4];
           at.load(pg, i, g);
           if (post) {
@@ -1110,7 +1156,7 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
     float* mine = share + turn * blockDim.y * dp;
     turn ^= 1;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) at.store(mine + threadIdx.y * dp, i, v + i * 4);
+    for (int i = 0; i < NV; ++i) at.store_sums(mine + threadIdx.y * dp, i, v + i * 4);
     __syncthreads();
     float* to = part + ((size_t)p.slot[a] * p.blocks + blockIdx.x) * dp;
     T* whole = a == 4 && p.chunks == 1 ? reinterpret_cast<T*>(j.dgate) + (long long)gate_row * d : nullptr;

@@ -85,6 +85,12 @@ int per_sm(const JointPlan& p, int compiled) {
   return n < 1 ? 1 : n;
 }
 
+// Shared memory of the rings.
+int ring_bytes(const JointPlan& p, int arrays, int dtype) {
+  const int threads = p.tpr * p.groups;
+  return p.stages * arrays * p.nv * size_of(dtype) / 2 * (threads + (p.vec ? 0 : threads / 32)) * 16;
+}
+
 JointPlan plan_forward(const PsgdJoint& j) {
   JointPlan p = {};
   p.vec = j.d % 8 == 0 && params_aligned(j) && rows_aligned(j.x, j.ld_x, j.dtype) && rows_aligned(j.y, j.ld_y, j.dtype) &&
@@ -92,7 +98,7 @@ JointPlan plan_forward(const PsgdJoint& j) {
           (!j.gate || rows_aligned(j.gate, j.d, j.dtype));
   shape(j.d, p, 0);
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
-  p.smem = p.vec ? p.stages * 2 * p.nv * p.tpr * p.groups * 8 * size_of(j.dtype) : 0;
+  p.smem = ring_bytes(p, 2, j.dtype);
   p.per_gate = j.gate ? (int)(j.rows / j.gates) : 1;
   const int want = ((int)j.rows + p.groups - 1) / p.groups, most = per_sm(p, joint_forward_blocks(p.wide, joint_flags(j, p))) * psgd_num_sms();
   p.blocks = want < most ? want : most;
@@ -123,10 +129,10 @@ JointPlan plan_backward(const PsgdJoint& j) {
   // Rows ahead: two for 16-bit types, one for fp32, as far as shared memory goes.
   const int threads = p.tpr * p.groups, columns = threads * p.nv * 64;
   const int arrays = p.wide == W16_512 || j.post || j.gate ? 4 : 3;
-  const int row = arrays * p.nv * threads * 8 * size_of(j.dtype), room = 220 * 1024 / per_sm - columns;
+  const int room = 220 * 1024 / per_sm - columns;
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
-  while (p.stages > 1 && p.stages * row > room) --p.stages;
-  p.ring = p.vec ? p.stages * row : 0;
+  while (p.stages > 1 && ring_bytes(p, arrays, j.dtype) > room) --p.stages;
+  p.ring = ring_bytes(p, arrays, j.dtype);
   p.smem = p.ring + columns;
   const int share = 2 * p.groups * round_up(j.d, 8) * 4;
   if (p.smem < share) p.smem = share;
