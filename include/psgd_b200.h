@@ -485,6 +485,8 @@ typedef struct PsgdLce {
 } PsgdLce;
 long long psgd_lce_workspace(const PsgdLce* a);
 int psgd_lce(const PsgdLce* a, int* dev_err, cudaStream_t stream);
+/* x (n values of dtype) *= *factor, a device scalar; a factor of one costs a launch and no traffic. */
+int psgd_lce_scale(void* x, int dtype, long long n, const float* factor, cudaStream_t stream);
 
 #ifdef __cplusplus
 }

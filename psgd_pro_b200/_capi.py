@@ -187,6 +187,7 @@ SIGNATURES = [
     ("psgd_joint_backward", c_int, [ctypes.POINTER(Joint), c_vp, c_ll, c_vp]),
     ("psgd_lce_workspace", c_ll, [ctypes.POINTER(Lce)]),
     ("psgd_lce", c_int, [ctypes.POINTER(Lce), c_vp, c_vp]),
+    ("psgd_lce_scale", c_int, [c_vp, c_int, c_ll, c_vp, c_vp]),
 ]
 
 # device error word bits (include/psgd_b200.h PSGD_ERR_*)

@@ -947,6 +947,21 @@ __global__ void __launch_bounds__(1024) lce_loss_kernel(const float* __restrict_
   if (threadIdx.x == 0) *loss = mean ? s / (float)max(n, 1) : s;
 }
 
+// x *= *factor, unless that is one (then nothing is read): the upstream gradient of a loss, which is nearly always one.
+template <typename T>
+__global__ void __launch_bounds__(256) lce_scale_kernel(T* __restrict__ x, long long n, const float* __restrict__ factor) {
+  const float f = *factor;
+  if (f == 1.f) return;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256)
+    x[i] = from_f32<T>(to_f32(x[i]) * f);
+}
+template <typename T>
+int scale(void* x, long long n, const float* factor, cudaStream_t stream) {
+  const long long want = (n + 255) / 256, most = 16LL * psgd_num_sms();
+  lce_scale_kernel<T><<<(int)(want < most ? want : most), 256, 0, stream>>>(reinterpret_cast<T*>(x), n, factor);
+  return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
+}
+
 // Joins the splits of a gradient: out[row] = alpha * sum over splits, in their order. Rows are the counted ones through
 // row_of, or all M of them as they are. V: values at a time (N a multiple, or 1).
 template <typename T, int V>
@@ -1250,5 +1265,17 @@ extern "C" int psgd_lce(const PsgdLce* a, int* dev_err, cudaStream_t stream) {
     case PSGD_F32: return run<float, __nv_bfloat16, float>(*a, dev_err, stream);
     case PSGD_BF16: return run<__nv_bfloat16, __nv_bfloat16, __half>(*a, dev_err, stream);
     default: return run<__half, __half, __half>(*a, dev_err, stream);
+  }
+}
+
+extern "C" int psgd_lce_scale(void* x, int dtype, long long n, const float* factor, cudaStream_t stream) {
+  using namespace psgd;
+  if (n < 0 || !factor || (n > 0 && !x)) return PSGD_EINVAL;
+  if (n == 0) return PSGD_OK;
+  switch (dtype) {
+    case PSGD_F32: return scale<float>(x, n, factor, stream);
+    case PSGD_BF16: return scale<__nv_bfloat16>(x, n, factor, stream);
+    case PSGD_F16: return scale<__half>(x, n, factor, stream);
+    default: return PSGD_EINVAL;
   }
 }

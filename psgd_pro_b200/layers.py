@@ -401,17 +401,33 @@ def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduc
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
+    """A scalar loss forms its gradients in the forward pass (6 N V D operations for everything; the backward pass then
+    only scales them, if the upstream gradient is not one). Losses by row, whose upstream gradients are not known yet, and
+    fp16, where a gradient before the upstream scale may be below the type's range, form them in the backward pass
+    (8 N V D)."""
+
     @staticmethod
     def forward(ctx, h, w, target, options):
-        ctx.options = options
+        ctx.options, ctx.grads = options, None
+        ctx.early = options["reduction"] != "none" and h.dtype != torch.float16
         ctx.save_for_backward(h, w, target)
-        return _lce(h, w, target, False, None, **options)[0]
+        loss, *grads = _lce(h, w, target, ctx.early, None, **options)
+        if ctx.early:
+            ctx.grads = grads
+        return loss
 
     @staticmethod
     def backward(ctx, grad):
-        h, w, target = ctx.saved_tensors
-        _, dh, dw = _lce(h, w, target, True, grad.float(), **ctx.options)
-        return dh if ctx.needs_input_grad[0] else None, dw if ctx.needs_input_grad[1] else None, None, None
+        need, grads = ctx.needs_input_grad, ctx.grads
+        ctx.grads = None  # they are the caller's now: a second pass (retain_graph) forms its own, in the same way
+        if grads is None:
+            h, w, target = ctx.saved_tensors
+            _, *grads = _lce(h, w, target, True, None if ctx.early else grad, **ctx.options)
+        if ctx.early:
+            for t, used in zip(grads, need):
+                if used and t.numel():
+                    _launch(t.get_device(), _capi.lib().psgd_lce_scale, t.data_ptr(), _TYPES[t.dtype], t.numel(), grad.data_ptr())
+        return grads[0] if need[0] else None, grads[1] if need[1] else None, None, None
 
 
 def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: int = -100, label_smoothing: float = 0.0,
@@ -424,10 +440,10 @@ def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: 
     (not even with NaN in h); 'mean' divides by the number of the others (0 when there is none). reduction 'none' keeps
     target's shape.
 
-    Under autograd the forward call keeps h, w and target only, and the backward call forms the loss again with both
-    gradients; where the gradient is wanted in any case linear_cross_entropy_grad does all in one (the same kernels, a
-    quarter fewer operations). piece_bytes bounds what is kept of the vocabulary's probabilities at a time (16 bits each,
-    fp32: 80 bits); tokens are taken in pieces of that size."""
+    Under autograd a scalar loss (mean, sum) of bf16 or fp32 inputs that require gradients forms them at once and holds
+    them for the backward pass; otherwise the backward pass forms loss and gradients again. Evaluation belongs under
+    torch.no_grad(). piece_bytes bounds what is kept of the vocabulary's probabilities at a time (16 bits each; fp32: 80
+    bits); tokens are taken in pieces of that size (of 128 at least)."""
     options = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, z_loss=z_loss, reduction=reduction,
                    piece_bytes=piece_bytes)
     if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
