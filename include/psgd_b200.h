@@ -468,8 +468,9 @@ int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cu
  * target sets PSGD_ERR_BAD_TARGET and counts nothing either). With lse = log sum exp of a row's logits l:
  *   loss = (1 - label_smoothing) (lse - l_target) + label_smoothing (lse - mean l) + z_loss lse^2
  * reduction PSGD_REDUCE_NONE (loss: n values, 0 where ignored), _MEAN over the counted rows (0 when there is none) or
- * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type, for the upstream
- * gradient grad (n values for _NONE, one otherwise; NULL: ones). Tokens are taken in pieces of at most piece_bytes of
+ * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type (either may be
+ * NULL), for the upstream gradient grad (n values for _NONE, one otherwise; NULL: ones). fp16: 1 + 2 z_loss lse stays
+ * below 255. Tokens are taken in pieces of at most piece_bytes of
  * kept exponentials (and at least 128 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
  * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong. */
 #define PSGD_REDUCE_NONE 0

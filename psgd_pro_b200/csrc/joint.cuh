@@ -88,6 +88,11 @@ PSGD_DEVI float sum2(F2 a) {
   return f.x + f.y;
 }
 
+PSGD_DEVI F2 where_nonzero(F2 m, F2 v) {  // v where m is not zero, zero elsewhere
+  const float2 a = un2(m), b = un2(v);
+  return f2(a.x != 0.f ? b.x : 0.f, a.y != 0.f ? b.y : 0.f);
+}
+
 // Eight 16-bit elements as four pairs.
 template <typename T>
 PSGD_DEVI void unpack8(uint4 a, F2* v) {
@@ -780,6 +785,7 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
         const F2 m = at.only(dx[n], i, k);  // (beyond d a layer norm's dx is not zero)
         if (use_y) {
           if (post) y[n] = layer ? fma2(y[n], ry, my) : mul2(y[n], ry);
+          else if (drop) y[n] = where_nonzero(m, y[n]);  // (an infinity that was dropped stays out of the gate's gradient)
           A[n] = fma2(m, y[n], A[n]);
         }
         if (post && layer) B[n] = add2(B[n], m);
@@ -1067,6 +1073,7 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
       at.store(reinterpret_cast<T*>(j.dx) + (long long)row * d, i, dx);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
+        if (use_y && !post && drop) y[k] = where_nonzero(m[k], y[k]);
         if (use_y) A[i * 4 + k] = fma2(m[k], y[k], A[i * 4 + k]);
         B[i * 4 + k] = add2(B[i * 4 + k], m[k]);
         m[k] = mul2(m[k], f[k]);

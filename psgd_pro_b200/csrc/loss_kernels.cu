@@ -1199,32 +1199,33 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
     if (!a.grads) continue;
 
     const uint16_t* gm = reinterpret_cast<const uint16_t*>(ws + l.g);
-    LceProblem& ph = args.p[0];  // dh = g w: g K-major, w (rows of K = vocabulary) MN-major
-    ph = LceProblem{};
-    for (int i = 0; i < l.limbs; ++i) {
-      if (int rc = encode(&ph.ta[i], gm + i * l.g_plane, half, rows, a.v, l.ld_kept, 128)) return rc;
-      if (int rc = encode(&ph.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, 64)) return rc;
+    args.nproblems = 0;
+    if (a.dh) {  // dh = g w: g K-major, w (rows of K = vocabulary) MN-major
+      LceProblem& ph = args.p[args.nproblems++] = LceProblem{};
+      for (int i = 0; i < l.limbs; ++i) {
+        if (int rc = encode(&ph.ta[i], gm + i * l.g_plane, half, rows, a.v, l.ld_kept, 128)) return rc;
+        if (int rc = encode(&ph.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, 64)) return rc;
+      }
+      ph.b_mn = 1, ph.M = rows, ph.N = a.d, ph.K = a.v, ph.dyn = 1, ph.row0 = row0, ph.splits = l.splits;
+      ph.row_of = row_of, ph.out = a.dh, ph.ld_out = a.d, ph.ld_part = l.ld_part;
+      ph.part = l.splits > 1 ? reinterpret_cast<float*>(ws + l.part) : nullptr;
     }
-    ph.b_mn = 1, ph.M = rows, ph.N = a.d, ph.K = a.v, ph.dyn = 1, ph.row0 = row0, ph.splits = l.splits;
-    ph.row_of = row_of, ph.out = a.dh, ph.ld_out = a.d;
-    ph.part = l.splits > 1 ? reinterpret_cast<float*>(ws + l.part) : nullptr;
-    ph.ld_part = l.ld_part;
-    LceProblem& pw = args.p[1];  // dw = g^T h: both with rows of K = tokens
-    pw = LceProblem{};
-    for (int i = 0; i < l.limbs; ++i) {
-      if (int rc = encode(&pw.ta[i], gm + i * l.g_plane, half, rows64, a.v, l.ld_kept, 64)) return rc;
-      if (int rc = encode(&pw.tb[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows64, a.d, l.ld_h, 64)) return rc;
+    if (a.dw) {  // dw = g^T h: both with rows of K = tokens
+      LceProblem& pw = args.p[args.nproblems++] = LceProblem{};
+      for (int i = 0; i < l.limbs; ++i) {
+        if (int rc = encode(&pw.ta[i], gm + i * l.g_plane, half, rows64, a.v, l.ld_kept, 64)) return rc;
+        if (int rc = encode(&pw.tb[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows64, a.d, l.ld_h, 64)) return rc;
+      }
+      pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = l.splits_w;
+      pw.out = a.dw, pw.ld_out = a.d, pw.ld_part = l.ld_part;
+      pw.part = l.splits_w > 1 ? reinterpret_cast<float*>(ws + l.part_w) : nullptr;
+      if (l.pieces > 1) {
+        float* acc = sizeof(T) == 4 ? reinterpret_cast<float*>(a.dw) : reinterpret_cast<float*>(ws + l.acc);
+        pw.acc = piece > 0 ? acc : nullptr;
+        pw.acc_out = piece + 1 < l.pieces ? acc : nullptr;
+        pw.ld_acc = sizeof(T) == 4 ? a.d : l.ld_part;
+      }
     }
-    pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = l.splits_w;
-    pw.part = l.splits_w > 1 ? reinterpret_cast<float*>(ws + l.part_w) : nullptr;
-    pw.ld_part = l.ld_part, pw.out = a.dw, pw.ld_out = a.d;
-    if (l.pieces > 1) {
-      float* acc = sizeof(T) == 4 ? reinterpret_cast<float*>(a.dw) : reinterpret_cast<float*>(ws + l.acc);
-      pw.acc = piece > 0 ? acc : nullptr;
-      pw.acc_out = piece + 1 < l.pieces ? acc : nullptr;
-      pw.ld_acc = sizeof(T) == 4 ? a.d : l.ld_part;
-    }
-    args.nproblems = 2;
     args.chunk = LIMBS == 1 ? 1 << 20 : 8;  // (a 16-bit gradient's own rounding is a hundred times the truncation)
     if (!none && piece + 1 == l.pieces) args.loss_rows = loss_rows, args.loss = a.loss, args.mean = mean;
     if (int rc = product_bn<OP, T, LIMBS, false>(l.bn_grads, args, stream)) return rc;
@@ -1235,10 +1236,9 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
                         dim3(256), 0, stream, (const float*)p.part, p.splits, p.M, a.d, p.ld_part, row0, p.row_of,
                         reinterpret_cast<T*>(out), (const LceState*)state);
     };
-    if (l.splits > 1)
-      if (int rc = join(ph, a.dh)) return rc;
-    if (l.splits_w > 1)
-      if (int rc = join(pw, a.dw)) return rc;
+    for (int i = 0; i < args.nproblems; ++i)
+      if (args.p[i].part)
+        if (int rc = join(args.p[i], args.p[i].out)) return rc;
   }
   if (!none && !a.grads)
     return pdl_launch(lce_loss_kernel, dim3(1), dim3(1024), 0, stream, (const float*)loss_rows, (const LceState*)state, (int)mean,
@@ -1258,7 +1258,7 @@ extern "C" long long psgd_lce_workspace(const PsgdLce* a) {
 extern "C" int psgd_lce(const PsgdLce* a, int* dev_err, cudaStream_t stream) {
   using namespace psgd;
   if (!a || !valid(*a) || !dev_err || a->n < 1 || !a->h || !a->w || !a->target || !a->loss || !a->workspace ||
-      !aligned16(a->workspace) || (a->grads && (!a->dh || !a->dw)))
+      !aligned16(a->workspace) || (a->grads && !a->dh && !a->dw))
     return PSGD_EINVAL;
   if (a->workspace_bytes < psgd_lce_workspace(a)) return PSGD_ESPACE;
   switch (a->dtype) {

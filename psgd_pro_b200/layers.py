@@ -18,6 +18,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from . import _capi
 from ._capi import check
@@ -81,7 +82,7 @@ def _generator(p, seed, offset, x):
         if seed.dtype != torch.int64 or seed.device != x.device or seed.numel() != 2 or not seed.is_contiguous():
             _fail("a seed tensor must hold two contiguous int64 values (seed, offset) on the inputs' device")
         return threshold, scale, 0, 0, seed.data_ptr()
-    return threshold, scale, seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF, None
+    return threshold, scale, int(seed) & 0xFFFFFFFFFFFFFFFF, int(offset) & 0xFFFFFFFFFFFFFFFF, None
 
 
 def _dropout(x, p, seed, offset, residual):
@@ -107,6 +108,7 @@ class _Dropout(torch.autograd.Function):
         return _dropout(x, p, seed, offset, residual)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dx = dropout_grad(dy, *ctx.mask) if ctx.needs_input_grad[0] else None
         return dx, None, None, None, dy if ctx.needs_input_grad[4] else None
@@ -290,6 +292,7 @@ class _ResidualNorm(torch.autograd.Function):
         return out, normed
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_out, d_normed):
         out, y, stats, weight, bias, post_weight, post_bias, gate = ctx.saved_tensors
         if d_out is None and d_normed is None:
@@ -359,7 +362,7 @@ def reset_errors():
     _ERRORS.reset()
 
 
-def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes):
+def _lce(h, w, target, need, grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes):
     code = _elements(h, "h")
     if reduction not in _REDUCTIONS:
         _fail("reduction must be 'none', 'mean' or 'sum'")
@@ -379,7 +382,7 @@ def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduc
             _fail("grad must be fp32 on the inputs' device: a scalar, or one value for each row with reduction 'none'")
         grad = grad.contiguous()
     loss = target.new_empty(target.shape if none else (), dtype=torch.float32)
-    dh, dw = (_new(h), _new(w)) if grads else (None, None)
+    dh, dw = (_new(t) if wanted else None for t, wanted in zip((h, w), need))
     if n == 0:
         for x in (loss, dw):
             if x is not None:
@@ -389,7 +392,7 @@ def _lce(h, w, target, grads, grad, ignore_index, label_smoothing, z_loss, reduc
     err = _ERRORS.get(index)
     s = _capi.Lce(h2.data_ptr(), w2.data_ptr(), t.data_ptr(), _ptr(grad), loss.data_ptr(), _ptr(dh), _ptr(dw), None,
                   ld_h, ld_w, ignore_index, 0, piece_bytes, n, d, v, code,
-                  _REDUCTIONS[reduction], grads, label_smoothing, z_loss)
+                  _REDUCTIONS[reduction], any(need), label_smoothing, z_loss)
     L = _capi.lib()
     size = L.psgd_lce_workspace(ctypes.byref(s))
     if size < 0:
@@ -411,23 +414,24 @@ class _LinearCrossEntropy(torch.autograd.Function):
         ctx.options, ctx.grads = options, None
         ctx.early = options["reduction"] != "none" and h.dtype != torch.float16
         ctx.save_for_backward(h, w, target)
-        loss, *grads = _lce(h, w, target, ctx.early, None, **options)
+        loss, *grads = _lce(h, w, target, ctx.needs_input_grad[:2] if ctx.early else (False, False), None, **options)
         if ctx.early:
             ctx.grads = grads
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
-        need, grads = ctx.needs_input_grad, ctx.grads
+        grads = ctx.grads
         ctx.grads = None  # they are the caller's now: a second pass (retain_graph) forms its own, in the same way
         if grads is None:
             h, w, target = ctx.saved_tensors
-            _, *grads = _lce(h, w, target, True, None if ctx.early else grad, **ctx.options)
+            _, *grads = _lce(h, w, target, ctx.needs_input_grad[:2], None if ctx.early else grad, **ctx.options)
         if ctx.early:
-            for t, used in zip(grads, need):
-                if used and t.numel():
+            for t in grads:
+                if t is not None and t.numel():
                     _launch(t.get_device(), _capi.lib().psgd_lce_scale, t.data_ptr(), _TYPES[t.dtype], t.numel(), grad.data_ptr())
-        return grads[0] if need[0] else None, grads[1] if need[1] else None, None, None
+        return *grads, None, None
 
 
 def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: int = -100, label_smoothing: float = 0.0,
@@ -448,11 +452,11 @@ def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: 
                    piece_bytes=piece_bytes)
     if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
         return _LinearCrossEntropy.apply(h, w, target, options)
-    return _lce(h, w, target, False, None, **options)[0]
+    return _lce(h, w, target, (False, False), None, **options)[0]
 
 
 def linear_cross_entropy_grad(h: Tensor, w: Tensor, target: Tensor, *, grad: Optional[Tensor] = None,
                               ignore_index: int = -100, label_smoothing: float = 0.0, z_loss: float = 0.0,
                               reduction: str = "mean", piece_bytes: int = DEFAULT_PIECE_BYTES):
     """(loss, dh, dw): the loss and the gradients of h and w for the upstream gradient `grad` (fp32; default ones)."""
-    return _lce(h, w, target, True, grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes)
+    return _lce(h, w, target, (True, True), grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes)

@@ -276,6 +276,32 @@ def test_joint_empty_and_nonfinite_rows(cuda):
     assert torch.equal(layers.residual_norm_forward(z, z, post_norm=True, norm="layer")[1], z)  # eps alone
 
 
+def test_joint_dropped_infinities_stay_out(cuda):
+    """y infinite or NaN exactly where dropout drops it: output, gradients and the gate's gradient are those of zeros there."""
+    g = torch.Generator().manual_seed(8)
+    keep = mask((40, 72), 0.3, 6, 2) != 0
+    x, y, gate, up = (rand(g, 40, 72).to(cuda), rand(g, 40, 72), rand(g, 4, 72).to(cuda), rand(g, 40, 72).to(cuda))
+    clean, dirty = (torch.where(keep, y, torch.tensor(v)).to(cuda) for v in (0.0, float("inf")))
+    dirty.view(-1)[(~keep).view(-1).nonzero()[::2, 0].to(cuda)] = float("nan")
+    got = []
+    for v in (clean, dirty):
+        options = dict(gate=gate, dropout_p=0.3, seed=6, offset=2)
+        out, normed, stats = layers.residual_norm_forward(x, v, **options)
+        b = layers.residual_norm_grad(up, up, out, v, stats, **options)
+        got.append((out, normed, b.dx, b.dy, b.dgate))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and all(torch.isfinite(t).all() for t in got[1])
+
+
+def test_second_derivatives_are_refused(cuda):
+    x = torch.randn(4, 8, device=cuda, requires_grad=True)
+    w = torch.randn(5, 8, device=cuda, requires_grad=True)
+    t = torch.zeros(4, dtype=torch.int64, device=cuda)
+    for loss in (layers.residual_norm(x, x)[1].sum(), layers.dropout(x, 0.5, 1).sum(), layers.linear_cross_entropy(x, w, t)):
+        g, = torch.autograd.grad(loss, x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            g.sum().backward()
+
+
 def test_joint_refusals(cuda):
     x, w = torch.ones(4, 16, device=cuda), torch.ones(16, device=cuda)
     f = layers.residual_norm
@@ -383,6 +409,17 @@ def test_loss_autograd_with_upstream_gradients(cuda, dtype, reduction):
     assert rel(loss, want[0]) <= 1e-5
     for x, y, ref in zip(got, again, want[1:]):
         assert rel(x, ref) <= PRODUCT[dtype] and torch.equal(x, y)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_loss_gradients_of_one_input(cuda, reduction):
+    h, w, t = (x.to(cuda) for x in lce_case(300, 72, 500, "bf16", 0.2, cuda))
+    up = torch.ones((), device=cuda) if reduction == "mean" else torch.ones(300, device=cuda)
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    both = torch.autograd.grad(layers.linear_cross_entropy(a, b, t, reduction=reduction), (a, b), up)
+    dh, = torch.autograd.grad(layers.linear_cross_entropy(a, w, t, reduction=reduction), a, up)
+    dw, = torch.autograd.grad(layers.linear_cross_entropy(h, b, t, reduction=reduction), b, up)
+    assert torch.equal(dh, both[0]) and torch.equal(dw, both[1])
 
 
 def test_loss_against_differences(cuda):
