@@ -434,24 +434,29 @@ PSGD_DEVI void logits_row(const LceProblem& p, const LceShape& sh, const LceLogi
     if (here) g.target_logit[row] = x;
   }
   float linear = 0.f;
-  if (g.linear)
+  if (g.linear) {
+    float part[4] = {};
 #pragma unroll
-    for (int k = 0; k < COLS; ++k) linear += k < width ? v[k] : 0.f;
+    for (int k = 0; k < COLS; ++k) part[k & 3] += k < width ? v[k] : 0.f;
+    linear = (part[0] + part[1]) + (part[2] + part[3]);
+  }
   if (width < COLS)
 #pragma unroll
     for (int k = 0; k < COLS; ++k)
       if (k >= width) v[k] = -INFINITY;
-  float top = v[0];
+  // (four chains each for the maximum and the sum: with two warps to a scheduler their latency is what a tile costs here)
+  float tops[4] = {v[0], v[1], v[2], v[3]}, sums[4] = {};
 #pragma unroll
-  for (int k = 1; k < COLS; ++k) top = fmaxf(top, v[k]);
+  for (int k = 4; k < COLS; ++k) tops[k & 3] = fmaxf(tops[k & 3], v[k]);
+  const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const float ref = top == -INFINITY || top != top ? 0.f : top;
-  float sum = 0.f;
 #pragma unroll
   for (int k = 0; k < COLS; ++k) {
     // 16 bits: 2^15 exp(l - m), the factor added to the exponent, whose rounding is 2^-21 at most
     v[k] = WIDE ? expf(v[k] - ref) : exp2_fast(fmaf(v[k] - ref, LOG2E, 15.f));
-    sum += v[k];
+    sums[k & 3] += v[k];
   }
+  float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
   if (!WIDE) sum *= 1.f / L_KEEP_SCALE;
   if (g.kept && live) {
     KT* to = reinterpret_cast<KT*>(g.kept) + row * g.ld_kept + n0;
@@ -1108,7 +1113,13 @@ int product(const LceArgs& args, cudaStream_t stream) {
     cudaGetLastError();
     return PSGD_ELAUNCH;
   }
-  return pdl_launch(k, dim3(psgd_num_sms() / 2 * 2), dim3(L_THREADS), C::SMEM, stream, args);
+  long long units = 0;  // (at most; the counted rows decide)
+  for (int i = 0; i < args.nproblems; ++i) {
+    const LceProblem& p = args.p[i];
+    units += (long long)((p.M + LM - 1) / LM) * ((p.N + BN - 1) / BN) * p.splits;
+  }
+  const long long clusters = psgd_num_sms() / 2;
+  return pdl_launch(k, dim3(2 * (int)(units < clusters ? units : clusters)), dim3(L_THREADS), C::SMEM, stream, args);
 }
 template <typename OP, typename OUT, int LIMBS, bool LOGITS>
 int product_bn(int bn, const LceArgs& args, cudaStream_t stream) {
