@@ -3,6 +3,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <atomic>
+
 #include "common.cuh"
 #include "philox.cuh"
 #include "psgd_b200.h"
@@ -143,6 +145,21 @@ int pdl_launch(void (*kernel)(P...), dim3 grid, dim3 block, int smem, cudaStream
   if (cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...) == cudaSuccess) return PSGD_OK;
   cudaGetLastError();  // else it would be taken for a later launch's
   return PSGD_ELAUNCH;
+}
+
+// Dynamic shared memory beyond what a kernel has without asking; `done` remembers the devices where it was granted, one
+// bit each. A refusal is cleared: it would be taken for a later launch's.
+template <typename K>
+int allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev > 63) return PSGD_ELAUNCH;
+  if ((done.load(std::memory_order_relaxed) >> dev) & 1) return PSGD_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    cudaGetLastError();
+    return PSGD_ELAUNCH;
+  }
+  done.fetch_or(1ull << dev, std::memory_order_relaxed);
+  return PSGD_OK;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }

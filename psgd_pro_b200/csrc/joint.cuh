@@ -17,8 +17,9 @@
 namespace psgd {
 
 constexpr int JOINT_MAX_D = PSGD_JOINT_MAX_D;
+// Dynamic shared memory that needs no asking (48 KB with the kernels' static one), and what is asked for otherwise.
+constexpr int JOINT_SMEM_FREE = 40 * 1024, JOINT_SMEM_MOST = 224 * 1024;
 constexpr int JOINT_MAX_GROUPS = 8;  // of a block, where a group has more than a warp
-constexpr int JOINT_MAX_THREADS = 512;
 // Kernels by the elements that a thread has of a row and the threads of a block: 8 (rows of up to 256 elements, a warp
 // each), 16 (up to 2048 elements: 128 threads; up to 4096: 256; beyond: 512, whose registers do not hold all the sums).
 enum JointWidth { W8 = 0, W16 = 1, W16_256 = 2, W16_512 = 3 };
@@ -41,17 +42,6 @@ int joint_forward_f16(const PsgdJoint& j, const JointPlan& p, cudaStream_t strea
 int joint_backward_f32(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
 int joint_backward_bf16(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
 int joint_backward_f16(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream);
-
-// Dynamic shared memory beyond the 48 KB that dynamic and static shared memory have without asking. A refusal is cleared:
-// it would be taken for the next launch's.
-template <typename K>
-int joint_allow_smem(K kernel, int smem) {
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-    cudaGetLastError();
-    return PSGD_ELAUNCH;
-  }
-  return PSGD_OK;
-}
 
 // ---- two fp32 values in one register pair -----------------------------------------------------------------------------
 struct F2 {
@@ -1185,20 +1175,31 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
 template <typename T, bool VEC, int W, int F>
 int joint_forward_launch(const PsgdJoint& j, const JointPlan& p, cudaStream_t stream) {
   auto k = joint_forward_kernel<T, VEC, W, F>;
-  if (int rc = joint_allow_smem(k, p.smem)) return rc;
+  static std::atomic<unsigned long long> done{0};
+  if (p.smem > JOINT_SMEM_FREE)
+    if (int rc = allow_smem(k, JOINT_SMEM_MOST, done)) return rc;
   k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p);
   return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
 }
 template <typename K>
-int joint_backward_start(K k, const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
-  if (int rc = joint_allow_smem(k, p.smem)) return rc;
+int joint_backward_start(K k, std::atomic<unsigned long long>& done, const PsgdJoint& j, const JointPlan& p, float* part,
+                         cudaStream_t stream) {
+  if (p.smem > JOINT_SMEM_FREE)
+    if (int rc = allow_smem(k, JOINT_SMEM_MOST, done)) return rc;
   k<<<p.blocks, dim3(p.tpr, p.groups), p.smem, stream>>>(j, p, part);
   return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
 }
 
 template <typename T, bool VEC, int W, int F>
 int joint_backward_launch(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
-  return joint_backward_start(joint_backward_kernel<T, VEC, W, F>, j, p, part, stream);
+  static std::atomic<unsigned long long> done{0};
+  return joint_backward_start(joint_backward_kernel<T, VEC, W, F>, done, j, p, part, stream);
+}
+
+template <typename T, bool VEC, bool DIRECT>
+int joint_backward_wide(const PsgdJoint& j, const JointPlan& p, float* part, cudaStream_t stream) {
+  static std::atomic<unsigned long long> done{0};
+  return joint_backward_start(joint_backward_wide_kernel<T, VEC, DIRECT>, done, j, p, part, stream);
 }
 
 inline int joint_flags(const PsgdJoint& j, const JointPlan& p) {
@@ -1258,10 +1259,8 @@ int joint_backward_of(const PsgdJoint& j, const JointPlan& p, float* part, cudaS
                    : joint_backward_launch<T, false, W16_256, F_RUNTIME>(j, p, part, stream);
     default:
       if (f & F_DIRECT)
-        return p.vec ? joint_backward_start(joint_backward_wide_kernel<T, true, true>, j, p, part, stream)
-                     : joint_backward_start(joint_backward_wide_kernel<T, false, true>, j, p, part, stream);
-      return p.vec ? joint_backward_start(joint_backward_wide_kernel<T, true, false>, j, p, part, stream)
-                   : joint_backward_start(joint_backward_wide_kernel<T, false, false>, j, p, part, stream);
+        return p.vec ? joint_backward_wide<T, true, true>(j, p, part, stream) : joint_backward_wide<T, false, true>(j, p, part, stream);
+      return p.vec ? joint_backward_wide<T, true, false>(j, p, part, stream) : joint_backward_wide<T, false, false>(j, p, part, stream);
   }
 }
 

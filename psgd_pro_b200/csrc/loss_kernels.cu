@@ -1109,10 +1109,8 @@ template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
 int product(const LceArgs& args, cudaStream_t stream) {
   using C = LceCfg<LIMBS, BN, LOGITS>;
   auto k = lce_product_kernel<OP, OUT, LIMBS, BN, LOGITS>;
-  if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
-    cudaGetLastError();
-    return PSGD_ELAUNCH;
-  }
+  static std::atomic<unsigned long long> done{0};
+  if (int rc = allow_smem(k, C::SMEM, done)) return rc;
   long long units = 0;  // (at most; the counted rows decide)
   for (int i = 0; i < args.nproblems; ++i) {
     const LceProblem& p = args.p[i];

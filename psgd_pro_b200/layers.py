@@ -363,36 +363,38 @@ def reset_errors():
 
 
 def _lce(h, w, target, need, grad, ignore_index, label_smoothing, z_loss, reduction, piece_bytes):
-    code = _elements(h, "h")
-    if reduction not in _REDUCTIONS:
+    dtype, index, shape = h.dtype, h.get_device(), h.shape
+    code, kind = _TYPES.get(dtype), _REDUCTIONS.get(reduction)
+    if code is None or index < 0:
+        _fail("h must be an fp32, bf16 or fp16 CUDA tensor")
+    if kind is None:
         _fail("reduction must be 'none', 'mean' or 'sum'")
-    if w.dim() != 2 or h.dim() < 1 or h.shape[-1] != w.shape[1] or w.shape[0] < 1 or w.shape[1] < 1:
+    if w.dim() != 2 or not shape or shape[-1] != w.shape[1] or w.numel() == 0:
         _fail("h (..., d) and w (v, d) must share d")
-    _like(w, h, "w")
-    if target.shape != h.shape[:-1] or target.dtype != torch.int64 or not target.is_cuda or target.get_device() != h.get_device():
+    if w.dtype != dtype or w.get_device() != index:
+        _fail("w must have the type and device of h")
+    if target.shape != shape[:-1] or target.dtype != torch.int64 or target.get_device() != index:
         _fail("target must hold one int64 value for each row of h, on its device")
     if not 0.0 <= label_smoothing <= 1.0:
         _fail("label_smoothing must lie in [0, 1]")
     v, d = w.shape
-    (h2, ld_h), (w2, ld_w), t = _rows(h, d), _rows(w, d), target.contiguous()
-    n = h2.numel() // d
-    none = reduction == "none"
     if grad is not None:
-        if grad.dtype != torch.float32 or grad.get_device() != h.get_device() or grad.shape != (target.shape if none else ()):
+        if grad.dtype != torch.float32 or grad.get_device() != index or grad.shape != (() if kind else target.shape):
             _fail("grad must be fp32 on the inputs' device: a scalar, or one value for each row with reduction 'none'")
         grad = grad.contiguous()
-    loss = target.new_empty(target.shape if none else (), dtype=torch.float32)
-    dh, dw = (_new(t) if wanted else None for t, wanted in zip((h, w), need))
+    (h, ld_h), (w, ld_w), target = _rows(h, d), _rows(w, d), target.contiguous()
+    n = target.numel()
+    loss = target.new_empty(() if kind else target.shape, dtype=torch.float32)
+    dh = h.new_empty(shape) if need[0] else None
+    dw = torch.empty_like(w) if need[1] and ld_w == d else w.new_empty((v, d)) if need[1] else None
     if n == 0:
         for x in (loss, dw):
             if x is not None:
                 x.zero_()
         return loss, dh, dw
-    index = h.get_device()
     err = _ERRORS.get(index)
-    s = _capi.Lce(h2.data_ptr(), w2.data_ptr(), t.data_ptr(), _ptr(grad), loss.data_ptr(), _ptr(dh), _ptr(dw), None,
-                  ld_h, ld_w, ignore_index, 0, piece_bytes, n, d, v, code,
-                  _REDUCTIONS[reduction], any(need), label_smoothing, z_loss)
+    s = _capi.Lce(h.data_ptr(), w.data_ptr(), target.data_ptr(), _ptr(grad), loss.data_ptr(), _ptr(dh), _ptr(dw), None, ld_h,
+                  ld_w, ignore_index, 0, piece_bytes, n, d, v, code, kind, need[0] or need[1], label_smoothing, z_loss)
     L = _capi.lib()
     size = L.psgd_lce_workspace(ctypes.byref(s))
     if size < 0:
