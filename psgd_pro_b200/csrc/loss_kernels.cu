@@ -15,6 +15,8 @@
 
 #include <float.h>
 
+#include <type_traits>
+
 namespace psgd {
 namespace {
 
@@ -158,8 +160,8 @@ PSGD_DEVI void limbs3(float x, float* l) {
   l[2] = r - l[1];
 }
 
-// Tensor-core operands from matrices: row i of h to its number among the counted rows, row i of w to row i, itself or its
-// bf16 limbs `plane` elements apart. Rows that do not count zero their row of dh instead. Blocks beyond the rows zero the operand's rows from
+// Tensor-core operands from matrices: row i of h to its number among the counted rows, row i of w to row i, itself or (WIDE)
+// its bf16 limbs `plane` elements apart. Rows that do not count zero their row of dh instead. Blocks beyond the rows zero the operand's rows from
 // the count to the next multiple of 64, which a reduction over rows reads.
 template <typename T>
 struct LceStage {
@@ -172,7 +174,7 @@ struct LceStage {
 // INLINE: there was no plan launch; every block counts the rows before its own (up to PLAN_INLINE of them: the reads are
 // shorter than a launch), and the last one of h finishes the plan.
 constexpr int PLAN_INLINE = 2048;
-template <typename T, bool VEC, bool INLINE>
+template <typename T, bool WIDE, bool VEC, bool INLINE>
 __global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, const LceStage<T> w, int d, const LcePlan plan) {
   constexpr int V = VEC ? 8 : 1;
   __shared__ int before[8];
@@ -236,7 +238,7 @@ __global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, con
   const T* src = a.src + (there ? i * a.ld : 0);
   uint16_t* out = a.out + r * a.ld_out;
   for (int e = lane * V; e < d; e += 32 * V) {
-    if constexpr (sizeof(T) == 2) {
+    if constexpr (!WIDE) {
       T* to = reinterpret_cast<T*>(out) + e;
       if constexpr (VEC) {
         *reinterpret_cast<uint4*>(to) = there ? *reinterpret_cast<const uint4*>(src + e) : make_uint4(0, 0, 0, 0);
@@ -1030,9 +1032,16 @@ struct Layout {
   size_t state, rank, row_of, row_target, loss_rows, target_logit, stats, linear, h, w, kept, g, part, part_w, acc, bytes;
 };
 
+// Whether the operands are three bf16 limbs: fp32 ones, and 16-bit ones of up to 2^20 products, where g, whose one rounding
+// to 16 bits is as large as that of the gradients themselves, does not average out over long sums. Limbs cost such a call 6
+// us on the GPU (7 x 32 x 85: 22.6 us against 16.4), less than its host code takes (28 us); from 2^24 on 10 us and more.
+bool wide_operands(const PsgdLce& a) {
+  return a.dtype == PSGD_F32 || (double)a.n * a.v * a.d <= (double)(1 << 20);
+}
+
 Layout layout(const PsgdLce& a) {
   Layout l = {};
-  const bool wide = a.dtype == PSGD_F32;
+  const bool wide = wide_operands(a);
   auto up = [](long long x, long long m) { return (x + m - 1) / m * m; };
   l.limbs = wide ? L_LIMBS : 1;
   // Narrow tiles (128 columns) where wide ones would not go twice around the clusters; fp32 always (three limbs a stage).
@@ -1094,7 +1103,7 @@ Layout layout(const PsgdLce& a) {
     l.g = wide ? take(2ull * l.limbs * l.g_plane) : l.kept;
     l.part = take(l.splits > 1 ? 4ull * l.splits * piece * l.ld_part : 0);
     l.part_w = take(l.splits_w > 1 ? 4ull * l.splits_w * a.v * l.ld_part : 0);
-    l.acc = take(l.pieces > 1 && !wide ? 4ull * a.v * l.ld_part : 0);
+    l.acc = take(l.pieces > 1 && a.dtype != PSGD_F32 ? 4ull * a.v * l.ld_part : 0);
   }
   l.bytes = at;
   return l;
@@ -1126,11 +1135,13 @@ int product_bn(int bn, const LceArgs& args, cudaStream_t stream) {
   return product<OP, OUT, LIMBS, 128, LOGITS>(args, stream);
 }
 
-// T: type of h, w and the gradients; OP: operand type of the tensor cores; KT: type of the kept exponentials.
-template <typename T, typename OP, typename KT>
+// T: type of h, w and the gradients. OP: operand type of the tensor cores; KT: type of the kept exponentials.
+template <typename T, bool WIDE>
 int run(const PsgdLce& a, int* err, cudaStream_t stream) {
+  using OP = std::conditional_t<WIDE, __nv_bfloat16, T>;
+  using KT = std::conditional_t<WIDE, float, __half>;
   constexpr bool half = is_half<OP>();
-  constexpr int LIMBS = sizeof(T) == 4 ? L_LIMBS : 1;
+  constexpr int LIMBS = WIDE ? L_LIMBS : 1;
   const Layout l = layout(a);
   uint8_t* ws = reinterpret_cast<uint8_t*>(a.workspace);
   LceState* state = reinterpret_cast<LceState*>(ws + l.state);
@@ -1152,13 +1163,13 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
                    (!l.stage_w || (aligned16(a.w) && a.ld_w * sizeof(T) % 16 == 0));
   const dim3 stage_grid(sh.blocks + sw.blocks);
   if (a.n <= PLAN_INLINE) {
-    auto k = vec ? lce_stage_kernel<T, true, true> : lce_stage_kernel<T, false, true>;
+    auto k = vec ? lce_stage_kernel<T, WIDE, true, true> : lce_stage_kernel<T, WIDE, false, true>;
     k<<<stage_grid, 256, 0, stream>>>(sh, sw, a.d, plan);
     if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
   } else {
     lce_plan_kernel<<<1, 1024, 0, stream>>>(plan);
     if (cudaGetLastError() != cudaSuccess) return PSGD_ELAUNCH;
-    if (int rc = pdl_launch(vec ? lce_stage_kernel<T, true, false> : lce_stage_kernel<T, false, false>, stage_grid, dim3(256),
+    if (int rc = pdl_launch(vec ? lce_stage_kernel<T, WIDE, true, false> : lce_stage_kernel<T, WIDE, false, false>, stage_grid, dim3(256),
                             0, stream, sh, sw, a.d, plan))
       return rc;
   }
@@ -1270,10 +1281,11 @@ extern "C" int psgd_lce(const PsgdLce* a, int* dev_err, cudaStream_t stream) {
       !aligned16(a->workspace) || (a->grads && !a->dh && !a->dw))
     return PSGD_EINVAL;
   if (a->workspace_bytes < psgd_lce_workspace(a)) return PSGD_ESPACE;
+  const bool wide = wide_operands(*a);
   switch (a->dtype) {
-    case PSGD_F32: return run<float, __nv_bfloat16, float>(*a, dev_err, stream);
-    case PSGD_BF16: return run<__nv_bfloat16, __nv_bfloat16, __half>(*a, dev_err, stream);
-    default: return run<__half, __half, __half>(*a, dev_err, stream);
+    case PSGD_F32: return run<float, true>(*a, dev_err, stream);
+    case PSGD_BF16: return wide ? run<__nv_bfloat16, true>(*a, dev_err, stream) : run<__nv_bfloat16, false>(*a, dev_err, stream);
+    default: return wide ? run<__half, true>(*a, dev_err, stream) : run<__half, false>(*a, dev_err, stream);
   }
 }
 
