@@ -129,7 +129,7 @@ JointPlan plan_backward(const PsgdJoint& j) {
   for (int a = 0; a < 5; ++a) p.slot[a] = there[a] ? p.slots++ : -1;
   // Rows ahead: two for 16-bit types, one for fp32, as far as shared memory goes.
   const int threads = p.tpr * p.groups, columns = threads * p.nv * 64;
-  const int arrays = p.wide == W16_512 || j.post || j.gate ? 4 : 3;
+  const int arrays = (f & F_RUNTIME) || j.post || j.gate ? 4 : 3;  // (as the kernel compiled for f has)
   const int room = 220 * 1024 / per_sm - columns;
   p.stages = j.dtype == PSGD_F32 ? 2 : 3;
   while (p.stages > 1 && ring_bytes(p, arrays, j.dtype) > room) --p.stages;

@@ -251,6 +251,23 @@ def test_joint_strides_views_and_missing_gradients(cuda):
                layers.residual_norm_grad(zero, d, out, y, stats).dx) == 0.0
 
 
+@pytest.mark.parametrize("d", [2056, 2057, 3001, 4095, 4100])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_joint_backward_of_long_rows_without_norm_or_gate(cuda, d, dtype):
+    """Rows of over 2048 elements, aligned or not, where neither y nor a gate is read."""
+    g = torch.Generator().manual_seed(d)
+    x, y, up, un = (rand(g, 7, d, dtype=TYPES[dtype]) for _ in range(4))
+    w = rand(g, d, std=0.2, mean=1.0)
+    out, _, stats = layers.residual_norm_forward(x.to(cuda), y.to(cuda), weight=w.to(cuda))
+    got = layers.residual_norm_grad(up.to(cuda), un.to(cuda), out, y.to(cuda), stats, weight=w.to(cuda))
+    o, w64 = out.double().cpu().requires_grad_(), w.double().requires_grad_()
+    n = o / (o.pow(2).mean(-1, keepdim=True) + 1e-6).sqrt() * w64
+    do, dw = torch.autograd.grad(n, (o, w64), un.double())
+    slack = 1.0 if dtype == "fp32" else 2.0
+    assert rel(got.dx, do + up.double()) <= ONE[dtype] * slack and rel(got.dy, do + up.double()) <= ONE[dtype] * slack
+    assert rel(got.dweight, dw) <= max(ONE[dtype], 1e-5) * slack
+
+
 @pytest.mark.parametrize("shape", [(4, 1, 24), (4, 6, 24), (1, 1, 24)])
 def test_joint_gate_shapes(cuda, shape):
     g = torch.Generator().manual_seed(1)
