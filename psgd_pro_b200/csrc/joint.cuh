@@ -228,11 +228,12 @@ struct Place {
       }
     }
   }
-  // A parameter vector of fp32 or of T, `otherwise` where there is none.
+  // A parameter vector of fp32 or of T, `otherwise` where it is missing; zero beyond d in any case (the sums over a row rely
+  // on it).
   PSGD_DEVI void param(const void* p, int dtype, float otherwise, int i, F2* v) const {
     if (!p) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = f2(otherwise);
+      for (int k = 0; k < 4; ++k) v[k] = only(f2(otherwise), i, k);
     } else if (dtype == PSGD_F32) {
       load(reinterpret_cast<const float*>(p), i, v);
     } else {

@@ -251,6 +251,27 @@ def test_joint_strides_views_and_missing_gradients(cuda):
                layers.residual_norm_grad(zero, d, out, y, stats).dx) == 0.0
 
 
+@pytest.mark.parametrize("d", [6, 40, 200, 333, 938, 2057, 4104])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+def test_joint_without_some_parameters(cuda, d, norm):
+    """Missing weights count as ones and missing biases as zeros, wherever a row ends inside a warp."""
+    g = torch.Generator().manual_seed(d)
+    x, y, up = (rand(g, 9, d, mean=0.3) for _ in range(3))
+    names = ["weight", "post_weight"] + (["bias", "post_bias"] if norm == "layer" else [])
+    for there in range(1 << len(names)):
+        on = {k: rand(g, d, std=0.2, mean=1.0) for i, k in enumerate(names) if there >> i & 1}
+        leaves = {k: v.to(cuda).requires_grad_() for k, v in dict(on, x=x, y=y).items()}
+        out, normed = layers.residual_norm(norm=norm, post_norm=True, scale=0.5, eps=1e-5, **leaves)
+        wide = {k: v.double().requires_grad_() for k, v in dict(on, x=x, y=y).items()}
+        ref = joint_ref(wide["x"], wide["y"], norm, True, *(wide.get(k) for k in ("weight", "bias", "post_weight", "post_bias")),
+                        None, 0.5, 1e-5, None)
+        assert rel(out, ref[0]) <= 2e-6 and rel(normed, ref[1]) <= 2e-6, on.keys()
+        got = torch.autograd.grad(normed, list(leaves.values()), up.to(cuda))
+        want = torch.autograd.grad(ref[1], list(wide.values()), up.double())
+        for k, a, b in zip(leaves, got, want):
+            assert rel(a, b) <= 2e-5, (k, on.keys())
+
+
 @pytest.mark.parametrize("d", [2056, 2057, 3001, 4095, 4100])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_joint_backward_of_long_rows_without_norm_or_gate(cuda, d, dtype):
