@@ -471,7 +471,7 @@ int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cu
  * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type (either may be
  * NULL), for the upstream gradient grad (n values for _NONE, one otherwise; NULL: ones). fp16: 1 + 2 z_loss lse stays
  * below 255. Tokens are taken in pieces of at most piece_bytes of
- * kept exponentials (and at least 128 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
+ * kept exponentials (and at least 256 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
  * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong. */
 #define PSGD_REDUCE_NONE 0
 #define PSGD_REDUCE_MEAN 1

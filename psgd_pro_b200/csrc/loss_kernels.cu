@@ -906,10 +906,12 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   }
   sum = sum_all(sum);
   if (a.linear) linear = sum_all(linear);
-  const float lse = ref + logf(sum), lt = a.target_logit[row];
+  // lse - l_t from differences with the maximum: lse itself is rounded at the size of the logits, and a row that is all but
+  // certain of its target has only the difference left (of its loss, and of 1 - p).
+  const float log_sum = logf(sum), lse = ref + log_sum, lt = a.target_logit[row], short_of = log_sum - (lt - ref);
   const int target = a.row_target[a.row0 + row];
   if (t == 0 && blockIdx.y == 0) {
-    float loss = a.smoothing == 0.f ? lse - lt : (1.f - a.smoothing) * (lse - lt) + a.smoothing * (lse - linear / (float)a.v);
+    float loss = a.smoothing == 0.f ? short_of : (1.f - a.smoothing) * short_of + a.smoothing * (lse - linear / (float)a.v);
     if (a.z != 0.f) loss += a.z * lse * lse;
     if (a.none) a.loss[a.row_of[a.row0 + row]] = loss;
     else a.loss_rows[a.row0 + row] = loss;
@@ -921,9 +923,9 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   const float pull = 1.f + 2.f * a.z * lse, uniform = a.smoothing / (float)a.v;
   const float scale = sizeof(KT) == 4 ? 1.f : 1.f / L_KEEP_SCALE;
   // the target's element from its fp32 logit: p - 1 without cancellation
-  const float at_target = c * (expm1f(lt - lse) + (pull - 1.f) * expf(lt - lse) + a.smoothing - uniform);
+  const float at_target = c * (expm1f(-short_of) + (pull - 1.f) * expf(-short_of) + a.smoothing - uniform), inverse = 1.f / sum;
   for (int i = v0 + t; i < v1; i += STEP) {
-    const float f = expf(st[(i * 8) >> shift].x - lse) * scale * pull;
+    const float f = expf(st[(i * 8) >> shift].x - ref) * inverse * scale * pull;
     float g[8];
     load_vec<KT, 8>(kept + i * 8, g);
 #pragma unroll

@@ -449,7 +449,7 @@ def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: 
     Under autograd a scalar loss (mean, sum) of bf16 or fp32 inputs that require gradients forms them at once and holds
     them for the backward pass; otherwise the backward pass forms loss and gradients again. Evaluation belongs under
     torch.no_grad(). piece_bytes bounds what is kept of the vocabulary's probabilities at a time (16 bits each; fp32: 80
-    bits); tokens are taken in pieces of that size (of 128 at least)."""
+    bits); tokens are taken in pieces of that size (of 256 at least)."""
     options = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, z_loss=z_loss, reduction=reduction,
                    piece_bytes=piece_bytes)
     if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):

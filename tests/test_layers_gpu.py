@@ -426,7 +426,7 @@ def test_loss_in_pieces_matches_the_whole(cuda, dtype):
     h, w, t = lce_case(700, 136, 1111, dtype, 0.25, cuda)
     on = [x.to(cuda) for x in (h, w, t)]
     whole = layers.linear_cross_entropy_grad(*on)
-    pieces = layers.linear_cross_entropy_grad(*on, piece_bytes=1)  # 128 tokens each; the last ones hold no counted row
+    pieces = layers.linear_cross_entropy_grad(*on, piece_bytes=1)  # 256 tokens each; the last one holds no counted row
     want = lce_ref(h, w, t)
     assert abs(whole[0].item() - pieces[0].item()) <= 1e-6 * abs(whole[0].item())
     assert torch.equal(whole[1], pieces[1]) or rel(pieces[1], want[1]) <= PRODUCT[dtype]
@@ -514,6 +514,26 @@ def test_loss_extreme_logits(cuda):
     _, dh, dw = layers.linear_cross_entropy_grad(h, w, t)
     ref = lce_ref(h, w, t.cpu())
     assert rel(dh, ref[1]) <= 1e-5 and rel(dw, ref[2]) <= 1e-5
+
+
+def test_loss_of_certain_rows(cuda):
+    """Targets ahead by 7 to 12: losses of 3e-2 down to 2e-4 at logits of about 34, whose fp32 rounding (of their
+    log-normaliser) is 2e-6, a hundredth of the smallest loss. Differences with the maximum are exact here (the logits
+    are multiples of 2^-10), so loss and 1 - p are right to the rounding of sums of 1 and small numbers, 6e-8 an addition and 16
+    additions at most: 5e-3 of the smallest."""
+    v = 50
+    h = torch.eye(6, 16, device=cuda)
+    ahead = torch.tensor([7.0, 8.0, 9.0, 10.0, 11.0, 12.0])
+    w = torch.zeros(v, 16)
+    w[:, :6] = 21.5 + (torch.randint(0, 1024, (v, 6), generator=torch.Generator().manual_seed(0)) / 1024)
+    for k in range(6):
+        w[k, k] = w[:, k].max() + ahead[k]
+    t = torch.arange(6)
+    rows = layers.linear_cross_entropy(h, w.to(cuda), t.to(cuda), reduction="none").double().cpu()
+    want = lce_ref(h, w, t, reduction="none")
+    assert ((rows - want[0]).abs() / want[0]).max().item() <= 5e-3
+    _, dh, _ = layers.linear_cross_entropy_grad(h, w.to(cuda), t.to(cuda), reduction="none")
+    assert ((dh.double().cpu() - want[1]).norm(dim=1) / want[1].norm(dim=1)).max().item() <= 5e-3
 
 
 def test_loss_strides_shapes_and_alignment(cuda):
