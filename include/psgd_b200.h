@@ -424,7 +424,7 @@ int psgd_apply_noalloc(void* param, int param_bf16, const float* pg, long long n
 /* Dropout with a counter-based mask: out = [residual +] (kept ? x * scale : 0) over n elements. Element i is kept when
  * 16-bit field i % 8 (low halves first) of the Philox4x32-10 output for counter (i / 8, offset), each as two 32-bit words,
  * and key seed is at least threshold (= round(65536 p), at most 65536). rng: two values (seed, offset) in device memory
- * instead of the two fields, or NULL. out may be x or residual. */
+ * instead of the two fields, or NULL. out overlaps neither x nor residual. */
 typedef struct PsgdDropout {
   const void* x; const void* residual; void* out;
   long long n;
