@@ -172,6 +172,12 @@ PSGD_DEVI void mbar_arrive_cluster_relaxed(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// Arrive on a barrier of either CTA of the cluster and add to the bytes it expects, without ordering (a pure signal).
+PSGD_DEVI void mbar_arrive_expect_tx_cluster_relaxed(uint32_t bar_cluster, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar_cluster), "r"(bytes)
+               : "memory");
+}
+
 // 2-D TMA tile load into this CTA's shared memory whose completion is counted on a barrier of either CTA of the
 // pair (the leader's, for the pair MMA). No multicast.
 PSGD_DEVI void tma_load_2d_pair(void* smem_dst, const CUtensorMap* tmap, uint32_t bar_cluster, int x, int y) {

@@ -556,9 +556,9 @@ PSGD_DEVI void add_columns(uint32_t at, float* v) {
 // B, the leader (rank 0) issues M = 256 products that read both CTAs' shared memory, and each CTA's TMEM receives its 128
 // rows. Against one-CTA tiles of 128 x 256 this takes a third less through L2 and shared memory for a product.
 //   warp 0      copies; warp 1 (leader) products; warps 4..11: TMEM lanes 32 (w % 4)..., half of the columns each.
-// Handshakes (waits bounded): full[s] at the leader counts both CTAs' copies of stage s, go[s] tells the peer that the
-// leader has armed it, empty[s] frees it (the products' commit, in both CTAs), tfull / tempty hand the two accumulators
-// over. An accumulator takes `chunk` blocks of K; the epilogue adds the chunks in registers and hands the accumulator
+// Handshakes (waits bounded): full[s] at the leader takes an arrival of each CTA with the bytes that it copies to stage s
+// (the phase cannot end before both have told theirs, so neither waits for the other), empty[s] frees it (the products'
+// commit, in both CTAs), tfull / tempty hand the two accumulators over. An accumulator takes `chunk` blocks of K; the epilogue adds the chunks in registers and hands the accumulator
 // back at once: the tensor cores' sums truncate (a bias of about 1.1e-9 a product, measured), so sums that are to be
 // right to fp32 stay short there, and the last step of a tile, from registers, never holds the tensor cores up.
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
@@ -570,8 +570,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + S * C::STAGE);
   uint64_t* empty = full + S;
-  uint64_t* go = empty + S;
-  uint64_t* tfull = go + S;
+  uint64_t* tfull = empty + S;
   uint64_t* tempty = tfull + 2;
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -581,9 +580,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
-      mbar_init(&go[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull[a], 1);
@@ -622,7 +620,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     if (warp == 0 && lane == 0) {
       // ---------------- copies (both CTAs) ----------------
       int s = 0;
-      uint32_t ph = 0, rounds = 0;  // rounds that the leader armed, landed before it leaves on abort
+      uint32_t ph = 0, rounds = 0;  // rounds that this CTA armed; they land before the leader leaves on abort
       int which, index;
       for (int k = 0; deal.get(k, which, index) && !*abort; ++k) {
         const LceProblem& p = args.p[which];
@@ -631,14 +629,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
         for (int kb = u.k0; kb < u.k1; kb += C::KS) {
           const int subs = min(C::KS, u.k1 - kb);
           if (!mbar_wait_for(&empty[s], ph ^ 1, abort, args.wait_ns)) break;
-          if (rank == 0) {
-            mbar_arrive_expect_tx(&full[s], 2u * C::BLOCK * (uint32_t)subs);
-            ++rounds;
-            mbar_arrive_cluster_relaxed(mapa_shared(&go[s], 1));
-          } else if (!mbar_wait_for(&go[s], ph, abort, args.wait_ns)) {
-            break;
-          }
           const uint32_t fb = mapa_shared(&full[s], 0);
+          mbar_arrive_expect_tx_cluster_relaxed(fb, C::BLOCK * (uint32_t)subs);
+          ++rounds;
           for (int j = 0; j < subs; ++j) {
             const int x = (kb + j) * LK;
 #pragma unroll
