@@ -913,10 +913,10 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   const int shift = a.stat == 64 ? 6 : 7;
   constexpr float unit = is_half<GT>() ? L_HALF_SCALE : 1.f;
   const float c = (a.grad ? a.grad[a.row_of[a.row0 + row]] / state->row_unit : 1.f) * unit;
-  const float pull = 1.f + 2.f * a.z * lse, uniform = a.smoothing / (float)a.v;
+  const float more = 2.f * a.z * lse, pull = 1.f + more, uniform = a.smoothing / (float)a.v;
   const float scale = sizeof(KT) == 4 ? 1.f : 1.f / L_KEEP_SCALE;
   // the target's element from its fp32 logit: p - 1 without cancellation
-  const float at_target = c * (expm1f(-short_of) + (pull - 1.f) * expf(-short_of) + a.smoothing - uniform), inverse = 1.f / sum;
+  const float at_target = c * (expm1f(-short_of) + more * expf(-short_of) + (a.smoothing - uniform)), inverse = 1.f / sum;
   for (int i = v0 + t; i < v1; i += STEP) {
     const float f = expf(st[(i * 8) >> shift].x - ref) * inverse * scale * pull;
     float g[8];

@@ -516,6 +516,16 @@ def test_loss_extreme_logits(cuda):
     assert rel(dh, ref[1]) <= 1e-5 and rel(dw, ref[2]) <= 1e-5
 
 
+def test_loss_penalty_alone(cuda):
+    """One class: p is one and only the log-normaliser's penalty is left, 2 z lse, with z lse from 1e-5 on (in 1 + 2 z lse that
+    would be right to 1e-7 / 2e-5 only)."""
+    g = torch.Generator().manual_seed(4)
+    h, w, t = rand(g, 40, 64, std=0.1), rand(g, 1, 64), torch.zeros(40, dtype=torch.int64)
+    _, dh, dw = layers.linear_cross_entropy_grad(h.to(cuda), w.to(cuda), t.to(cuda), z_loss=1e-5)
+    want = lce_ref(h, w, t, 0.0, 1e-5)
+    assert rel(dh, want[1]) <= 1e-5 and rel(dw, want[2]) <= 1e-5
+
+
 def test_loss_of_certain_rows(cuda):
     """Targets ahead by 7 to 12: losses of 3e-2 down to 2e-4 at logits of about 34, whose fp32 rounding (of their
     log-normaliser) is 2e-6, a hundredth of the smallest loss. Differences with the maximum are exact here (the logits
