@@ -14,9 +14,9 @@
 //
 // What bounds it (8192 x 2048 x 32000 bf16, 6144 rows counted, 2.42 TFLOP: 2.2 ms, 1.09 PFLOP/s under the power cap;
 // alone on a cool GPU 600 + 135 + 1100 us in the three long launches): the products by what the SMs can take from L2, 64
-// bytes a clock each, which a 256 x 256 tile of two SMs needs for every 512 clocks of products (13.3 TB/s and 82% of the
-// tensor pipe at depth 4096, measured); at depth 1024 the tiles' starts and ends cost a third (62%). `rows` moves 4
-// bytes a logit at 5.9 TB/s. Small calls cost their four launches, 27 us.
+// bytes a clock each, which a 256 x 256 tile of two SMs needs for every 512 clocks of products (13.2 TB/s and 83 to 88% of
+// the tensor pipe at depth 4096, measured); at depth 1024 the tiles' starts and ends cost a third (63 to 67%, the gradients
+// 75%). `rows` moves 4 bytes a logit at 5.9 TB/s. Small calls cost their four launches, 27 us.
 #include "elem.cuh"
 
 #include <float.h>
