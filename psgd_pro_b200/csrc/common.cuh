@@ -161,6 +161,11 @@ PSGD_DEVI uint32_t mapa_shared(const void* p, uint32_t rank) {
   return r;
 }
 
+// A word into the shared memory of either CTA of the cluster (address from mapa_shared).
+PSGD_DEVI void store_cluster(uint32_t at, uint32_t v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
 // Arrive on a barrier of either CTA of the cluster (address from mapa_shared), releasing this thread's earlier
 // memory operations to the cluster.
 PSGD_DEVI void mbar_arrive_cluster(uint32_t bar_cluster) {

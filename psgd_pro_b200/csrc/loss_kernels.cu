@@ -18,6 +18,7 @@
 // the tensor pipe at depth 4096, measured); at depth 1024 the tiles' starts and ends cost a third (63 to 67%, the gradients
 // 75%). `rows` moves 4 bytes a logit at 5.9 TB/s. Small calls cost their four launches, 27 us.
 #include "elem.cuh"
+#include "pair_rounds.h"
 
 #include <float.h>
 
@@ -557,8 +558,8 @@ PSGD_DEVI void add_columns(uint32_t at, float* v) {
 // rows. Against one-CTA tiles of 128 x 256 this takes a third less through L2 and shared memory for a product.
 //   warp 0      copies; warp 1 (leader) products; warps 4..11: TMEM lanes 32 (w % 4)..., half of the columns each.
 // Handshakes (waits bounded): full[s] at the leader takes an arrival of each CTA with the bytes that it copies to stage s
-// (the phase cannot end before both have told theirs, so neither waits for the other), empty[s] frees it (the products'
-// commit, in both CTAs), tfull / tempty hand the two accumulators over. An accumulator takes `chunk` blocks of K; the epilogue adds the chunks in registers and hands the accumulator
+// (the phase cannot end before both have told theirs, so neither waits for the other; what a pair that gives up does with
+// rounds that only one of them began: pair_rounds.h), empty[s] frees it (the products' commit, in both CTAs), tfull / tempty hand the two accumulators over. An accumulator takes `chunk` blocks of K; the epilogue adds the chunks in registers and hands the accumulator
 // back at once: the tensor cores' sums truncate (a bias of about 1.1e-9 a product, measured), so sums that are to be
 // right to fp32 stay short there, and the last step of a tile, from registers, never holds the tensor cores up.
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>
@@ -575,6 +576,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
   uint64_t* drain = tempty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile uint32_t* issued = tmem_slot + 2;     // rounds of copies that this CTA issued
+  volatile uint32_t* peer_word = tmem_slot + 3;  // the peer's, and whether it gave up, from the peer
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();  // 0: leader
 
@@ -589,6 +592,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     }
     mbar_init(drain, 1);
     *abort = 0;
+    *issued = 0;
     fence_barrier_init();
   }
   if (warp == 0 && lane < 2 * args.nproblems * LIMBS) {  // (the maps are arguments: no launch before writes them)
@@ -620,7 +624,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     if (warp == 0 && lane == 0) {
       // ---------------- copies (both CTAs) ----------------
       int s = 0;
-      uint32_t ph = 0, rounds = 0;  // rounds that this CTA armed; they land before the leader leaves on abort
+      uint32_t ph = 0, rounds = 0;
       int which, index;
       for (int k = 0; deal.get(k, which, index) && !*abort; ++k) {
         const LceProblem& p = args.p[which];
@@ -655,18 +659,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
           if (++s == S) s = 0, ph ^= 1;
         }
       }
-      if (*abort && rank == 0) {
-        for (int i = 0; i < S; ++i) {
-          const uint32_t n = rounds / S + ((uint32_t)i < rounds % S);
-          volatile int never = 0;
-          if (n) mbar_wait(&full[i], (n - 1) & 1, &never);
-        }
-      }
+      *issued = rounds;
     } else if (warp == 1 && lane == 0 && rank == 0) {
       // ---------------- products (leader) ----------------
       int s = 0;
       uint32_t ph = 0, i = 0;
-      bool issued = false, ok = true;
+      bool ok = true;
       int which, index;
       for (int k = 0; ok && deal.get(k, which, index); ++k) {
         const LceProblem& p = args.p[which];
@@ -711,18 +709,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
                 more = 1;
               }
             }
-            issued = true;
             umma_commit_pair(&empty[s], 3);
             if (++s == S) s = 0, ph ^= 1;
           }
           if (!ok) break;
           umma_commit_pair(&tfull[acc], 3);
         } while (kb < u.k1);
-      }
-      if (*abort && issued) {  // every issued product (it reads both CTAs' shared memory) finishes first
-        umma_commit_pair(drain, 1);
-        volatile int never = 0;
-        mbar_wait(drain, 0, &never);
       }
     }
   } else {
@@ -812,9 +804,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     }
   }
 
+  // Neither CTA releases shared memory or TMEM while the other may still use them. Each tells the other, before they meet,
+  // how many rounds of copies it issued and whether it gave up: both are final after the block's barrier.
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // neither CTA releases shared memory or TMEM while the other may still use them
+  if (threadIdx.x == 0) store_cluster(mapa_shared((const void*)peer_word, rank ^ 1), *issued << 1 | (*abort != 0));
+  __syncwarp();
+  cluster_sync();
+  if (*abort || (*peer_word & 1u)) {
+    // One of them left work behind. The leader, whose barriers all copies report to, waits until those of both CTAs have
+    // landed and until the products that it issued (they read both CTAs' shared memory and write both's TMEM) are done;
+    // the peer waits for the leader. A CTA that gave up is behind by rounds that it never copied.
+    if (rank == 0 && threadIdx.x == 0) {
+      volatile int never = 0;
+      for (int i = 0; i < S; ++i) {
+        const StageLeft left = stage_left(*issued, *peer_word >> 1, S, i);
+        if (left.arrive) mbar_arrive(&full[i]);
+        if (left.wait) mbar_wait(&full[i], left.parity, &never);
+      }
+    }
+    if (rank == 0 && warp == 1 && lane == 0) {  // (the thread that issued them)
+      volatile int never = 0;
+      umma_commit_pair(drain, 1);
+      mbar_wait(drain, 0, &never);
+    }
+    __syncwarp();
+    cluster_sync();
+  }
   tc_fence_after();
   if (warp == 1) {
     __syncwarp();
