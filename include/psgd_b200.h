@@ -112,8 +112,8 @@ int psgd_num_sms(void);
 #define PSGD_ERR_BAD_DESC 8        /* a descriptor failed a device-side check */
 #define PSGD_ERR_NONFINITE 16      /* psgd_factor_update: a factor's L or the Procrustes step came out NaN / Inf */
 
-/* Sets how long the GEMM kernels' waits for work (a TMA stage, a free stage, an accumulator) may take before the
- * launch gives up and sets PSGD_ERR_TIMEOUT_* (default 2 s; 0 restores it) for launches made after the call;
+/* Sets how long the product kernels' waits for work (a TMA stage, a free stage, an accumulator; the GEMM's and the
+ * cross entropy's) may take before the launch gives up and sets PSGD_ERR_TIMEOUT_* (default 2 s; 0 restores it) for launches made after the call;
  * returns the previous limit. An aborting CTA still waits for its own copies and MMAs in flight with the default
  * limit before it releases shared memory and TMEM. No counterpart in the reference (it has no device waits). */
 unsigned long long psgd_set_wait_limit_ns(unsigned long long ns);

@@ -24,6 +24,7 @@ enum : int {
 
 // A wait gives up after this many nanoseconds of %globaltimer; legitimate waits are microseconds.
 constexpr unsigned long long WAIT_LIMIT_NS = 2000000000ull;
+unsigned long long wait_limit();  // (host) WAIT_LIMIT_NS, or what psgd_set_wait_limit_ns set: launches pass it on
 
 PSGD_DEVI uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 

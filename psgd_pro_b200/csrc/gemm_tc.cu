@@ -1553,11 +1553,11 @@ static int num_sms() {
   return n;
 }
 
-// Limit of the GEMM kernels' waits for work (a TMA stage, a free stage, an accumulator), passed to every launch:
+// Limit of the product kernels' waits for work (a TMA stage, a free stage, an accumulator), passed to every launch:
 // WAIT_LIMIT_NS unless psgd_set_wait_limit_ns changed it. The waits of an aborting CTA for its own copies and MMAs
 // in flight keep WAIT_LIMIT_NS whatever this is, so shared memory and TMEM are never released under them.
 static std::atomic<unsigned long long> g_wait_limit_ns{WAIT_LIMIT_NS};
-static unsigned long long wait_limit() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
+unsigned long long wait_limit() { return g_wait_limit_ns.load(std::memory_order_relaxed); }
 
 // Raises the dynamic shared-memory limit of a kernel once per device (never inside a graph capture afterwards).
 static bool smem_attr_once(const void* fn, int bytes) {

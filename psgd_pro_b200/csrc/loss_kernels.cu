@@ -1194,7 +1194,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
   LceArgs args = {};
   args.state = state;
   args.err = err;
-  args.wait_ns = WAIT_LIMIT_NS;
+  args.wait_ns = wait_limit();
   for (int piece = 0; piece < l.pieces; ++piece) {
     const int row0 = piece * l.piece, rows = a.n - row0 < l.piece ? a.n - row0 : l.piece;
     const int rows64 = (rows + 63) / 64 * 64;
