@@ -9,8 +9,9 @@ reference, whose models run on torch's own operators):
 
 Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 and each output is rounded once. Work is
 enqueued on the current stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
-The functions take part in autograd; the *_forward / *_grad forms are the same launches for callers that hold the
-gradients themselves (KronWhiten.step_math takes them as they come). Argument errors raise RuntimeError at the call.
+The functions take part in autograd (once: second derivatives and forward mode raise); the *_forward / *_grad forms are the
+same launches for callers that hold the gradients themselves (KronWhiten.step_math takes them as they come) and that
+autograd does not see. Argument errors raise RuntimeError at the call.
 A target that is no class is found on the device: it counts as ignored, and later linear_cross_entropy calls (and
 check_errors(), which waits) raise until reset_errors(), as for the operators of psgd_pro_b200.ops."""
 import ctypes
@@ -18,6 +19,7 @@ from typing import NamedTuple, Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _capi
@@ -71,6 +73,14 @@ def _new(t):
     return torch.empty_like(t) if t.is_contiguous() else torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
+def _differentiated(*tensors):
+    """Whether autograd has to see the call: a gradient will be asked for, or an input carries a forward-mode tangent, which a
+    launch of its own would drop without a word (the autograd functions have no forward-mode formula and raise)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 # ---- dropout --------------------------------------------------------------------------------------------------------
 def _generator(p, seed, offset, x):
     """(threshold, scale, seed, offset, rng pointer) of a mask."""
@@ -122,7 +132,7 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0, residual: Optional[Tenso
     is 1 / (1 - T / 65536), so p has a resolution of 2^-16. The same (seed, offset) gives the same mask: take another
     offset for each use and step. seed may instead be an int64 CUDA tensor (seed, offset), read by the kernel, so that a
     captured CUDA graph draws another mask at each replay; it must not change before the backward pass has run."""
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
+    if _differentiated(x, residual):
         return _Dropout.apply(x, p, seed, offset, residual)
     return _dropout(x, p, seed, offset, residual)
 
@@ -315,7 +325,7 @@ def residual_norm(x: Tensor, y: Tensor, *, norm: str = "rms", post_norm: bool = 
     residual scale. Dropout as in dropout(), over the elements of x in row-major order."""
     options = dict(norm=norm, post_norm=post_norm, scale=scale, eps=eps, dropout_p=dropout_p, seed=seed, offset=offset)
     tensors = (x, y, weight, bias, post_weight, post_bias, gate)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+    if _differentiated(*tensors):
         return _ResidualNorm.apply(*tensors, options)
     return residual_norm_forward(x, y, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, gate=gate,
                                  **options)[:2]
@@ -452,7 +462,7 @@ def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: 
     bits); tokens are taken in pieces of that size (of 256 at least)."""
     options = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, z_loss=z_loss, reduction=reduction,
                    piece_bytes=piece_bytes)
-    if torch.is_grad_enabled() and (h.requires_grad or w.requires_grad):
+    if _differentiated(h, w):
         return _LinearCrossEntropy.apply(h, w, target, options)
     return _lce(h, w, target, (False, False), None, **options)[0]
 

@@ -2,6 +2,12 @@
 import os
 import re
 
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from psgd_pro_b200 import layers
+
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "psgd_pro_b200", "csrc")
 
 
@@ -14,3 +20,34 @@ def test_every_bounded_launch_takes_the_settable_wait_limit():
         assert not re.search(r"wait_ns\s*=\s*WAIT_LIMIT_NS", text), name
         given += re.findall(r"wait_limit\(\)\)|wait_ns = wait_limit\(\)", text)
     assert len(given) >= 4
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The launches replaced by plain ones, so that calls on host tensors run through autograd's side of the module."""
+    monkeypatch.setattr(layers, "_dropout", lambda x, p, seed, offset, residual: x * 2 if residual is None else residual + x * 2)
+    monkeypatch.setattr(layers, "residual_norm_forward", lambda x, y, **_: (x + y, x + y, torch.ones(1)))
+    monkeypatch.setattr(layers, "residual_norm_grad", lambda d_out, d_normed, out, y, *_, **__: layers.ResidualNormGrads(
+        torch.ones_like(out), torch.ones_like(y), *[None] * 5))
+    monkeypatch.setattr(layers, "_lce", lambda h, w, t, need, *_, **__: ((h @ w.T).sum(), torch.ones_like(h), torch.ones_like(w)))
+
+
+CALLS = {
+    "dropout": lambda a, b: layers.dropout(a, 0.5, 1),
+    "dropout residual": lambda a, b: layers.dropout(b, 0.5, 1, residual=a),
+    "joint": lambda a, b: layers.residual_norm(a, b),
+    "joint weight": lambda a, b: layers.residual_norm(b, b, weight=a),
+    "loss": lambda a, b: layers.linear_cross_entropy(a, b, torch.zeros(4, dtype=torch.int64)),
+    "loss weight": lambda a, b: layers.linear_cross_entropy(b, a, torch.zeros(4, dtype=torch.int64)),
+}
+
+
+@pytest.mark.parametrize("call", list(CALLS))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(launches, call, grad):
+    """A tangent is not lost without a word, whether or not gradients are recorded; the same call without one runs."""
+    a, b = torch.ones(4, 4), torch.ones(4, 4)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        CALLS[call](a, b)
+        with pytest.raises(RuntimeError, match="forward mode"):
+            CALLS[call](forward_ad.make_dual(a, torch.ones(4, 4)), b)
