@@ -114,13 +114,19 @@ def _dropout(x, p, seed, offset, residual):
 class _Dropout(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, p, seed, offset, residual):
-        ctx.mask = (p, seed, offset)
+        # (a seed tensor is saved as one, so that a change of it before the backward pass raises there)
+        ctx.mask = (p, None if isinstance(seed, Tensor) else seed, offset)
+        ctx.save_for_backward(seed if isinstance(seed, Tensor) else None)
         return _dropout(x, p, seed, offset, residual)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        dx = dropout_grad(dy, *ctx.mask) if ctx.needs_input_grad[0] else None
+        dx = None
+        if ctx.needs_input_grad[0]:
+            p, seed, offset = ctx.mask
+            rng, = ctx.saved_tensors
+            dx = dropout_grad(dy, p, seed if rng is None else rng, offset)
         return dx, None, None, None, dy if ctx.needs_input_grad[4] else None
 
 
@@ -131,7 +137,8 @@ def dropout(x: Tensor, p: float, seed, offset: int = 0, residual: Optional[Tenso
     (i / 8, offset) under the 64-bit key `seed` is at least T = round(65536 p), whatever the type, shape or strides; the scale
     is 1 / (1 - T / 65536), so p has a resolution of 2^-16. The same (seed, offset) gives the same mask: take another
     offset for each use and step. seed may instead be an int64 CUDA tensor (seed, offset), read by the kernel, so that a
-    captured CUDA graph draws another mask at each replay; it must not change before the backward pass has run."""
+    captured CUDA graph draws another mask at each replay; it must not change before the backward pass has run (autograd
+    raises where it sees a change in place)."""
     if _differentiated(x, residual):
         return _Dropout.apply(x, p, seed, offset, residual)
     return _dropout(x, p, seed, offset, residual)
@@ -296,19 +303,21 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, x, y, weight, bias, post_weight, post_bias, gate, options):
         out, normed, stats = residual_norm_forward(x, y, weight=weight, bias=bias, post_weight=post_weight,
                                                    post_bias=post_bias, gate=gate, **options)
-        ctx.save_for_backward(out, y, stats, weight, bias, post_weight, post_bias, gate)
-        ctx.options = options
+        rng = options["seed"] if options["dropout_p"] and isinstance(options["seed"], Tensor) else None
+        ctx.save_for_backward(out, y, stats, weight, bias, post_weight, post_bias, gate, rng)
+        ctx.options = dict(options, seed=0) if rng is not None else options
         ctx.set_materialize_grads(False)
         return out, normed
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out, d_normed):
-        out, y, stats, weight, bias, post_weight, post_bias, gate = ctx.saved_tensors
+        out, y, stats, weight, bias, post_weight, post_bias, gate, rng = ctx.saved_tensors
         if d_out is None and d_normed is None:
             return (None,) * 8
+        options = ctx.options if rng is None else dict(ctx.options, seed=rng)
         g = residual_norm_grad(d_out, d_normed, out, y, stats, weight=weight, bias=bias, post_weight=post_weight,
-                               post_bias=post_bias, gate=gate, **ctx.options)
+                               post_bias=post_bias, gate=gate, **options)
         return (*(t if need else None for t, need in zip(g, ctx.needs_input_grad)), None)
 
 

@@ -51,3 +51,16 @@ def test_forward_mode_is_refused(launches, call, grad):
         CALLS[call](a, b)
         with pytest.raises(RuntimeError, match="forward mode"):
             CALLS[call](forward_ad.make_dual(a, torch.ones(4, 4)), b)
+
+
+@pytest.mark.parametrize("call", ["dropout", "dropout residual", "joint"])
+def test_a_seed_tensor_changed_before_the_backward_pass_is_noticed(launches, call):
+    x = torch.ones(4, 4, requires_grad=True)
+    rng = torch.tensor([3, 0])
+    f = {"dropout": lambda: layers.dropout(x, 0.5, rng), "dropout residual": lambda: layers.dropout(x, 0.5, rng, residual=x),
+         "joint": lambda: sum(layers.residual_norm(x, x, dropout_p=0.5, seed=rng))}[call]
+    torch.autograd.grad(f().sum(), x)
+    y = f().sum()
+    rng[1] += 1
+    with pytest.raises(RuntimeError, match="inplace"):
+        torch.autograd.grad(y, x)

@@ -58,3 +58,26 @@ def test_loss_stays_inside_a_shorter_wait_limit(cuda):
     finally:
         assert lib.psgd_set_wait_limit_ns(0) == 200_000_000
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- autograd --------------------------------------------------------------------------------------------------------
+def test_seed_tensors_under_autograd(cuda):
+    """The masks of a seed tensor are those of the same numbers, forward and backward, and a change of it in between raises."""
+    x, y, up = (torch.randn(20, 48, device=cuda, requires_grad=k < 2) for k in range(3))
+    rng = torch.tensor([11, 5], device=cuda)
+
+    def both(**k):
+        a = layers.dropout(x, 0.3, residual=y, **k)
+        b, c = layers.residual_norm(x, y, dropout_p=0.3, **k)
+        return a, b, c
+
+    got, want = both(seed=rng), both(seed=11, offset=5)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for pair in zip(got, want):
+        a, b = (torch.autograd.grad(v, (x, y), up, retain_graph=True) for v in pair)  # (out and normed are of one node)
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    late = both(seed=rng)
+    rng[1] += 1
+    for a in late:
+        with pytest.raises(RuntimeError, match="inplace"):
+            torch.autograd.grad(a, (x, y), up)
