@@ -39,12 +39,22 @@ constexpr int L_UNIT = 8;            // what a unit costs besides its K blocks (
 constexpr float L_KEEP_SCALE = 32768.f;
 // g is held times 2^8 when it is fp16: p below 2^-14 keeps its bits down to 2^-22 and |g| may reach 255.
 constexpr float L_HALF_SCALE = 256.f;
+// Upstream gradients by row have the range of fp32, which fp16 operands do not: g takes their significand alone, in [1/2, 1).
+// dh multiplies a row by 2^e of its own at the end, so that rows do not affect each other; for dw, h takes 2^e, exactly but
+// for what lies below 2^-29 of the largest |upstream h| of the call, which is brought just below 2^L_REACH.
+constexpr int L_REACH = 15, L_NO_REACH = -1000;
 
 struct LceState {  // device scalars of one call
   int counted;
-  float alpha;     // factor of both gradients
-  float row_unit;  // per-row upstream gradients are divided by this
+  float alpha;  // factor of both gradients
+  int reach;    // fp16 by rows: every finite |upstream h| is below 2^reach
 };
+
+// x = m 2^e with |m| in [1/2, 1) (zero, infinities and NaN: themselves, e = 0).
+PSGD_DEVI float split_power(float x, int& e) {
+  e = 0;
+  return fabsf(x) <= FLT_MAX ? frexpf(x, &e) : x;
+}
 
 // The error word may be pinned host memory, where atomics are not to be relied on: bits are added by a plain store (when
 // two kinds of error meet, one of them is reported).
@@ -79,12 +89,10 @@ struct LcePlan {
       loss[i] = 0.f;
     }
   }
-  PSGD_DEVI void finish(int total, float top) const {
+  PSGD_DEVI void finish(int total) const {
     state->counted = total;
-    // fp16 gradients: per-row upstream values are taken relative to the largest, so that g stays in range
-    const float unit = half && none() && grad && top > 0.f ? top : 1.f;
-    state->row_unit = unit;
-    float alpha = half ? unit / L_HALF_SCALE : 1.f;
+    state->reach = L_NO_REACH;
+    float alpha = half ? 1.f / L_HALF_SCALE : 1.f;
     if (!none() && grad) alpha *= *grad;
     if (reduction == PSGD_REDUCE_MEAN) alpha /= (float)max(total, 1);
     state->alpha = alpha;
@@ -97,9 +105,7 @@ constexpr int PLAN_GROUPS = 64;  // groups of 32 targets that a warp has at a ti
 __global__ void __launch_bounds__(1024) lce_plan_kernel(const LcePlan a) {
   __shared__ int count[PLAN_GROUPS * 32];
   __shared__ int warp_total[32];
-  __shared__ float tops[32];
   const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-  float top = 0.f;
   bool bad = false;
   int total = 0;
   pdl_trigger();
@@ -109,7 +115,6 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const LcePlan a) {
     for (int g = 0; g < groups; ++g) {
       const int i = base + g * 1024 + t;
       const bool counted = a.counts(i < a.n ? a.target[i] : a.ignore, bad);
-      if (a.none() && a.grad && counted) top = fmaxf(top, fabsf(a.grad[i]));
       const uint32_t m = __ballot_sync(0xffffffffu, counted);
       if (lane == 0) count[g * 32 + warp] = __popc(m);
     }
@@ -149,13 +154,7 @@ __global__ void __launch_bounds__(1024) lce_plan_kernel(const LcePlan a) {
     __syncthreads();
   }
   if (bad) report(a.err, ERR_BAD_TARGET);
-  top = warp_max(top);
-  if (lane == 0) tops[warp] = top;
-  __syncthreads();
-  if (t == 0) {
-    for (int w = 1; w < 32; ++w) top = fmaxf(top, tops[w]);
-    a.finish(total, top);
-  }
+  if (t == 0) a.finish(total);
 }
 
 // ---- stage -----------------------------------------------------------------------------------------------------------
@@ -185,7 +184,6 @@ template <typename T, bool WIDE, bool VEC, bool INLINE>
 __global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, const LceStage<T> w, int d, const LcePlan plan) {
   constexpr int V = VEC ? 8 : 1;
   __shared__ int before[8];
-  __shared__ float tops[8];
   pdl_trigger();
   if (!INLINE) pdl_wait();
   const bool first = (int)blockIdx.x < h.blocks;
@@ -197,22 +195,16 @@ __global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, con
     const bool last = (int)blockIdx.x == h.blocks - 1;  // (beyond every row: it counts them all)
     const int upto = min(i0, plan.n);
     int mine = 0;
-    float top = 0.f;
     bool bad = false;
 #pragma unroll 4
-    for (int k = threadIdx.x; k < upto; k += 256) {
-      const bool yes = plan.counts(plan.target[k], bad);
-      mine += yes;
-      if (last && yes && plan.none() && plan.grad) top = fmaxf(top, fabsf(plan.grad[k]));
-    }
+    for (int k = threadIdx.x; k < upto; k += 256) mine += plan.counts(plan.target[k], bad);
     mine = __reduce_add_sync(0xffffffffu, mine);
-    top = warp_max(top);
-    if (lane == 0) before[warp] = mine, tops[warp] = top;
+    if (lane == 0) before[warp] = mine;
     __syncthreads();
     counted = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) counted += before[k], top = fmaxf(top, tops[k]);
-    if (last && threadIdx.x == 0) plan.finish(counted, top);
+    for (int k = 0; k < 8; ++k) counted += before[k];
+    if (last && threadIdx.x == 0) plan.finish(counted);
     if (last && bad) report(plan.err, ERR_BAD_TARGET);
     if (i0 < plan.n) {  // this block's rows; a warp a row, each with the targets of all eight
       const long long x = lane < 8 && i0 + lane < plan.n ? plan.target[i0 + lane] : plan.ignore;
@@ -270,6 +262,48 @@ __global__ void __launch_bounds__(256) lce_stage_kernel(const LceStage<T> h, con
   }
 }
 
+// fp16 by rows, for every counted row, a warp each: what its row of dh is multiplied by in the end, and how far upstream times
+// h reaches (a maximum: the order of its atomics does not matter).
+__global__ void __launch_bounds__(256) lce_reach_kernel(const __half* __restrict__ h, long long ld, int d, const float* __restrict__ grad,
+                                                        const int* __restrict__ row_of, float* __restrict__ row_scale, LceState* state) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= state->counted) return;
+  int e;
+  const float m = split_power(grad[row_of[r]], e);
+  if (lane == 0) row_scale[r] = ldexpf(state->alpha, e);
+  if (m == 0.f || !(fabsf(m) <= FLT_MAX)) return;
+  float top = 0.f;
+  for (int c = lane; c < d; c += 32) {
+    const float x = fabsf(__half2float(h[r * ld + c]));
+    if (x <= FLT_MAX) top = fmaxf(top, x);
+  }
+  top = warp_max(top);
+  if (lane == 0 && top > 0.f) {
+    int k;
+    split_power(top, k);
+    atomicMax(&state->reach, e + k);
+  }
+}
+// fp16 by rows: a piece's rows of h, done with as the logits' operand, times their upstream 2^e, as dw's.
+__global__ void __launch_bounds__(256) lce_lift_kernel(__half* __restrict__ h, long long ld, int d, const float* __restrict__ grad,
+                                                       const int* __restrict__ row_of, int row0, int rows, const LceState* state) {
+  pdl_trigger();
+  pdl_wait();
+  const int r = row0 + blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= min(row0 + rows, state->counted)) return;
+  int e;
+  const float m = split_power(grad[row_of[r]], e);
+  if (!(fabsf(m) <= FLT_MAX)) return;  // (its g is infinite or NaN, and so is dw)
+  const int by = e + L_REACH - state->reach;
+  for (int c = lane; c < d; c += 32) {
+    const float x = __half2float(h[r * ld + c]);
+    // (a row that counts nothing may have any h: zero, so that it does not leave the type's range)
+    if (fabsf(x) <= FLT_MAX) h[r * ld + c] = __float2half_rn(m == 0.f ? 0.f : ldexpf(x, by));
+  }
+}
+
 // ---- the products ----------------------------------------------------------------------------------------------------
 // D (M x N) = A B^T over K. An operand is K-major (rows of M or N, K contiguous) or MN-major (rows of K, M or N contiguous:
 // *_mn). fp32 operands are three bf16 limbs: the products of limbs (i, j) with i + j <= 2 (2^-24 of the whole is left out).
@@ -283,11 +317,20 @@ struct LceProblem {
   const int* row_of;
   void* out;
   long long ld_out;
+  const float* row_scale;  // dh, fp16 by rows: instead of alpha, by counted row
+  int lifted;              // dw, fp16 by rows: h was brought below 2^L_REACH
   float* part;       // splits > 1: [split][M][ld_part], joined by lce_join_kernel
   const float* acc;  // earlier pieces' sums [M][ld_acc], added
   float* acc_out;    // sums so far, fp32, instead of out
   long long ld_part, ld_acc;
 };
+// What the sums of a gradient of type T are multiplied by, but for row_scale.
+template <typename T>
+PSGD_DEVI float lce_alpha(const LceState* state, int lifted) {
+  if constexpr (is_half<T>())
+    if (lifted) return ldexpf(state->alpha, state->reach - L_REACH);
+  return state->alpha;
+}
 struct LceShape {
   int M, K, tiles_m, tiles_n, kblocks, units, unit_kblocks;
 };
@@ -512,6 +555,8 @@ PSGD_DEVI void grad_row(const LceProblem& p, const LceShape& sh, int split, long
     return;
   }
   constexpr int S = 32 / sizeof(T);
+  if constexpr (is_half<T>())
+    if (p.row_scale && live) alpha = p.row_scale[p.row0 + row];
 #pragma unroll
   for (int k = 0; k < COLS; ++k) v[k] *= alpha;
   const int at = live ? (p.row_of ? p.row_of[p.row0 + row] : (int)row) : -1;
@@ -736,13 +781,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(L_THREADS, 1)
     }
     float* turn = reinterpret_cast<float*>(smem + S * C::STAGE + 512) + (warp - 4) * (32 * 33);
     const uint32_t lead0 = mapa_shared(&tempty[0], 0), lead1 = mapa_shared(&tempty[1], 0);
-    const float alpha = args.state->alpha;
+    const float alpha0 = lce_alpha<OUT>(args.state, args.p[0].lifted), alpha1 = lce_alpha<OUT>(args.state, args.p[1].lifted);
     uint32_t i = 0;
     bool ok = true;
     int which, index;
     for (int k = 0; ok && deal.get(k, which, index); ++k) {
       const LceProblem& p = args.p[which];
       const LceShape& sh = which ? s1 : s0;
+      const float alpha = which ? alpha1 : alpha0;
       const LceUnit u = lce_unit(p, sh, index);
       const int rounds = (u.k1 - u.k0 + C::KS - 1) / C::KS, chunks = max(1, (rounds + chunk - 1) / chunk);
       const long long row = (long long)u.tm * LM + rank * 128 + q * 32 + lane;
@@ -928,7 +974,13 @@ __global__ void __launch_bounds__(256) lce_rows_kernel(const LceRows a, const Lc
   if (!a.kept) return;
   const int shift = a.stat == 64 ? 6 : 7;
   constexpr float unit = is_half<GT>() ? L_HALF_SCALE : 1.f;
-  const float c = (a.grad ? a.grad[a.row_of[a.row0 + row]] / state->row_unit : 1.f) * unit;
+  float up = a.grad ? a.grad[a.row_of[a.row0 + row]] : 1.f;
+  if constexpr (is_half<GT>())
+    if (a.grad) {
+      int e;
+      up = split_power(up, e);  // (2^e: row_scale, and dw's h)
+    }
+  const float c = up * unit;
   const float more = 2.f * a.z * lse, pull = 1.f + more, uniform = a.smoothing / (float)a.v;
   const float scale = sizeof(KT) == 4 ? 1.f : 1.f / L_KEEP_SCALE;
   // the target's element from its fp32 logit: p - 1 without cancellation
@@ -986,16 +1038,17 @@ int scale(void* x, long long n, const float* factor, cudaStream_t stream) {
   return cudaGetLastError() == cudaSuccess ? PSGD_OK : PSGD_ELAUNCH;
 }
 
-// Joins the splits of a gradient: out[row] = alpha * sum over splits, in their order. Rows are the counted ones through
+// Joins the splits of a gradient: out[row] = alpha (or the row's factor) * sum over splits, in their order. Rows are the counted ones through
 // row_of, or all M of them as they are. V: values at a time (N a multiple, or 1).
 template <typename T, int V>
 __global__ void __launch_bounds__(256) lce_join_kernel(const float* __restrict__ part, int splits, int M, int N,
                                                        long long ld_part, int row0, const int* __restrict__ row_of,
-                                                       T* __restrict__ out, const LceState* state) {
+                                                       const float* __restrict__ row_scale, int lifted, T* __restrict__ out,
+                                                       const LceState* state) {
   pdl_wait();
   const int there = row_of ? min(M, max(0, state->counted - row0)) : M, per_row = N / V;
   const long long n = (long long)there * per_row, plane = M * ld_part;
-  const float alpha = state->alpha;
+  const float alpha = lce_alpha<T>(state, lifted);
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
     const int r = (int)(i / per_row), c = (int)(i - (long long)r * per_row) * V;
     float s[V] = {};
@@ -1006,8 +1059,9 @@ __global__ void __launch_bounds__(256) lce_join_kernel(const float* __restrict__
 #pragma unroll
       for (int e = 0; e < V; ++e) s[e] += x[e];
     }
+    const float by = is_half<T>() && row_scale ? row_scale[row0 + r] : alpha;
 #pragma unroll
-    for (int e = 0; e < V; ++e) s[e] *= alpha;
+    for (int e = 0; e < V; ++e) s[e] *= by;
     store_vec<T, V>(out + (long long)(row_of ? row_of[row0 + r] : r) * N + c, s);
   }
 }
@@ -1046,7 +1100,7 @@ struct Layout {
   int limbs, tiles, piece, pieces, splits, splits_w, bn, bn_grads, stat;
   bool stage_w;
   long long ld_h, ld_w, ld_kept, ld_part, h_plane, w_plane, g_plane;
-  size_t state, rank, row_of, row_target, loss_rows, target_logit, stats, linear, h, w, kept, g, part, part_w, acc, bytes;
+  size_t state, rank, row_of, row_target, loss_rows, row_scale, target_logit, stats, linear, h, w, kept, g, part, part_w, acc, bytes;
 };
 
 // Whether the operands are three bf16 limbs: fp32 ones, and 16-bit ones of up to 2^20 products, where g, whose one rounding
@@ -1107,6 +1161,7 @@ Layout layout(const PsgdLce& a) {
   l.row_of = take(4ull * a.n);
   l.row_target = take(4ull * a.n);
   l.loss_rows = take(4ull * a.n);
+  l.row_scale = take(!wide && a.dtype == PSGD_F16 && a.grads && a.reduction == PSGD_REDUCE_NONE ? 4ull * a.n : 0);
   l.target_logit = take(4ull * piece);
   l.stats = take(8ull * piece * l.tiles);
   l.linear = take(a.label_smoothing != 0.f ? 4ull * piece * l.tiles : 0);
@@ -1191,6 +1246,15 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
       return rc;
   }
 
+  // fp16 by rows: what to multiply dh's rows and dw with
+  const bool by_rows = half && a.grads && none && a.grad;
+  float* row_scale = reinterpret_cast<float*>(ws + l.row_scale);
+  if constexpr (half)
+    if (by_rows)
+      if (int rc = pdl_launch(lce_reach_kernel, dim3((a.n + 7) / 8), dim3(256), 0, stream, (const __half*)h, l.ld_h, a.d, a.grad,
+                              (const int*)row_of, row_scale, state))
+        return rc;
+
   LceArgs args = {};
   args.state = state;
   args.err = err;
@@ -1234,6 +1298,11 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
                          : pdl_launch(lce_rows_kernel<KT, OP, false>, dim3(rows64, cols), dim3(256), 0, stream, r, (const LceState*)state))
       return rc;
     if (!a.grads) continue;
+    if constexpr (half)
+      if (by_rows && a.dw)
+        if (int rc = pdl_launch(lce_lift_kernel, dim3((rows + 7) / 8), dim3(256), 0, stream, (__half*)h, l.ld_h, a.d, a.grad,
+                                (const int*)row_of, row0, rows, (const LceState*)state))
+          return rc;
 
     const uint16_t* gm = reinterpret_cast<const uint16_t*>(ws + l.g);
     args.nproblems = 0;
@@ -1244,6 +1313,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
         if (int rc = encode(&ph.tb[i], w + i * l.w_plane, half, a.v, a.d, ld_w, 64)) return rc;
       }
       ph.b_mn = 1, ph.M = rows, ph.N = a.d, ph.K = a.v, ph.dyn = 1, ph.row0 = row0, ph.splits = l.splits;
+      ph.row_scale = by_rows ? row_scale : nullptr;
       ph.row_of = row_of, ph.out = a.dh, ph.ld_out = a.d, ph.ld_part = l.ld_part;
       ph.part = l.splits > 1 ? reinterpret_cast<float*>(ws + l.part) : nullptr;
     }
@@ -1254,6 +1324,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
         if (int rc = encode(&pw.tb[i], h + i * l.h_plane + (long long)row0 * l.ld_h, half, rows64, a.d, l.ld_h, 64)) return rc;
       }
       pw.a_mn = pw.b_mn = 1, pw.M = a.v, pw.N = a.d, pw.K = rows, pw.dyn = 2, pw.row0 = row0, pw.splits = l.splits_w;
+      pw.lifted = by_rows;
       pw.out = a.dw, pw.ld_out = a.d, pw.ld_part = l.ld_part;
       pw.part = l.splits_w > 1 ? reinterpret_cast<float*>(ws + l.part_w) : nullptr;
       if (l.pieces > 1) {
@@ -1271,7 +1342,7 @@ int run(const PsgdLce& a, int* err, cudaStream_t stream) {
       const long long n = (long long)p.M * a.d / (eight ? 8 : 1), want = (n + 255) / 256, most = 8LL * psgd_num_sms();
       return pdl_launch(eight ? lce_join_kernel<T, 8> : lce_join_kernel<T, 1>, dim3((int)(want < most ? want : most)),
                         dim3(256), 0, stream, (const float*)p.part, p.splits, p.M, a.d, p.ld_part, row0, p.row_of,
-                        reinterpret_cast<T*>(out), (const LceState*)state);
+                        p.row_scale, p.lifted, reinterpret_cast<T*>(out), (const LceState*)state);
     };
     for (int i = 0; i < args.nproblems; ++i)
       if (args.p[i].part)

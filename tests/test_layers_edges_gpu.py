@@ -81,3 +81,64 @@ def test_seed_tensors_under_autograd(cuda):
     for a in late:
         with pytest.raises(RuntimeError, match="inplace"):
             torch.autograd.grad(a, (x, y), up)
+
+
+# ---- upstream gradients by row ---------------------------------------------------------------------------------------
+def by_rows_bounds(h, w, t, up, smoothing, z):
+    """What may be lost of dh's rows and of dw's, in 64 bits: the kept exponentials rounded once to fp16 (2^-11 of p's part of
+    g), g once more (2^-11 of a value, or the 2^-25 of what is below the type's range, at 2^8 times g), a hundredth of that
+    for the fp32 arithmetic in between, and each value of the result rounded once to fp16."""
+    rows = (t != -100).nonzero()[:, 0]
+    h, w, up = h.double()[rows], w.double(), up.double()[rows]
+    logits = h @ w.T
+    lse = logits.logsumexp(1)
+    part = (logits - lse[:, None]).exp() * (1 + 2 * z * lse)[:, None]
+    g = (part - smoothing / w.shape[0]).scatter_add_(1, t[rows][:, None], torch.full_like(lse, smoothing - 1)[:, None])
+    dg = (1.01 * 2.0 ** -11 * (g.abs() + part.abs()) + 2.0 ** -32) * up.abs()[:, None]
+    dh, dw = (g * up[:, None]) @ w, (g * up[:, None]).T @ h
+    off_h = dg @ w.abs() + dh.abs() * 2.0 ** -11 + 2.0 ** -24
+    off_w = dg.T @ h.abs() + dw.abs() * 2.0 ** -11 + 2.0 ** -24
+    return rows, dh, dw, off_h, off_w
+
+
+@pytest.mark.parametrize("n,d,v,pieces", [(300, 264, 2003, False), (300, 264, 2003, True), (2500, 72, 300, False), (700, 301, 1003, True)])
+def test_fp16_losses_by_row_with_upstream_gradients_of_all_sizes(cuda, n, d, v, pieces):
+    """Rows do not affect each other: upstream gradients over 24 binary orders, zeros among them, and every value of dh and dw
+    within what the roundings to fp16 take."""
+    h, w, t = lce_case(n, d, v, "fp16", 0.2, cuda)
+    g = torch.Generator(device="cuda").manual_seed(n)
+    up = torch.randn(n, generator=g, device=cuda) * 2.0 ** (torch.rand(n, generator=g, device=cuda) * 24 - 16)
+    up[::17] = 0.0
+    _, dh, dw = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none", label_smoothing=0.05, z_loss=1e-3,
+                                                 **({"piece_bytes": 1} if pieces else {}))
+    rows, want_h, want_w, off_h, off_w = by_rows_bounds(h, w, t, up, 0.05, 1e-3)
+    assert ((dh.double()[rows] - want_h).abs() <= off_h).all()
+    assert ((dw.double() - want_w).abs() <= off_w).all()
+    assert not dh[t == -100].any() and not dh[::17].any()
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = layers.linear_cross_entropy(a, b, t, reduction="none", label_smoothing=0.05, z_loss=1e-3)
+    again = torch.autograd.grad(loss, (a, b), up)
+    if not pieces:
+        assert torch.equal(again[0], dh) and torch.equal(again[1], dw)
+    layers.check_errors()
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+def test_an_infinite_upstream_gradient_stays_in_its_row(cuda, dtype, bad):
+    h, w, t = lce_case(300, 264, 2003, dtype, 0.2, cuda)
+    up = torch.linspace(0.5, 2.0, 300, device=cuda)
+    row = int((t != -100).nonzero()[7, 0])
+    want = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none")
+    up[row] = bad
+    _, dh, dw = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none")
+    others = torch.arange(300, device=cuda) != row
+    assert torch.equal(dh[others], want[1][others]) and not torch.isfinite(dh[row]).any() and not torch.isfinite(dw).any()
+
+
+def test_fp16_losses_by_row_of_nothing(cuda):
+    """All upstream gradients zero, or none of the rows counted."""
+    h, w, t = lce_case(300, 264, 2003, "fp16", 0.2, cuda)
+    for up, target in ((torch.zeros(300, device=cuda), t), (torch.ones(300, device=cuda), torch.full_like(t, -100))):
+        _, dh, dw = layers.linear_cross_entropy_grad(h, w, target, grad=up, reduction="none")
+        assert not dh.any() and not dw.any()
