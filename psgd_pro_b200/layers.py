@@ -15,6 +15,7 @@ autograd does not see. Argument errors raise RuntimeError at the call.
 A target that is no class is found on the device: it counts as ignored, and later linear_cross_entropy calls (and
 check_errors(), which waits) raise until reset_errors(), as for the operators of psgd_pro_b200.ops."""
 import ctypes
+import threading
 from typing import NamedTuple, Optional
 
 import torch
@@ -346,13 +347,16 @@ class _ErrorWords:
     at any time, without a copy or an event: the calls that follow (or check_errors) raise."""
 
     def __init__(self):
-        self.words = {}
+        self.words, self.lock = {}, threading.Lock()
 
     def get(self, device):
         w = self.words.get(device)
         if w is None:
-            t = torch.zeros(1, dtype=torch.int32).pin_memory()
-            w = self.words[device] = (t, ctypes.c_int.from_address(t.data_ptr()), t.data_ptr())
+            with self.lock:  # (one word a device, whichever thread asks first: kernels keep its address)
+                w = self.words.get(device)
+                if w is None:
+                    t = torch.zeros(1, dtype=torch.int32).pin_memory()
+                    w = self.words[device] = (t, ctypes.c_int.from_address(t.data_ptr()), t.data_ptr())
         if w[1].value:
             _fail(f"an earlier linear_cross_entropy reported: {_capi.describe_err(w[1].value)}")
         return w[2]
@@ -363,7 +367,7 @@ class _ErrorWords:
             self.get(device)
 
     def reset(self):
-        for device, w in self.words.items():
+        for device, w in list(self.words.items()):
             torch.cuda.synchronize(device)
             w[1].value = 0
 

@@ -1,6 +1,8 @@
 """Host side of psgd_pro_b200.layers and its C entries at their edges, without a GPU."""
 import os
 import re
+import threading
+import time
 
 import pytest
 import torch
@@ -64,3 +66,22 @@ def test_a_seed_tensor_changed_before_the_backward_pass_is_noticed(launches, cal
     rng[1] += 1
     with pytest.raises(RuntimeError, match="inplace"):
         torch.autograd.grad(y, x)
+
+
+def test_first_calls_of_several_threads_share_one_error_word(monkeypatch):
+    """A second word would leave the one that a kernel was given to the allocator."""
+    made = []
+
+    def pin(t):
+        made.append(t)
+        time.sleep(0.05)  # (the other threads arrive meanwhile)
+        return t
+
+    monkeypatch.setattr(torch.Tensor, "pin_memory", pin)
+    words, got = layers._ErrorWords(), []
+    threads = [threading.Thread(target=lambda: got.append(words.get(0))) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(made) == 1 and len(got) == 4 and len(set(got)) == 1
