@@ -472,7 +472,9 @@ int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cu
  * NULL), for the upstream gradient grad (n values for _NONE, one otherwise; NULL: ones). fp16: 1 + 2 z_loss lse stays
  * below 255. Tokens are taken in pieces of at most piece_bytes of
  * kept exponentials (and at least 256 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
- * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong. */
+ * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong.
+ * n, d and v are at most PSGD_LCE_MAX. */
+#define PSGD_LCE_MAX 1073741824
 #define PSGD_REDUCE_NONE 0
 #define PSGD_REDUCE_MEAN 1
 #define PSGD_REDUCE_SUM 2

@@ -141,6 +141,7 @@ PSGD_F32, PSGD_BF16, PSGD_F16 = 0, 1, 2
 PSGD_NORM_RMS, PSGD_NORM_LAYER = 0, 1
 PSGD_REDUCE_NONE, PSGD_REDUCE_MEAN, PSGD_REDUCE_SUM = 0, 1, 2
 JOINT_MAX_D = 8192
+LCE_MAX = 1 << 30
 PSGD_PREP_NORMAL, PSGD_PREP_TRANS, PSGD_PREP_DIRECT = 0, 1, 2
 PREP_ROWS = 8
 ROT_ROWS = 8

@@ -1183,7 +1183,7 @@ Layout layout(const PsgdLce& a) {
 
 bool valid(const PsgdLce& a) {
   return a.n >= 0 && a.d >= 1 && a.v >= 1 && a.dtype >= 0 && a.dtype <= 2 && a.ld_h >= a.d && a.ld_w >= a.d &&
-         a.reduction >= 0 && a.reduction <= 2 && a.piece_bytes >= 0 && a.n <= (1 << 30) && a.v <= (1 << 30);
+         a.reduction >= 0 && a.reduction <= 2 && a.piece_bytes >= 0 && a.n <= PSGD_LCE_MAX && a.d <= PSGD_LCE_MAX && a.v <= PSGD_LCE_MAX;
 }
 
 template <typename OP, typename OUT, int LIMBS, int BN, bool LOGITS>

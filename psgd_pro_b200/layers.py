@@ -401,6 +401,8 @@ def _lce(h, w, target, need, grad, ignore_index, label_smoothing, z_loss, reduct
     if not 0.0 <= label_smoothing <= 1.0:
         _fail("label_smoothing must lie in [0, 1]")
     v, d = w.shape
+    if max(target.numel(), v, d) > _capi.LCE_MAX:
+        _fail(f"h and w may have up to {_capi.LCE_MAX} rows, each of as many elements")
     if grad is not None:
         if grad.dtype != torch.float32 or grad.get_device() != index or grad.shape != (() if kind else target.shape):
             _fail("grad must be fp32 on the inputs' device: a scalar, or one value for each row with reduction 'none'")

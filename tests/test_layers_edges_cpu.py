@@ -1,4 +1,5 @@
 """Host side of psgd_pro_b200.layers and its C entries at their edges, without a GPU."""
+import ctypes
 import os
 import re
 import threading
@@ -8,8 +9,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from psgd_pro_b200 import layers
+from psgd_pro_b200 import _capi, layers
 
+HDR = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "psgd_b200.h")
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "psgd_pro_b200", "csrc")
 
 
@@ -85,3 +87,15 @@ def test_first_calls_of_several_threads_share_one_error_word(monkeypatch):
     for t in threads:
         t.join()
     assert len(made) == 1 and len(got) == 4 and len(set(got)) == 1
+
+
+def test_sizes_of_the_loss_beyond_its_index_arithmetic_are_refused():
+    defs = dict(re.findall(r"#define (PSGD_\w+) (\d+)", open(HDR).read()))
+    assert int(defs["PSGD_LCE_MAX"]) == _capi.LCE_MAX
+    L = _capi.lib()
+    for name in ("n", "d", "v"):
+        k = _capi.Lce(n=1, d=1, v=1, ld_h=1 << 40, ld_w=1 << 40)
+        setattr(k, name, _capi.LCE_MAX)
+        assert L.psgd_lce_workspace(ctypes.byref(k)) > 0
+        setattr(k, name, _capi.LCE_MAX + 1)
+        assert L.psgd_lce_workspace(ctypes.byref(k)) == -1, name

@@ -83,6 +83,15 @@ def test_seed_tensors_under_autograd(cuda):
             torch.autograd.grad(a, (x, y), up)
 
 
+def test_sizes_beyond_the_index_arithmetic_are_refused(cuda):
+    """Not taken modulo 2^32, which four billion rows (expanded ones here: no memory) would be on their way to the kernels."""
+    one = torch.zeros(1, 1, device=cuda)
+    many, targets = one.expand((1 << 32) + 3, 1), torch.zeros(1, dtype=torch.int64, device=cuda).expand((1 << 32) + 3)
+    for h, w, t in ((many, one, targets), (one, many, targets[:1])):
+        with pytest.raises(RuntimeError, match="rows"):
+            layers.linear_cross_entropy(h, w, t)
+
+
 # ---- upstream gradients by row ---------------------------------------------------------------------------------------
 def by_rows_bounds(h, w, t, up, smoothing, z):
     """What may be lost of dh's rows and of dw's, in 64 bits: the kept exponentials rounded once to fp16 (2^-11 of p's part of
