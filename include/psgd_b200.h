@@ -440,7 +440,7 @@ int psgd_dropout(const PsgdDropout* d, cudaStream_t stream);
  * param_dtype (PSGD_F32 or dtype), or NULL (ones / zeros). gate: `gates` rows of d values, each serving rows / gates consecutive rows, or
  * NULL. stats: four fp32 values a row (mean and 1 / deviation of post, then of the second norm), 16-byte aligned.
  * Dropout as in PsgdDropout (threshold 0: none), element index row * d + column, keep_scale on the kept values.
- * x and y (and d_out, d_normed) have row strides ld_* in elements; every other matrix is contiguous.
+ * x and y (and d_out, d_normed) have row strides ld_* in elements, at least d and below 2^31; every other matrix is contiguous.
  * Backward: x holds the forward pass's out; d_out / d_normed may be NULL (zero); writes dx, dy, dweight and, where the
  * forward pass has them, dbias (layer), dpost_weight, dpost_bias (post, layer), dgate. Sums over rows have a fixed order.
  * The workspace of psgd_joint_workspace(j) bytes is 16-byte aligned. rows = 0 launches nothing. */

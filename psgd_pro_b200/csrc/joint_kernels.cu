@@ -64,6 +64,9 @@ bool valid(const PsgdJoint& j) {
   if ((j.param_dtype != PSGD_F32 && j.param_dtype != j.dtype) || (j.kind != PSGD_NORM_RMS && j.kind != PSGD_NORM_LAYER)) return false;
   const long long most = 1LL << 31;
   if (j.ld_x >= most || j.ld_y >= most || j.ld_d_out >= most || j.ld_d_normed >= most) return false;
+  // (rows do not overlap; a matrix that is not there has no stride)
+  if (j.rows > 1 && ((j.x && j.ld_x < j.d) || (j.y && j.ld_y < j.d) || (j.d_out && j.ld_d_out < j.d) || (j.d_normed && j.ld_d_normed < j.d)))
+    return false;
   if (j.threshold > 65536u || (j.gate && (j.gates < 1 || j.rows % j.gates))) return false;
   return true;
 }

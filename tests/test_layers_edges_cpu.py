@@ -99,3 +99,19 @@ def test_sizes_of_the_loss_beyond_its_index_arithmetic_are_refused():
         assert L.psgd_lce_workspace(ctypes.byref(k)) > 0
         setattr(k, name, _capi.LCE_MAX + 1)
         assert L.psgd_lce_workspace(ctypes.byref(k)) == -1, name
+
+
+def test_joint_row_strides_below_a_row_are_refused():
+    """Also negative ones: rows would be read from before the tensor."""
+    L = _capi.lib()
+    at = dict(x="ld_x", y="ld_y", d_out="ld_d_out", d_normed="ld_d_normed")
+    base = dict({p: 16 for p in at}, **{ld: 16 for ld in at.values()}, rows=4, d=16, eps=1.0)
+    assert L.psgd_joint_workspace(ctypes.byref(_capi.Joint(**base))) > 0
+    for p, ld in at.items():
+        for bad in (15, 0, -16, 1 << 31):
+            j = _capi.Joint(**dict(base, **{ld: bad}))
+            assert L.psgd_joint_workspace(ctypes.byref(j)) == -1, (ld, bad)
+            assert L.psgd_joint_forward(ctypes.byref(j), None) == -1 and L.psgd_joint_backward(ctypes.byref(j), 16, 1 << 30, None) == -1
+    for p, ld in at.items():
+        if p != "x":  # a matrix that is not there needs no stride
+            assert L.psgd_joint_workspace(ctypes.byref(_capi.Joint(**dict(base, **{p: None, ld: 0})))) > 0
