@@ -416,7 +416,7 @@ int psgd_apply_noalloc(void* param, int param_bf16, const float* pg, long long n
 
 /* ---------------------------------------------------------------------------------------------------------
  * Operators of the model that is trained (no counterpart in the reference). Element types: PSGD_F32 / BF16 / F16;
- * arithmetic, statistics and sums are fp32. */
+ * arithmetic, statistics and sums are fp32 (but for the operands of the 16-bit losses' gradients: PsgdLce). */
 #define PSGD_F32 0
 #define PSGD_BF16 1
 #define PSGD_F16 2
@@ -470,7 +470,8 @@ int psgd_joint_backward(const PsgdJoint* j, void* workspace, long long bytes, cu
  * reduction PSGD_REDUCE_NONE (loss: n values, 0 where ignored), _MEAN over the counted rows (0 when there is none) or
  * _SUM (loss: one value). grads != 0: also dh (n x d) and dw (v x d), contiguous, of the inputs' type (either may be
  * NULL), for the upstream gradient grad (n values for _NONE, one otherwise; NULL: ones). fp16: 1 + 2 z_loss lse stays
- * below 255. Tokens are taken in pieces of at most piece_bytes of
+ * below 255. Of 16-bit inputs, beyond 2^20 products n v d, exp(l - max) is kept in fp16 and the gradient of l is rounded once
+ * to the inputs' type before the products that form dh and dw; else operands are bf16 limbs worth 24 bits. Tokens are taken in pieces of at most piece_bytes of
  * kept exponentials (and at least 256 tokens). Workspace: psgd_lce_workspace(a) bytes, 16-byte aligned.
  * dev_err may be pinned host memory that the device can reach: nothing is stored there unless something is wrong.
  * n, d and v are at most PSGD_LCE_MAX. */

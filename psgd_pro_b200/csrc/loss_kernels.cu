@@ -4,7 +4,7 @@
 // for the rows whose target counts. The steps, each one launch:
 //   plan     numbers the counted rows (the others cost nothing below, and no value of theirs is read again);
 //   stage    gathers their rows of h as tensor-core operands (fp32: three bf16 limbs); zeros the other rows of dh;
-//   logits   tile by tile on the tensor cores; the epilogue keeps, per row and 256 columns of the vocabulary, the
+//   logits   tile by tile on the tensor cores; the epilogue keeps, per row and 64 or 128 columns of the vocabulary, the
 //            maximum m and sum of exp(l - m) in fp32 and, for gradients, exp(l - m) itself in 16 bits;
 //   rows     joins those statistics to lse and the loss, and turns exp(l - m) into g in place;
 //   grads    dh = g w and dw = g^T h as one list of tiles (w, g and h are read in the orientation they have, by
@@ -35,7 +35,7 @@ constexpr int L_LIMBS = 3;          // of an fp32 operand
 constexpr int L_GROUP_M = 4;         // row tiles that walk the column tiles together (L2 reuse of both operands)
 constexpr int L_UNIT = 8;            // what a unit costs besides its K blocks (its last step), in K blocks: about 2.5 us
 // Kept exponentials are fp16 of 2^15 exp(l - m), exp(l - m) in [0, 1]: 11 significant bits down to 2^-29 of the row's
-// maximum in these 256 columns, so that the one rounding to 16 bits that matters is that of g.
+// maximum in these columns (half a tile's), so that the one rounding to 16 bits that matters is that of g.
 constexpr float L_KEEP_SCALE = 32768.f;
 // g is held times 2^8 when it is fp16: p below 2^-14 keeps its bits down to 2^-22 and |g| may reach 255.
 constexpr float L_HALF_SCALE = 256.f;
@@ -1103,9 +1103,11 @@ struct Layout {
   size_t state, rank, row_of, row_target, loss_rows, row_scale, target_logit, stats, linear, h, w, kept, g, part, part_w, acc, bytes;
 };
 
-// Whether the operands are three bf16 limbs: fp32 ones, and 16-bit ones of up to 2^20 products, where g, whose one rounding
-// to 16 bits is as large as that of the gradients themselves, does not average out over long sums. Limbs cost such a call 6
-// us on the GPU (7 x 32 x 85: 22.6 us against 16.4), less than its host code takes (28 us); from 2^24 on 10 us and more.
+// Whether the operands are three bf16 limbs: fp32 ones, and 16-bit ones of up to 2^20 products, where limbs cost the call
+// 6 us on the GPU (7 x 32 x 85: 22.6 us against 16.4), less than its host code takes (28 us), and leave the gradients no rounding
+// but their own. Beyond, g is rounded to 16 bits (1e-3 of the gradients in the 2-norm, less where dw's sum over n or dh's over v
+// has many terms of one size, more where one term leads: 1.7e-3 at most, as much as their own rounding): limbs would cost 10
+// us and more from 2^24 products on, and six times the products in the end.
 bool wide_operands(const PsgdLce& a) {
   return a.dtype == PSGD_F32 || (double)a.n * a.v * a.d <= (double)(1 << 20);
 }

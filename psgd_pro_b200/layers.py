@@ -7,8 +7,8 @@ reference, whose models run on torch's own operators):
   linear_cross_entropy   the loss of a large vocabulary from the last hidden states and the head's weight, with both
                          gradients, without ever keeping the logits
 
-Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 and each output is rounded once. Work is
-enqueued on the current stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
+Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 and each output is rounded once (the gradients of
+16-bit losses also carry the rounding of an operand: linear_cross_entropy). Work is enqueued on the current stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
 The functions take part in autograd (once: second derivatives and forward mode raise); the *_forward / *_grad forms are the
 same launches for callers that hold the gradients themselves (KronWhiten.step_math takes them as they come) and that
 autograd does not see. Argument errors raise RuntimeError at the call.
@@ -471,8 +471,15 @@ def linear_cross_entropy(h: Tensor, w: Tensor, target: Tensor, *, ignore_index: 
     (not even with NaN in h); 'mean' divides by the number of the others (0 when there is none). reduction 'none' keeps
     target's shape.
 
+    Precision: losses are fp32 whatever the type (logits from tensor-core sums of at most 1024 products, added in fp32). The
+    gradients of 16-bit inputs are products of operands of that type: d loss / d l is rounded to it once (and before that
+    the exponentials to fp16), which adds about 1e-3 (bf16; fp16: 2e-4) to the 1.7e-3 (2e-4) of the gradients' own rounding, in the
+    2-norm. Calls of up to 2^20 products n v d, where it costs nothing, have three bf16 limbs there instead, as fp32 inputs
+    do (about 1e-6).
+
     Under autograd a scalar loss (mean, sum) of bf16 or fp32 inputs that require gradients forms them at once and holds
-    them for the backward pass; otherwise the backward pass forms loss and gradients again. Evaluation belongs under
+    them for the backward pass, which multiplies them by an upstream gradient other than one (and rounds them once more, if it
+    is no power of two); otherwise the backward pass forms loss and gradients again. Evaluation belongs under
     torch.no_grad(). piece_bytes bounds what is kept of the vocabulary's probabilities at a time (16 bits each; fp32: 80
     bits); tokens are taken in pieces of that size (of 256 at least)."""
     options = dict(ignore_index=ignore_index, label_smoothing=label_smoothing, z_loss=z_loss, reduction=reduction,
