@@ -7,8 +7,9 @@ reference, whose models run on torch's own operators):
   linear_cross_entropy   the loss of a large vocabulary from the last hidden states and the head's weight, with both
                          gradients, without ever keeping the logits
 
-Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 and each output is rounded once (the gradients of
-16-bit losses also carry the rounding of an operand: linear_cross_entropy). Work is enqueued on the current stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
+Tensors are CUDA fp32, bf16 or fp16; arithmetic, statistics and sums are fp32 and each output is rounded once (the
+gradients of 16-bit losses also carry the rounding of an operand: linear_cross_entropy). Work is enqueued on the current
+stream of the inputs' device; outputs and workspaces come from torch's allocator on that stream.
 The functions take part in autograd (once: second derivatives and forward mode raise); the *_forward / *_grad forms are the
 same launches for callers that hold the gradients themselves (KronWhiten.step_math takes them as they come) and that
 autograd does not see. Argument errors raise RuntimeError at the call.
