@@ -250,3 +250,32 @@ def test_only_the_kept_exponentials_and_g_are_rounded_on_the_way(cuda, dtype):
     g = (g * scale).to(TYPES[dtype]).double() / (scale * 600)
     for got, want in ((dh, g @ W), (dw, g.T @ H)):
         assert (got == want.to(TYPES[dtype])).double().mean().item() >= 0.95
+
+
+def test_saved_tensor_hooks_and_checkpointing(cuda):
+    """What the backward passes need goes through autograd's hooks, and a recomputed forward pass gives the same gradients."""
+    from torch.autograd.graph import save_on_cpu
+    from torch.utils.checkpoint import checkpoint
+    h, w, t = lce_case(60, 48, 500, "bf16", 0.2, cuda)
+    rng = torch.tensor([4, 9], device=cuda)
+    leaves = [v.clone().requires_grad_() for v in (h, torch.randn_like(h), torch.ones(48, device=cuda, dtype=h.dtype), w)]
+
+    def model(x, y, weight, head):
+        x = layers.dropout(x, 0.2, rng)
+        x, normed = layers.residual_norm(x, y, post_norm=True, weight=weight, dropout_p=0.2, seed=rng)
+        return layers.linear_cross_entropy(normed, head, t) + layers.linear_cross_entropy(normed, head, t, reduction="none").sum()
+
+    want = torch.autograd.grad(model(*leaves), leaves)
+    with save_on_cpu():
+        loss = model(*leaves)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, leaves), want))
+    for reentrant in (True, False):
+        again = [v.detach().clone().requires_grad_() for v in leaves]
+        checkpoint(model, *again, use_reentrant=reentrant).backward()
+        assert all(torch.equal(a.grad, b) for a, b in zip(again, want))
+    seen = []
+    x = leaves[0].detach().clone().requires_grad_()
+    y = layers.dropout(x, 0.2, rng)
+    y.register_hook(lambda g: seen.append(1) or 2 * g)
+    got, = torch.autograd.grad(model(y, *leaves[1:]), x)
+    assert seen == [1] and torch.isfinite(got).all()
