@@ -85,12 +85,7 @@ PSGD_DEVI void store_vec(T* p, const float* v) {
   }
 }
 
-// One element of a parameter vector whose type is known at run time (PSGD_F32 / PSGD_BF16 / PSGD_F16).
-PSGD_DEVI float load_any(const void* p, int dtype, long long i) {
-  if (dtype == PSGD_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == PSGD_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return __half2float(reinterpret_cast<const __half*>(p)[i]);
-}
+// One element of a vector whose type is known at run time (PSGD_F32 / PSGD_BF16 / PSGD_F16).
 PSGD_DEVI void store_any(void* p, int dtype, long long i, float v) {
   if (dtype == PSGD_F32) reinterpret_cast<float*>(p)[i] = v;
   else if (dtype == PSGD_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);

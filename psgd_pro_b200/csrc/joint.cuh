@@ -211,8 +211,8 @@ struct Place {
         if (off) out = from_byte(shuffle_up(mine), mine, 16u - off);
         const bool full = at - back + E <= d && (lane > 0 || off == 0);
         if (full) *reinterpret_cast<uint4*>(row + at - back) = out;
-        // The first thread's own elements, the last one's left-over ones, and the row's end (which the last thread may meet
-        // before its left-over ones: those then lie beyond it).
+        // The first thread's own elements, the last one's left-over ones, and the row's end (where the last thread's store is cut
+        // off, nothing is left over).
         const bool rest = full && lane == 31 && off;
         if (!full || rest) {
           const int first = full ? at : at - back, least = full ? E - back : lane > 0 ? 0 : back;
@@ -221,10 +221,6 @@ struct Place {
           for (int k = 0; k < E; ++k)
             if (k >= least && first + k < d) row[first + k] = element(out, k);
         }
-        if (!full && lane == 31 && off)
-#pragma unroll
-          for (int k = 0; k < E; ++k)
-            if (k >= E - back && at + k < d) row[at + k] = element(mine, k);
       }
     }
   }
@@ -898,18 +894,12 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 // with all of a row in registers, which spill, 165 us.)
 template <typename T, bool VEC, bool DIRECT>
 __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJoint j, const JointPlan p, float* part) {
-  constexpr int W = W16_512, F = F_RUNTIME;
-  constexpr int NV = width_nv(W), P = NV * 4;
-  constexpr bool RT = F & F_RUNTIME;
-  const bool post = RT ? j.post != 0 : bool(F & F_POST);
-  const bool gate = RT ? j.gate != nullptr : bool(F & F_GATE);
-  const bool layer = RT ? j.kind == PSGD_NORM_LAYER : bool(F & F_LAYER);
-  const bool drop = RT ? j.threshold != 0 : bool(F & F_DROP);
-  const bool direct = DIRECT;
+  constexpr int W = W16_512, NV = width_nv(W), P = NV * 4;
+  const bool post = j.post != 0, gate = j.gate != nullptr, layer = j.kind == PSGD_NORM_LAYER, drop = j.threshold != 0;
+  constexpr bool direct = DIRECT;
   const bool use_y = post || gate;
   extern __shared__ uint4 smem[];
-  constexpr int NS = RT || (F & F_LAYER) ? 2 : 1;
-  using Sum = GroupSum<NS, width_threads(W) / 32>;
+  using Sum = GroupSum<2, width_threads(W) / 32>;
   __shared__ __align__(16) float red[Sum::FLOATS];
   const int d = j.d, dp = (d + 7) & ~7;
   const Place<T, VEC> at(d);
@@ -917,8 +907,7 @@ __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJ
   Sum sum(red);
   const Keep keep(drop ? j.seed : 0, drop ? j.offset : 0, drop ? j.rng : nullptr, j.threshold);
   const float inv_d = 1.f / (float)d, c = j.scale * (drop ? j.keep_scale : 1.f);
-  constexpr int ARRAYS = RT || (F & (F_POST | F_GATE)) ? 4 : 3;  // d_normed, d_out, out and, where it is needed, y
-  Ring16<T, VEC, NV, ARRAYS> ring(smem, p.stages);
+  Ring16<T, VEC, NV, 4> ring(smem, p.stages);
 
   JointRows it;
   it.groups = blockDim.y, it.direct = direct, it.per_gate = p.per_gate;
