@@ -1,10 +1,10 @@
 // Dropout whose mask is a function of (seed, offset, element index) and is formed again wherever it is needed, so it is
 // never stored: out = [residual +] keep ? x * scale : 0. The backward pass is the same kernel on the gradient.
 //
-// Bound by memory traffic with a residual (46.1M bf16 values: 46.4 us, 5.96 TB/s of 6.46 that a copy has) and by the
-// generator's multiplications without one (16.8M fp16 values: 14.4 us, 4.66 TB/s; the issue slots are 58% busy and the
-// multiplier is what warps wait for). One generator call of ten rounds serves 8 elements; a thread has two calls' data
-// under way (one: 52 us), four blocks an SM (six, with 42 registers, spill: 92 us).
+// Bound by memory traffic with a residual (46.1M bf16 values: 49 to 51 us, 5.5 to 5.6 TB/s of 6.46 that a copy has). Without
+// one (16.8M fp16 values: 16.4 us, 4.1 TB/s) by latency: a thread's loads, its ten dependent rounds and its stores follow each
+// other (the issue slots are 58% busy; the multiplications alone would take some 5 us). One generator call of ten rounds
+// serves 8 elements; a thread has two calls' data under way (one: 49.6 and 18.3 us), four blocks an SM (six: 49.7 and 16.5).
 #include "elem.cuh"
 
 namespace psgd {

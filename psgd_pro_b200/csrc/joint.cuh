@@ -4,7 +4,7 @@
 // + bias. statistics: (mean, 1 / deviation) of post, then of pre, per row.
 //
 // Both passes would be bound by memory traffic (a row in and out once), and the forward pass nearly is (8192 x 2048 bf16,
-// rms norms and a gate: 25 us, 5.3 TB/s of 6.46 that a copy has). About 100 instructions per thread for 8 elements are
+// rms norms and a gate: 28 us, 4.8 TB/s of 6.46 that a copy has; 23.6 us under the profiler). About 100 instructions per thread for 8 elements are
 // what the SMs can issue in the time that the copies take, so arithmetic goes two elements to an instruction
 // (f32x2), everything a call does not have is compiled out, what is constant along a column is kept out of the rows'
 // loop, and a thread has 16 elements, which halves the share of the sums over a row against 8 (46 us, and 28 million
@@ -545,9 +545,9 @@ __global__ void __launch_bounds__(width_threads(W), joint_forward_blocks(W, F)) 
 //   dy = f m, through the post norm as above;  A = sum m yh and B = sum m over rows give
 //   dpost_weight = c gate A, dpost_bias = c gate B, dgate = c (post_weight A + post_bias B): one multiply-add a row for
 //   three gradients. dweight = sum d_normed hat, dbias = sum d_normed.
-// Bound by instructions and their latency (8192 x 2048 bf16, rms norms and a gate: 47.5 us with the last step, of which
-// 41 us here at 54% of the issue slots, 4.9 TB/s; 16384 x 1024, layer norm and dropout: 43 us, the generator being a
-// third of it): five sixths of the instructions are unpacking, the two sums over a row and the multiply-adds that the
+// Bound by the latency of its instructions, and of the two sums over a row that follow each other, with 16 warps on an SM to
+// hide it (8192 x 2048 bf16, rms norms and a gate: 49 us with the last step, of which 41 us here at 54% of the issue slots, 4.9
+// TB/s; 16384 x 1024, layer norm and dropout: 43 us, the generator being a third of it): five sixths of the instructions are unpacking, the two sums over a row and the multiply-adds that the
 // formulas ask for.
 // The sums over rows are kept in registers and written once a block, as rows of `part`, which
 // joint_reduce_kernel adds in a fixed order.
@@ -569,8 +569,8 @@ struct JointRows {  // a group's rows: every groups-th one, or (direct) every gr
 };
 
 // Threads of a block, and blocks that an SM holds, by the registers that a thread needs. Fewer and larger blocks leave fewer
-// sums over rows to the last step, smaller ones even out the SMs (8192 x 2048, rms: 128 threads 49.5 us, 256 47.3, 512 47.2;
-// 16384 x 1024, layer norm with dropout: 44.8, 45.1, 48.7).
+// sums over rows to the last step, smaller ones even out the SMs (8192 x 2048, rms: 128 threads 52.7 us, 256 49.2, 512 48.4;
+// 16384 x 1024, layer norm with dropout: 44.6, 43.2, 47.2).
 PSGD_HD constexpr bool joint_heavy(int f) { return (f & F_RUNTIME) || (f & F_DIRECT) || ((f & F_POST) && (f & F_LAYER)); }
 PSGD_HD constexpr int joint_backward_threads(int w, int f) {
   return w == W8 ? 256 : w == W16 ? ((f & F_LAYER) && (f & F_GATE) && !joint_heavy(f) ? 384 : 256) : width_threads(w);
@@ -890,8 +890,9 @@ __global__ void __launch_bounds__(joint_backward_threads(W, F), joint_backward_b
 
 // Rows of over 4096 elements: 512 threads have 128 registers each, which the sums over rows half fill. The row stays in
 // shared memory and each step of it goes through the thread's elements eight at a time,
-// forming again what the step before had; everything else is as above. (2000 x 8192 bf16, layer norms and a gate: 111 us;
-// with all of a row in registers, which spill, 165 us.)
+// forming again what the step before had; everything else is as above. (2000 x 8192 bf16, layer norms and a gate: 114 us, 27% of
+// a copy's rate, with 32 bytes of a thread spilled; with all of a row in registers 165 us. With gate groups of few rows, whose
+// sums take more registers, 712 bytes are spilled, with unaligned rows 816: 3000 x 4099, a gate a row: 404 us, 8%.)
 template <typename T, bool VEC, bool DIRECT>
 __global__ void __launch_bounds__(512, 1) joint_backward_wide_kernel(const PsgdJoint j, const JointPlan p, float* part) {
   constexpr int W = W16_512, NV = width_nv(W), P = NV * 4;

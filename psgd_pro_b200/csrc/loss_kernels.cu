@@ -12,11 +12,11 @@
 // One pass over the vocabulary with kept exponentials costs 6 N V D operations; forming the logits again for the
 // gradients, the alternative that keeps nothing, costs 8 N V D. What is kept is bounded: tokens are taken in pieces.
 //
-// What bounds it (8192 x 2048 x 32000 bf16, 6144 rows counted, 2.42 TFLOP: 2.2 ms, 1.09 PFLOP/s under the power cap;
+// What bounds it (8192 x 2048 x 32000 bf16, 6144 rows counted, 2.42 TFLOP: 2.15 ms, 1.12 PFLOP/s under the power cap;
 // alone on a cool GPU 600 + 135 + 1100 us in the three long launches): the products by what the SMs can take from L2, 64
 // bytes a clock each, which a 256 x 256 tile of two SMs needs for every 512 clocks of products (13.2 TB/s and 83 to 88% of
-// the tensor pipe at depth 4096, measured); at depth 1024 the tiles' starts and ends cost a third (63 to 67%, the gradients
-// 75%). `rows` moves 4 bytes a logit at 5.9 TB/s. Small calls cost their four launches, 27 us.
+// the tensor pipe at depth 4096, measured); at depth 1024 too, where a tile's results are a larger part of that traffic (12.3
+// TB/s and 63 to 67% of the pipe in the logits, 14.3 and 75% in the gradients). `rows` moves 4 bytes a logit at 5.9 TB/s. Small calls cost their four launches, 27 us.
 #include "elem.cuh"
 #include "pair_rounds.h"
 
@@ -35,7 +35,7 @@ constexpr int L_LIMBS = 3;          // of an fp32 operand
 constexpr int L_GROUP_M = 4;         // row tiles that walk the column tiles together (L2 reuse of both operands)
 constexpr int L_UNIT = 8;            // what a unit costs besides its K blocks (its last step), in K blocks: about 2.5 us
 // Kept exponentials are fp16 of 2^15 exp(l - m), exp(l - m) in [0, 1]: 11 significant bits down to 2^-29 of the row's
-// maximum in these columns (half a tile's), so that the one rounding to 16 bits that matters is that of g.
+// maximum in these columns (half a tile's), so that in bf16 calls the one rounding that matters is that of g.
 constexpr float L_KEEP_SCALE = 32768.f;
 // g is held times 2^8 when it is fp16: p below 2^-14 keeps its bits down to 2^-22 and |g| may reach 255.
 constexpr float L_HALF_SCALE = 256.f;
