@@ -106,7 +106,7 @@ int psgd_gemm_launch(const void* dev_table, const uint32_t* dev_tiles, int ntile
 int psgd_num_sms(void);
 
 /* Device error word bits (*dev_err of every entry point; bits accumulate until the caller clears the word). */
-#define PSGD_ERR_TIMEOUT_FULL 1    /* a wait for a TMA stage (or the wait probe's barrier) gave up */
+#define PSGD_ERR_TIMEOUT_FULL 1    /* a wait for a TMA stage (or the wait probe's barrier; in psgd_lce any wait) gave up */
 #define PSGD_ERR_TIMEOUT_EMPTY 2   /* a wait for a free stage gave up */
 #define PSGD_ERR_TIMEOUT_ACC 4     /* a wait on an accumulator handoff gave up */
 #define PSGD_ERR_BAD_DESC 8        /* a descriptor failed a device-side check */

@@ -279,3 +279,23 @@ def test_saved_tensor_hooks_and_checkpointing(cuda):
     y.register_hook(lambda g: seen.append(1) or 2 * g)
     got, = torch.autograd.grad(model(y, *leaves[1:]), x)
     assert seen == [1] and torch.isfinite(got).all()
+
+
+def test_fp16_losses_by_row_of_one_input_and_in_a_graph(cuda):
+    """Either gradient alone has the bits of both together, and a captured call those of a launched one, for other upstream
+    gradients too."""
+    h, w, t = lce_case(600, 136, 1003, "fp16", 0.2, cuda)
+    up = torch.randn(600, device=cuda) * torch.logspace(-3, 3, 600, device=cuda)
+    want = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none")
+    a, b = h.clone().requires_grad_(), w.clone().requires_grad_()
+    dh, = torch.autograd.grad(layers.linear_cross_entropy(a, w, t, reduction="none"), a, up)
+    dw, = torch.autograd.grad(layers.linear_cross_entropy(h, b, t, reduction="none"), b, up)
+    assert torch.equal(dh, want[1]) and torch.equal(dw, want[2])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none")
+    for turn in range(2):
+        graph.replay()
+        want = layers.linear_cross_entropy_grad(h, w, t, grad=up, reduction="none")
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        up.copy_(up.flip(0) * 3)
