@@ -260,7 +260,9 @@ def residual_norm_grad(d_out: Optional[Tensor], d_normed: Optional[Tensor], out:
                        post_bias=None, gate=None, scale: float = 1.0, eps: float = 1e-6, dropout_p: float = 0.0, seed=0,
                        offset: int = 0) -> ResidualNormGrads:
     """Gradients of residual_norm's inputs from those of its outputs (None: zero), its output `out`, its input y and the
-    stats of the forward call with the same options."""
+    stats of the forward call with the same options. The stats are those of the sum before its rounding to `out`, which is
+    what the second norm is formed again from here: a 16-bit residual stream whose mean is far above its deviation has the
+    gradients of that rounding."""
     s, rows, pd, keep = _joint_spec(out, y, norm, post_norm, weight, bias, post_weight, post_bias, gate, scale, eps,
                                     dropout_p, seed, offset)
     d, device, shape = s.d, out.get_device(), out.shape
